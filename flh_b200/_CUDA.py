@@ -344,6 +344,147 @@ def rope_kv(qkv, cos, sin, q_out, k_cache, v_cache, B, S, nh, nkv, cur, q_by_tok
     return q_out
 
 
+# ---- a KV cache that is drafted into and evicted from (include/flh_b200.h): sequences with lengths of their own, a tree of drafted
+# tokens behind each of them.  lengths, positions, tree, path and accepted are tensors on the device: what they hold is read when the
+# work runs, also when a recorded graph is replayed.
+_TREE_MAX, _CACHE_MAX_LAYERS = 64, 128
+
+
+def _check_caches(k, v, name="k_cache"):
+    _check(k.dim() == 4 and v.shape == k.shape, f"{name} and its v must be [B, kv heads, T, D] of the same shape")
+    _check(k.dtype in (torch.float16, torch.bfloat16) and v.dtype == k.dtype, f"{name} and its v must both be float16 or bfloat16")
+    _check(k.is_contiguous() and v.is_contiguous(), f"{name} and its v must be contiguous")
+
+
+def _check_ints(t, shape, name):
+    _check(t.dtype == torch.int32 and tuple(t.shape) == shape and t.is_contiguous(), f"{name} must be contiguous int32 {list(shape)}")
+
+
+def _check_device(first, *others):
+    _check(first.is_cuda, "tensors must be CUDA")
+    _check(all(t is None or t.device == first.device for t in others), "tensors must be on one device")
+
+
+def rope_kv_at(qkv, cos, sin, positions, lengths, k_cache, v_cache, nh):
+    """rope_kv for drafted tokens: token s of sequence b is turned by row positions[b, s] of the tables and its k and v go to entry
+    lengths[b] + s of the caches [B, nkv, T, D]; entries T and up do not exist.  qkv [B*S, (nh + 2 nkv) * D] contiguous, float16 or
+    bfloat16; cos, sin f32 [P, D/2]; positions int32 [B, S]; lengths int32 [B].  -> q [B, S, nh, D].  A position that the tables
+    do not have makes that token's q and k NaN."""
+    _check_caches(k_cache, v_cache)
+    B, nkv, T, D = k_cache.shape
+    _check(positions.dim() == 2, "positions must be int32 [B, S]")
+    S = positions.shape[1]
+    _check_ints(positions, (B, S), "positions")
+    _check_ints(lengths, (B,), "lengths")
+    _check(qkv.dtype == k_cache.dtype and qkv.is_contiguous() and tuple(qkv.shape) == (B * S, (nh + 2 * nkv) * D), "qkv must be contiguous [B*S, (nh + 2 nkv) * D] of the caches' type")
+    _check(cos.dtype == torch.float32 and cos.is_contiguous() and cos.dim() == 2 and cos.shape[1] * 2 == D, "cos must be contiguous float32 [P, D/2]")
+    _check(sin.dtype == torch.float32 and sin.is_contiguous() and sin.shape == cos.shape, "sin must be contiguous float32 [P, D/2]")
+    _check_device(qkv, cos, sin, positions, lengths, k_cache, v_cache)
+    q = torch.empty((B, S, nh, D), dtype=qkv.dtype, device=qkv.device)
+    with _guard(qkv.device):
+        _lib.check(_lib.load().flh_b200_rope_kv_at(_ptr(qkv), BF16 if qkv.dtype == torch.bfloat16 else F16, _ptr(cos), _ptr(sin), cos.shape[0], _ptr(positions),
+                                                   _ptr(lengths), _ptr(q), _ptr(k_cache), _ptr(v_cache), B, S, nh, nkv, D, T, _stream(qkv)), "rope_kv_at")
+    return q
+
+
+def tree_attention(q, k_cache, v_cache, lengths, tree=None, weights=None, scale=None):
+    """Attention of S = 1 .. 64 drafted tokens of every sequence over a cache: token (b, s) sees entries 0 .. lengths[b] - 1 and, of the
+    drafted entries lengths[b] + j, those whose bit j is set in tree[b, s].  q [B, S, nh, D] (any strides that are multiples of
+    8 elements, the last dimension contiguous), caches [B, nkv, T, D], D 64 or 128, all float16 or all bfloat16; nh a multiple of
+    nkv; lengths int32 [B]; tree int64 [S] or [B, S], or None for a chain (S = 1: ordinary decode).  scale: 1 / sqrt(D) by default.
+    weights (f32 [B, nkv, T]): to every entry is added what all tokens and heads of the group gave it, what
+    cache_evict goes by.  -> [B, S, nh, D].  A token that sees no entry has zeros."""
+    _check_caches(k_cache, v_cache)
+    B, nkv, T, D = k_cache.shape
+    _check(q.dim() == 4 and q.shape[0] == B and q.shape[3] == D, "q must be [B, S, heads, D] for caches [B, kv heads, T, D]")
+    S, nh = q.shape[1], q.shape[2]
+    _check(q.dtype == k_cache.dtype, "q must have the caches' type")
+    _check(1 <= S <= _TREE_MAX, f"q must have 1 .. {_TREE_MAX} tokens")
+    _check(nkv > 0 and nh > 0 and nh % nkv == 0, "the heads of q must be a multiple of the kv heads")
+    _check(D in (64, 128), "the head size must be 64 or 128")
+    _check(q.stride(3) == 1 and all(st % 8 == 0 for st, n in zip(q.stride()[:3], q.shape) if n > 1), "the last dimension of q must be contiguous, its other strides multiples of 8")
+    _check_ints(lengths, (B,), "lengths")
+    _check(tree is None or (tree.dtype == torch.int64 and tree.is_contiguous() and tuple(tree.shape) in ((S,), (B, S))), "tree must be contiguous int64 [S] or [B, S]")
+    _check(weights is None or (weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == (B, nkv, T)), "weights must be contiguous float32 [B, kv heads, T]")
+    _check_device(q, k_cache, v_cache, lengths, tree, weights)
+    out = torch.empty((B, S, nh, D), dtype=q.dtype, device=q.device)
+    sb, ss, sh = (st if n > 1 else 0 for st, n in zip(q.stride()[:3], q.shape))
+    lib = _lib.load()
+    with _guard(q.device):
+        ws = _scratch(q.device, max(16, lib.flh_b200_tree_attention_workspace_bytes(B, S, nh, nkv, D, T, weights is not None)))
+        _lib.check(lib.flh_b200_tree_attention(
+            _ptr(q), sb, ss, sh, BF16 if q.dtype == torch.bfloat16 else F16, _ptr(k_cache), _ptr(v_cache), _ptr(lengths), _ptr(tree),
+            0 if tree is None or tree.dim() == 1 else S, 1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(out), _ptr(weights), B, S, nh, nkv, D, T,
+            _ptr(ws), ws.numel(), _stream(q)), "tree_attention")
+    return out
+
+
+def tree_attention_status():
+    """[code, cta, 0, 0] of the attention's bounded waits; synchronises.  0 = clean."""
+    out = (ctypes.c_int * 4)()
+    _lib.check(_lib.load().flh_b200_tree_attention_status(out), "tree_attention_status")
+    return list(out)
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _check_layers(k_caches, v_caches, weights, lengths):
+    _check(1 <= len(k_caches) <= _CACHE_MAX_LAYERS and len(v_caches) == len(k_caches) and (weights is None or len(weights) == len(k_caches)),
+           f"k, v and weights must be lists of the same 1 .. {_CACHE_MAX_LAYERS} layers")
+    first = k_caches[0]
+    _check(first.dim() == 4 and first.dtype in (torch.float16, torch.bfloat16), "caches must be [B, kv heads, T, D], float16 or bfloat16")
+    for t in (*k_caches, *v_caches):
+        _check(t.shape == first.shape and t.dtype == first.dtype and t.is_contiguous(), "the caches of all layers must be contiguous and alike")
+    for t in weights or ():
+        _check(t.shape == first.shape[:3] and t.dtype == torch.float32 and t.is_contiguous(), "weights must be contiguous float32 [B, kv heads, T]")
+    B, nkv, T, D = first.shape
+    _check(D % 8 == 0 and 8 <= D <= 256, "the head size must be a multiple of 8 up to 256")
+    _check(T > 0, "the caches must have entries")
+    _check_ints(lengths, (B,), "lengths")
+    return B, nkv, T, D, BF16 if first.dtype == torch.bfloat16 else F16
+
+
+def cache_accept(k_caches, v_caches, lengths, path, accepted, drafted, weights=None):
+    """The accepted branch of a tree of `drafted` tokens, in the caches of all layers (lists of [B, nkv, T, D]) by one launch: for i <
+    accepted[b] entry lengths[b] + path[b, i] moves to lengths[b] + i (path int32 [B, A], accepted int32 [B]), in place and as if
+    all were read before any is written.  An index outside 0 .. drafted - 1 leaves entry i as it is.  weights (a list of f32 [B, nkv, T]): moved along, and zero for the drafted
+    entries behind the accepted ones.  -> the new lengths, lengths + accepted (int32 [B])."""
+    B, nkv, T, D, dtype = _check_layers(k_caches, v_caches, weights, lengths)
+    _check(1 <= drafted <= _TREE_MAX, f"drafted must be 1 .. {_TREE_MAX}")
+    _check(path.dim() == 2 and path.shape[1] <= drafted, "path must be int32 [B, A] with A <= drafted")
+    _check_ints(path, (B, path.shape[1]), "path")
+    _check_ints(accepted, (B,), "accepted")
+    _check_device(lengths, path, accepted, *k_caches, *v_caches, *(weights or ()))
+    now = torch.empty_like(lengths)
+    with _guard(lengths.device):
+        _lib.check(_lib.load().flh_b200_cache_accept(
+            _pointers(k_caches), _pointers(v_caches), None if weights is None else _pointers(weights), len(k_caches), dtype, _ptr(lengths), _ptr(path),
+            _ptr(accepted), _ptr(now), B, nkv, D, T, path.shape[1], int(drafted), _stream(lengths)), "cache_accept")
+    return now
+
+
+def cache_evict(k_caches, v_caches, weights, lengths, keep, recent):
+    """Down to `keep` entries a head, in the caches of all layers (lists of [B, nkv, T, D]): where a sequence has more, its last `recent`
+    stay and, of the others, the keep - recent with the largest weights (lists of f32 [B, nkv, T]; NaN is the largest, ties go to the
+    lower index).  What stays moves together in order, in place.  -> (kept int32 [layers, B, nkv, keep]: the entries that
+    stayed, -1 behind the last; their weights f32 [layers, B, nkv, T], 0 behind the last; the new lengths int32 [B])."""
+    _check(weights is not None, "weights must be lists of float32 [B, kv heads, T]")
+    B, nkv, T, D, dtype = _check_layers(k_caches, v_caches, weights, lengths)
+    _check(1 <= keep <= T and 0 <= recent <= keep, "keep must be 1 .. T and recent 0 .. keep")
+    _check_device(lengths, *k_caches, *v_caches, *weights)
+    L, dev = len(k_caches), lengths.device
+    kept = torch.empty((L, B, nkv, keep), dtype=torch.int32, device=dev)
+    left = torch.empty((L, B, nkv, T), dtype=torch.float32, device=dev)
+    now = torch.empty_like(lengths)
+    with _guard(dev):
+        _lib.check(_lib.load().flh_b200_cache_evict(
+            _pointers(k_caches), _pointers(v_caches), _pointers(weights), L, dtype, _ptr(lengths), int(keep), int(recent), _ptr(kept), _ptr(left), _ptr(now),
+            B, nkv, D, T, _stream(lengths)), "cache_evict")
+    return kept, left, now
+
+
 def rmsnorm_quant_token_asym_i4(x, eps: float, hadamard: bool = False, clip: float = 1.0):
     """RMS-norm (weight 1) + per-token asymmetric int4 in one pass, K = 4096 or 8192 (include/flh_b200.h).
     x [M, K] f16/bf16 (row stride allowed) -> (q u8[M,K/2], scale f16[M], zero f16[M])."""

@@ -32,6 +32,16 @@ SIGNATURES = {
                                      c_int, c_int, c_void_p]),
     "flh_b200_rope_kv_by_token_f16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                      c_int, c_int, c_void_p]),
+    "flh_b200_rope_kv_at": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                                    c_int, c_int, c_long, c_void_p]),
+    "flh_b200_tree_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_long, c_int]),
+    "flh_b200_tree_attention": (c_int, [c_void_p, c_long, c_long, c_long, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_float, c_void_p,
+                                        c_void_p, c_int, c_int, c_int, c_int, c_int, c_long, c_void_p, c_size_t, c_void_p]),
+    "flh_b200_tree_attention_status": (c_int, [c_void_p]),
+    "flh_b200_cache_accept": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_long,
+                                      c_int, c_int, c_void_p]),
+    "flh_b200_cache_evict": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                     c_int, c_long, c_void_p]),
     "flh_b200_gptq_block": (c_int, [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int,
                                     c_float, c_void_p, c_long, c_void_p, c_void_p]),
     "flh_b200_sign_table_bytes": (c_size_t, [c_int]),

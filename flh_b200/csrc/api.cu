@@ -1,6 +1,6 @@
 // C ABI of libflh_b200.so: argument validation, error strings, algorithm choice.
 // Every entry point only enqueues work on the caller's stream.
-#include "common.cuh"
+#include "attn_common.cuh"
 #include <string.h>
 
 namespace flh {
@@ -64,6 +64,16 @@ int launch_silu_mul(const void *, int, long, long, long, void *, cudaStream_t);
 int launch_square(const void *, int, long, void *, cudaStream_t);
 int launch_silu_mul_quant_token_tc(const void *, int, long, long, long, int, const uint32_t *, float, uint8_t *, void *, void *, cudaStream_t);
 int launch_rope_kv(const void *, const float *, const float *, void *, void *, void *, int, int, int, int, int, int, int, int, cudaStream_t);
+int launch_rope_kv_at(const void *, int, const float *, const float *, long, const int32_t *, const int32_t *, void *, void *, void *, int, int, int, int,
+                      int, long, cudaStream_t);
+int launch_cache_accept(void *const *, void *const *, float *const *, int, const int32_t *, const int32_t *, const int32_t *, int32_t *, int, int, int, long,
+                        int, int, cudaStream_t);
+int launch_cache_evict(void *const *, void *const *, const float *const *, int, const int32_t *, int32_t *, float *, int32_t *, int, int, int, long, int, int,
+                       cudaStream_t);
+size_t tree_attention_workspace_bytes(int, int, int, int, int, long, bool);
+int launch_tree_attention(TreeAttnParams, bool, uint8_t *, cudaStream_t);
+int attn_tree_status(int *);
+int attn_tree_status_clear();
 int quant_token_tc_status(int *);
 int launch_gptq_block(const float *, long, const float *, long, const float *, const float *, long, const int *, long, int, int, int,
                       float, float *, long, float *, cudaStream_t);
@@ -256,6 +266,94 @@ int flh_b200_rope_kv_f16(const void *qkv, const float *cos, const float *sin, vo
 int flh_b200_rope_kv_by_token_f16(const void *qkv, const float *cos, const float *sin, void *q_out, void *k_cache, void *v_cache,
                                   int B, int S, int nh, int nkv, int D, int T, int cur, void *stream) {
     return rope_kv(qkv, cos, sin, q_out, k_cache, v_cache, B, S, nh, nkv, D, T, cur, 1, stream);
+}
+
+static bool tree_shape(int B, int S, int nh, int nkv, int D, long T) {
+    return B >= 0 && S >= 1 && S <= FLH_B200_TREE_MAX_TOKENS && nkv > 0 && nh > 0 && nh % nkv == 0 && (D == 64 || D == 128) && T >= 1 && T <= 1L << 21;
+}
+
+int flh_b200_rope_kv_at(const void *qkv, int dtype, const float *cos, const float *sin, long P, const int32_t *positions, const int32_t *lengths,
+                        void *q_out, void *k_cache, void *v_cache, int B, int S, int nh, int nkv, int D, long T, void *stream) {
+    FLH_REQUIRE(dtype == FLH_B200_F16 || dtype == FLH_B200_BF16, FLH_B200_EINVAL, "bad dtype %d", dtype);
+    FLH_REQUIRE(B >= 0 && S >= 0 && nh > 0 && nkv > 0 && D > 0 && D % 16 == 0 && T >= 0 && P >= 0, FLH_B200_EINVAL, "bad shape B=%d S=%d nh=%d nkv=%d D=%d T=%ld", B, S,
+                nh, nkv, D, T);
+    FLH_REQUIRE((long)B * S < 1L << 31 && ((long)nh + 2L * nkv) * D < 1L << 31, FLH_B200_EINVAL, "too many tokens or heads");
+    if (B == 0 || S == 0) return 0;
+    FLH_REQUIRE(qkv && cos && sin && positions && lengths && q_out && k_cache && v_cache, FLH_B200_EINVAL, "null pointer");
+    FLH_REQUIRE(aligned16(qkv) && aligned16(cos) && aligned16(sin) && aligned16(q_out) && aligned16(k_cache) && aligned16(v_cache), FLH_B200_EALIGN,
+                "pointers must be 16-byte aligned");
+    return launch_rope_kv_at(qkv, dtype, cos, sin, P, positions, lengths, q_out, k_cache, v_cache, B, S, nh, nkv, D, T, static_cast<cudaStream_t>(stream));
+}
+
+size_t flh_b200_tree_attention_workspace_bytes(int B, int S, int nh, int nkv, int D, long T, int with_weights) {
+    return tree_shape(B, S, nh, nkv, D, T) && B ? tree_attention_workspace_bytes(B, S, nh, nkv, D, T, with_weights != 0) : 0;
+}
+
+int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache, const int32_t *lengths,
+                            const int64_t *tree, long tree_stride, float scale, void *out, float *weights, int B, int S, int nh, int nkv, int D, long T,
+                            void *ws, size_t ws_bytes, void *stream) {
+    FLH_REQUIRE(dtype == FLH_B200_F16 || dtype == FLH_B200_BF16, FLH_B200_EINVAL, "bad dtype %d", dtype);
+    FLH_REQUIRE(tree_shape(B, S, nh, nkv, D, T), FLH_B200_EINVAL, "bad shape B=%d S=%d nh=%d nkv=%d D=%d T=%ld (S 1 .. 64, D 64 or 128, nh a multiple of nkv)", B, S, nh, nkv,
+                D, T);
+    // every count of tiles, rows and blocks stays within 31 bits
+    FLH_REQUIRE((long)S * (nh / nkv) <= 1L << 20 && (long)B * nkv < 1L << 26 && (long)B * nkv * (((long)S * (nh / nkv) + 15) / 16) * ((T + 31) / 32) < 1L << 31 &&
+                (long)B * nh * S < 1L << 31, FLH_B200_EINVAL, "too many sequences, heads or entries: B=%d S=%d nh=%d T=%ld", B, S, nh, T);
+    FLH_REQUIRE(scale > 0.0f && scale <= 3.0e38f, FLH_B200_EINVAL, "scale must be positive and finite");
+    FLH_REQUIRE(q_sb % 8 == 0 && q_ss % 8 == 0 && q_sh % 8 == 0, FLH_B200_EALIGN, "strides of q must be multiples of 8 elements");
+    FLH_REQUIRE(tree_stride == 0 || tree_stride == S, FLH_B200_EINVAL, "tree must be [S] or [B, S]");
+    if (B == 0) return 0;
+    FLH_REQUIRE(q && k_cache && v_cache && lengths && out, FLH_B200_EINVAL, "null pointer");
+    FLH_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && aligned16(ws), FLH_B200_EALIGN, "pointers must be 16-byte aligned");
+    FLH_REQUIRE(ws && ws_bytes >= tree_attention_workspace_bytes(B, S, nh, nkv, D, T, weights != nullptr), FLH_B200_EINVAL, "workspace of %zu bytes is too small", ws_bytes);
+    TreeAttnParams p = {};
+    p.q = q; p.q_sb = q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
+    p.lengths = lengths; p.tree = tree; p.tree_sb = tree_stride;
+    p.k = k_cache; p.v = v_cache; p.out = out; p.weights = weights;
+    p.B = B; p.S = S; p.nh = nh; p.nkv = nkv; p.D = D; p.T = (int)T;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    return launch_tree_attention(p, dtype == FLH_B200_BF16, static_cast<uint8_t *>(ws), static_cast<cudaStream_t>(stream));
+}
+
+int flh_b200_tree_attention_status(int *out) {
+    FLH_REQUIRE(out, FLH_B200_EINVAL, "null pointer");
+    const int rc = attn_tree_status(out);
+    return rc || !out[0] ? rc : attn_tree_status_clear();
+}
+
+static int cache_shape(int layers, int dtype, int B, int nkv, int D, long T) {
+    FLH_REQUIRE(dtype == FLH_B200_F16 || dtype == FLH_B200_BF16, FLH_B200_EINVAL, "bad dtype %d", dtype);
+    FLH_REQUIRE(layers >= 1 && layers <= FLH_B200_CACHE_MAX_LAYERS, FLH_B200_EINVAL, "layers must be 1 .. %d", FLH_B200_CACHE_MAX_LAYERS);
+    FLH_REQUIRE(B >= 0 && nkv > 0 && D >= 8 && D % 8 == 0 && D <= 256 && T >= 1 && T <= 1L << 30 && (long)B * nkv < 1L << 24, FLH_B200_EINVAL,
+                "bad shape B=%d nkv=%d D=%d T=%ld (D a multiple of 8 up to 256)", B, nkv, D, T);
+    return 0;
+}
+
+int flh_b200_cache_accept(void *const *k, void *const *v, float *const *w, int layers, int dtype, const int32_t *lengths, const int32_t *path,
+                          const int32_t *accepted, int32_t *now, int B, int nkv, int D, long T, int A, int drafted, void *stream) {
+    const int rc = cache_shape(layers, dtype, B, nkv, D, T);
+    if (rc) return rc;
+    FLH_REQUIRE(drafted >= 1 && drafted <= FLH_B200_TREE_MAX_TOKENS && A >= 0 && A <= drafted, FLH_B200_EINVAL, "drafted must be 1 .. 64 and the path no longer: %d, %d", drafted, A);
+    if (B == 0) return 0;
+    FLH_REQUIRE(k && v && lengths && (path || A == 0) && accepted && now != lengths, FLH_B200_EINVAL, "null pointer, or now is lengths");
+    for (int i = 0; i < layers; ++i) {
+        FLH_REQUIRE(k[i] && v[i] && (!w || w[i]), FLH_B200_EINVAL, "null pointer in layer %d", i);
+        FLH_REQUIRE(aligned16(k[i]) && aligned16(v[i]), FLH_B200_EALIGN, "caches must be 16-byte aligned");
+    }
+    return launch_cache_accept(k, v, w, layers, lengths, path, accepted, now, B, nkv, D, T, A, drafted, static_cast<cudaStream_t>(stream));
+}
+
+int flh_b200_cache_evict(void *const *k, void *const *v, const float *const *w, int layers, int dtype, const int32_t *lengths, int keep, int recent,
+                         int32_t *kept, float *left, int32_t *now, int B, int nkv, int D, long T, void *stream) {
+    const int rc = cache_shape(layers, dtype, B, nkv, D, T);
+    if (rc) return rc;
+    FLH_REQUIRE(keep >= 1 && keep <= T && recent >= 0 && recent <= keep, FLH_B200_EINVAL, "keep must be 1 .. T and recent 0 .. keep: %d, %d", keep, recent);
+    if (B == 0) return 0;
+    FLH_REQUIRE(k && v && w && lengths && kept && left && now && now != lengths, FLH_B200_EINVAL, "null pointer, or now is lengths");
+    for (int i = 0; i < layers; ++i) {
+        FLH_REQUIRE(k[i] && v[i] && w[i], FLH_B200_EINVAL, "null pointer in layer %d", i);
+        FLH_REQUIRE(aligned16(k[i]) && aligned16(v[i]), FLH_B200_EALIGN, "caches must be 16-byte aligned");
+    }
+    return launch_cache_evict(k, v, w, layers, lengths, kept, left, now, B, nkv, D, T, keep, recent, static_cast<cudaStream_t>(stream));
 }
 
 const char *flh_b200_quant_token_kernel(long M, long K, int hadamard, int kfac) {

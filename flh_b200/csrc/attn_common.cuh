@@ -1,0 +1,145 @@
+// What the kernels of the attention over a cache with drafted entries share: the order of the work, the visibility of entries, and
+// the join of partial results.
+//
+// Rows: the S drafted tokens of a sequence times the g query heads that share a kv head are R = S g rows over the same keys;
+// row r is token r / g, head r % g of the group.  A job is a block of rows of one (sequence, kv head); its keys come in tiles.  All
+// tiles of all jobs in a row (sequence, then head, then block of rows) are cut into equal shares, one for each CTA, wherever the
+// cuts fall: a batch of uneven lengths is as balanced as one long sequence, and the lengths are read on the device, so that a
+// recorded launch follows them.  A job that lies within one share is finished there; of a job that was cut each CTA
+// writes a partial result (sum of exponentials, maximum, weighted sum of V) to a slot of its own and the join kernel adds them in order.
+#pragma once
+#include "tc_common.cuh"
+
+namespace flh {
+
+struct TreeAttnParams {
+    const void *q;
+    long q_sb, q_ss, q_sh;                 // strides in elements; the head's values are contiguous
+    const int32_t *lengths;
+    const int64_t *tree;                   // ancestor bits [S] or [B, S]; null: a chain
+    long tree_sb;
+    const void *k, *v;                     // [B, nkv, T, D]
+    void *out;                             // [B, S, nh, D]
+    float *weights;                        // [B, nkv, T], added to; or null
+    int B, S, nh, nkv, g, D, R, nrb;       // nrb: blocks of rows
+    int T;
+    float scale_log2;                      // scale * log2(e): scores live in powers of two
+    int shares, min_share;                 // CTAs, tiles that a share has at least
+    float *part_o;                         // [2 shares][rows of a block][D]
+    float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
+    float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
+    float *scores;                         // [B, nkv, R, score_ld] (with weights and few rows), or null
+    long score_ld;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ int committed(const TreeAttnParams &p, int b) { return min(max(p.lengths[b], 0), p.T); }
+__device__ __forceinline__ int entries(const TreeAttnParams &p, int len) { return min(len + p.S, p.T); }    // len <= T < 2^30
+
+// The drafted entries that a token sees, as bits; those behind the end of the cache do not exist.
+__device__ __forceinline__ uint64_t drafted_bits(const TreeAttnParams &p, int b, int s, int len) {
+    const int n = entries(p, len) - len;
+    const uint64_t exist = n >= 64 ? ~0ull : (1ull << n) - 1;
+    return exist & (p.tree ? (uint64_t)p.tree[b * p.tree_sb + s] : ~0ull >> (63 - s));
+}
+
+// Tiles of all jobs up to sequence b (exclusive); warp-uniform.  upto = B: all of them.
+template <int TILE>
+__device__ __forceinline__ int tiles_before(const TreeAttnParams &p, int upto, int lane) {
+    int sum = 0;
+    for (int i = lane; i < upto; i += 32) sum += (entries(p, committed(p, i)) + TILE - 1) / TILE;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum * p.nkv * p.nrb;
+}
+__device__ __forceinline__ int share_tiles(const TreeAttnParams &p, int total) { return max((total + p.shares - 1) / p.shares, p.min_share); }
+
+// A walk over jobs in order: the job that holds a tile.
+template <int TILE>
+struct JobWalk {
+    int b, job, nt, len, begin;            // sequence; job within the sequence (head * nrb + block of rows); its tiles; first tile
+    // from the start of the order to the job of tile u (u < total); warp-uniform
+    __device__ void seek(const TreeAttnParams &p, int u, int lane) {
+        const int per = p.nkv * p.nrb;
+        int base = 0, b0 = 0;
+        for (;;) {                         // 32 sequences at a time
+            const int i = b0 + lane;
+            const int mine = i < p.B ? (entries(p, committed(p, i)) + TILE - 1) / TILE * per : 0;
+            int incl = mine;
+            for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += t; }
+            const unsigned over = __ballot_sync(0xffffffffu, base + incl > u);
+            if (over || b0 + 32 >= p.B) {
+                const int l = over ? __ffs(over) - 1 : 31;
+                b = min(b0 + l, p.B - 1);
+                base += __shfl_sync(0xffffffffu, incl - mine, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
+            b0 += 32;
+        }
+        len = committed(p, b);
+        nt = (entries(p, len) + TILE - 1) / TILE;
+        job = (u - base) / nt;
+        begin = base + job * nt;
+    }
+    __device__ __forceinline__ void next(const TreeAttnParams &p) {
+        begin += nt;
+        if (++job == p.nkv * p.nrb) {
+            job = 0;
+            if (++b < p.B) {
+                len = committed(p, b);
+                nt = (entries(p, len) + TILE - 1) / TILE;
+            } else {
+                b = p.B;                   // behind the last job: no tile comes here
+                nt = 1 << 30;
+            }
+        }
+    }
+};
+
+// Two 16-bit values of the tensors' type as binary32, and back.
+template <bool BF16> __device__ __forceinline__ float2 widen(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+template <bool BF16> __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
+    if (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <bool BF16> __device__ __forceinline__ float load16(const void *p, long i) {
+    if (BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+    return __half2float(static_cast<const __half *>(p)[i]);
+}
+template <bool BF16> __device__ __forceinline__ void store16(void *p, long i, float x) {
+    if (BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
+    else static_cast<__half *>(p)[i] = __float2half_rn(x);
+}
+template <bool BF16> __device__ __forceinline__ bool nonfinite16(uint16_t u) { return BF16 ? (u & 0x7f80u) == 0x7f80u : (u & 0x7c00u) == 0x7c00u; }
+
+// 1 / l of a row whose exponentials sum to l, as the factor of its weighted sum.  A row that sees nothing is zero; one whose scores
+// are all -inf is NaN, as a softmax has it.
+__device__ __forceinline__ float row_factor(float l, bool empty) { return l == 0.0f && empty ? 0.0f : 1.0f / l; }
+
+// What the values of drafted entries that are not finite add to one element of the weighted sum of a row: they are kept out of
+// the matrix product, where a weight of zero would still make them NaN for rows that do not see them.  bad: those entries; m: the
+// maximum that the sum is relative to.
+template <bool BF16>
+__device__ __noinline__ float nonfinite_part(const TreeAttnParams &p, uint64_t bad, uint64_t seen, int b, int kvh, int row, int d, int len, float m) {
+    const long q0 = b * p.q_sb + (row / p.g) * p.q_ss + (long)(kvh * p.g + row % p.g) * p.q_sh;
+    float sum = 0.0f;
+    for (uint64_t left = bad & seen; left; left &= left - 1) {
+        const long at = (((long)b * p.nkv + kvh) * p.T + len + __ffsll((long long)left) - 1) * p.D;
+        const float x = load16<BF16>(p.v, at + d);
+        if (fabsf(x) <= 3.4e38f) continue;
+        float dot = 0.0f;
+        for (int i = 0; i < p.D; ++i) dot = fmaf(load16<BF16>(p.q, q0 + i), load16<BF16>(p.k, at + i), dot);
+        sum += exp2_approx(fmaf(dot, p.scale_log2, -m)) * x;
+    }
+    return sum;
+}
+
+}  // namespace flh

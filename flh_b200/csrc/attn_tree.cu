@@ -1,0 +1,552 @@
+// Attention of drafted tokens over a KV cache whose sequences have lengths of their own, and its accumulated weights.
+//
+//   o[b, s, h] = sum_t p[t] v[b, h / g, t],  p = softmax over the entries t that token s sees of scale * q[b, s, h] . k[b, h / g, t]
+//   weights[b, kvh, t] += sum over s and the heads of the group of p[t]
+//
+// Token s of sequence b sees every committed entry (t < lengths[b]) and, of the drafted ones (t = lengths[b] + j, j < S), those
+// whose bit j is set in tree[b, s]; S = 1 is ordinary decode.
+//
+// A pass reads K and V once: 4 D bytes an entry against 4 R D operations (R = S g rows share a kv head's entries), so that up to a few
+// dozen rows the memory is what bounds it.  attn_mma_kernel is built for that: every warp streams key tiles of its own through a ring
+// of TMA loads in shared memory, keeps the running maximum and sum of its rows in registers and needs no other warp until its
+// share of a job ends (mma.sync: 16 rows by 8 keys by 16 values; the tensor cores are at a fraction of their rate).
+#include "attn_common.cuh"
+#include "tc_pair.cuh"
+
+namespace flh {
+namespace {
+
+__device__ int g_status_attn[4];
+
+constexpr int kTile = 32;                  // keys of a tile
+constexpr int kWarps = 4, kThreadsAttn = kWarps * 32;
+
+template <int MT> constexpr int ring_slots() { return MT == 1 ? 3 : 2; }    // of a warp, so that two CTAs fit an SM; a slot is the K or the V part of a tile
+template <int D> constexpr int slot_bytes() { return kTile * D * 2; }
+template <int D, int MT> constexpr int q_pitch() { return D * 2 + 16; }                       // bytes; the 16 keep ldmatrix free of conflicts
+template <int D, int MT> constexpr int attn_smem() { return 1024 + kWarps * ring_slots<MT>() * slot_bytes<D>() + 16 * MT * q_pitch<D, MT>() + kWarps * 16 * MT * 32 * 4; }
+
+__device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 rows of 8-byte pieces: where piece (row, 16-byte chunk) of a tile of 128-byte swizzled rows lies
+template <int ROWS> __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
+    return (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// MT: blocks of 16 rows of a job.
+template <int D, int MT, bool BF16>
+__global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap,
+                                                                   const __grid_constant__ CUtensorMap vmap) {
+    constexpr int kRows = 16 * MT, kNT = kTile / 8, kKS = D / 16, kDT = D / 8, kSlot = slot_bytes<D>(), kSlots = ring_slots<MT>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sm_q = smem + kWarps * kSlots * kSlot;
+    float *sm_o = reinterpret_cast<float *>(sm_q + kRows * q_pitch<D, MT>());      // [warp][row][32 columns]
+    __shared__ uint64_t full[kWarps][kSlots];
+    __shared__ uint64_t seen[kRows];
+    __shared__ unsigned long long bad;
+    __shared__ float sm_m[kWarps][kRows], sm_l[kWarps][kRows];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3;
+    uint8_t *ring = smem + warp * kSlots * kSlot;
+    const uint32_t ring_u = smem_u32(ring), full_u = smem_u32(&full[warp][0]);
+    if (lane == 0)
+        for (int i = 0; i < kSlots; ++i) mbar_init(full_u + 8 * i, 1);
+    if (tid == 0) { abort_flag = 0; bad = 0; }
+    fence_proxy_async();
+    __syncthreads();
+    pdl_wait();
+    pdl_trigger();
+
+    const int total = tiles_before<kTile>(p, p.B, lane), share = share_tiles(p, total);
+    const long first = (long)blockIdx.x * share;
+    if (first >= total) return;
+    const int u0 = (int)first, u1 = (int)min((long)total, first + share);
+    JobWalk<kTile> cur, ahead;             // the job worked on, and the one that the loads have come to
+    cur.seek(p, u0, lane);
+    ahead = cur;
+
+    // item i of this warp: K (i even) or V (i odd) of its tile i / 2, into slot i % kSlots
+    int u_ahead = u0 + warp, item = 0;
+    auto issue = [&]() {
+        if (u_ahead >= u1) return;
+        while (u_ahead >= ahead.begin + ahead.nt) ahead.next(p);
+        if (lane == 0) {
+            const uint32_t bar = full_u + 8 * (item % kSlots), dst = ring_u + (item % kSlots) * kSlot;
+            const CUtensorMap *map = item & 1 ? &vmap : &kmap;
+            mbar_expect_tx(bar, kSlot);
+            for (int h = 0; h < D / 64; ++h)
+                tma_load_tile(dst + h * (kTile * 128), map, h * 64, (u_ahead - ahead.begin) * kTile, ahead.b * p.nkv + ahead.job / p.nrb, bar);
+        }
+        if (item & 1) u_ahead += kWarps;
+        ++item;
+    };
+    for (int i = 0; i < kSlots; ++i) issue();
+    int used = 0;                          // items taken from the ring
+    bool alive = true;
+
+    for (int piece = u0; piece < u1;) {
+        while (piece >= cur.begin + cur.nt) cur.next(p);
+        const int piece_end = min(u1, cur.begin + cur.nt);
+        const int b = cur.b, kvh = cur.job / p.nrb, row0 = (cur.job - kvh * p.nrb) * kRows, len = cur.len, n = entries(p, len);
+        // rows of q, and what they see of the drafted entries
+        __syncthreads();                   // the piece before is written out
+        for (int i = tid; i < kRows * (D / 8); i += kThreadsAttn) {
+            const int r = i / (D / 8), c = i - r * (D / 8), row = row0 + r;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < p.R) {
+                const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+            }
+            *reinterpret_cast<uint4 *>(sm_q + r * q_pitch<D, MT>() + c * 16) = x;
+        }
+        if (tid < kRows) seen[tid] = row0 + tid < p.R ? drafted_bits(p, b, (row0 + tid) / p.g, len) : 0;
+        if (tid == 0) bad = 0;
+        __syncthreads();
+        float o[MT][kDT][4], m[MT][2], l[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t][0] = m[t][1] = -INFINITY;
+            l[t][0] = l[t][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kDT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
+        }
+        int u = piece + ((u0 + warp - piece) % kWarps + kWarps) % kWarps;
+        for (; u < piece_end && alive; u += kWarps) {
+            const int key0 = (u - cur.begin) * kTile;
+            // scores: 16 MT rows by 32 keys
+            float sc[MT][kNT][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < kNT; ++i) sc[t][i][0] = sc[t][i][1] = sc[t][i][2] = sc[t][i][3] = 0.0f;
+            int slot = used % kSlots;
+            alive = mbar_wait_warp(g_status_attn, full_u + 8 * slot, (used / kSlots) & 1, &abort_flag, 31);
+            if (!alive) break;
+            const uint32_t ks = ring_u + slot * kSlot;
+#pragma unroll
+            for (int k2 = 0; k2 < kKS / 2; ++k2) {                              // 32 values of the heads at a time
+                uint32_t a[MT][8];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        ldsm4(smem_u32(sm_q) + (t * 16 + (lane & 15)) * q_pitch<D, MT>() + (k2 * 4 + hh * 2 + (lane >> 4)) * 16,
+                              a[t][4 * hh], a[t][4 * hh + 1], a[t][4 * hh + 2], a[t][4 * hh + 3]);
+#pragma unroll
+                for (int i = 0; i < kNT; ++i) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm4(ks + swizzled<kTile>(i * 8 + (lane & 7), k2 * 4 + (lane >> 3)), b0, b1, b2, b3);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        mma16816<BF16>(sc[t][i], a[t][0], a[t][1], a[t][2], a[t][3], b0, b1);
+                        mma16816<BF16>(sc[t][i], a[t][4], a[t][5], a[t][6], a[t][7], b2, b3);
+                    }
+                }
+            }
+            __syncwarp();
+            ++used;
+            issue();
+            const bool tail = key0 + kTile > len;                              // drafted entries, or none at all, in this tile
+            if (tail) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint64_t bits = seen[t * 16 + grp + (e >> 1) * 8];
+#pragma unroll
+                        for (int i = 0; i < kNT; ++i) {
+                            const int j = key0 + i * 8 + quad * 2 + (e & 1) - len;
+                            if (j >= 0 && (j >= 64 || !((bits >> j) & 1))) sc[t][i][e] = -INFINITY;
+                        }
+                    }
+            }
+            if (p.scores) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const int row = row0 + t * 16 + grp + hh * 8;
+                        if (row < p.R) {
+                            float *dst = p.scores + (((long)b * p.nkv + kvh) * p.R + row) * p.score_ld + key0 + quad * 2;
+#pragma unroll
+                            for (int i = 0; i < kNT; ++i)
+                                *reinterpret_cast<float2 *>(dst + i * 8) = make_float2(sc[t][i][2 * hh], sc[t][i][2 * hh + 1]);
+                        }
+                    }
+            }
+            // running maximum and sum; the sum is of the exponentials in binary32, before they are rounded for the product
+            uint32_t pr[MT][kNT][2];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < kNT; ++i) mx = fmaxf(mx, fmaxf(sc[t][i][2 * hh], sc[t][i][2 * hh + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    mx *= p.scale_log2;                                         // scale > 0
+                    const float was = m[t][hh], now = fmaxf(was, mx), base = now == -INFINITY ? 0.0f : now;
+                    m[t][hh] = now;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < kNT; ++i) {
+                        const float x = exp2_approx(fmaf(sc[t][i][2 * hh], p.scale_log2, -base)), y = exp2_approx(fmaf(sc[t][i][2 * hh + 1], p.scale_log2, -base));
+                        sum += x + y;
+                        pr[t][i][hh] = narrow<BF16>(x, y);
+                    }
+                    const float keep = exp2_approx(was - base);
+                    l[t][hh] = l[t][hh] * keep + sum;
+                    if (__any_sync(0xffffffffu, now != was)) {
+#pragma unroll
+                        for (int i = 0; i < kDT; ++i) { o[t][i][2 * hh] *= keep; o[t][i][2 * hh + 1] *= keep; }
+                    }
+                }
+            slot = used % kSlots;
+            alive = mbar_wait_warp(g_status_attn, full_u + 8 * slot, (used / kSlots) & 1, &abort_flag, 32);
+            if (!alive) break;
+            const uint32_t vs = ring_u + slot * kSlot;
+            if (tail) {
+                // rows of V behind the sequence's end become zero, and so do values of drafted entries that are not finite
+                for (int i = lane; i < kTile * (D / 8); i += 32) {
+                    const int row = i / (D / 8), chunk = i - row * (D / 8), t = key0 + row;
+                    if (t < len) continue;
+                    uint8_t *at = ring + slot * kSlot + swizzled<kTile>(row, chunk);
+                    uint4 x = *reinterpret_cast<const uint4 *>(at);
+                    uint16_t *h = reinterpret_cast<uint16_t *>(&x);
+                    bool changed = false;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (t >= n || nonfinite16<BF16>(h[e])) { h[e] = 0; changed = true; }
+                    if (changed) *reinterpret_cast<uint4 *>(at) = x;
+                    if (changed && t < n) atomicOr(&bad, 1ull << (t - len));
+                }
+                __syncwarp();
+            }
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) {
+#pragma unroll
+                for (int i = 0; i < kDT; i += 2) {
+                    uint32_t b0, b1, b2, b3;
+                    ldsm4t(vs + swizzled<kTile>(k * 16 + (lane & 15), i + (lane >> 4)), b0, b1, b2, b3);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        mma16816<BF16>(o[t][i], pr[t][2 * k][0], pr[t][2 * k][1], pr[t][2 * k + 1][0], pr[t][2 * k + 1][1], b0, b1);
+                        mma16816<BF16>(o[t][i + 1], pr[t][2 * k][0], pr[t][2 * k][1], pr[t][2 * k + 1][0], pr[t][2 * k + 1][1], b2, b3);
+                    }
+                }
+            }
+            if (tail) fence_proxy_async();                                      // the slot was written here: TMA writes it next
+            __syncwarp();
+            ++used;
+            issue();
+        }
+        // the warps' results, each relative to its own maximum, become one
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                float sum = l[t][hh];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (quad == 0) { sm_m[warp][t * 16 + grp + hh * 8] = m[t][hh]; sm_l[warp][t * 16 + grp + hh * 8] = sum; }
+            }
+        __syncthreads();
+        float mine[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                const int r = t * 16 + grp + hh * 8;
+                float top = sm_m[0][r];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+                mine[t][hh] = exp2_approx(m[t][hh] - (top == -INFINITY ? 0.0f : top));
+            }
+        const bool whole = piece == cur.begin && piece_end == cur.begin + cur.nt;
+        const long part = 2L * blockIdx.x + (piece != u0);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {                                      // 32 columns at a time
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        *reinterpret_cast<float2 *>(sm_o + (warp * kRows + t * 16 + grp + hh * 8) * 32 + ((i * 8 + quad * 2) ^ ((grp & 3) * 8))) =
+                            make_float2(o[t][c * 4 + i][2 * hh] * mine[t][hh], o[t][c * 4 + i][2 * hh + 1] * mine[t][hh]);
+            __syncthreads();
+            for (int i = tid; i < kRows * 32; i += kThreadsAttn) {
+                const int r = i >> 5, col = i & 31, row = row0 + r;
+                if (row >= p.R) continue;
+                float top = sm_m[0][r], sum = 0.0f, acc = 0.0f;
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+                const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    sum += sm_l[w][r] * exp2_approx(sm_m[w][r] - base);
+                    acc += sm_o[(w * kRows + r) * 32 + (col ^ ((r & 3) * 8))];
+                }
+                const int d = c * 32 + col;
+                if (bad) acc += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, row, d, len, base);
+                if (whole) {
+                    const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+                    store16<BF16>(p.out, (((long)b * p.S + s) * p.nh + h) * D + d, acc * row_factor(sum, len == 0 && !seen[r]));
+                } else {
+                    p.part_o[(part * kRows + r) * D + d] = acc;
+                }
+                if (d == 0) {
+                    if (whole) { if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum); }
+                    else p.part_ml[part * kRows + r] = make_float2(top, sum);
+                }
+            }
+            __syncthreads();
+        }
+        piece = piece_end;
+    }
+}
+
+// Row (job, row of its block) of a job that several shares hold: their partial results in order.  A block per row, a thread per
+// column, kJoin groups of threads over the shares.
+constexpr int kJoin = 4;
+template <int D, int ROWS, bool BF16>
+__global__ void __launch_bounds__(D * kJoin) attn_join_kernel(const __grid_constant__ TreeAttnParams p) {
+    __shared__ float sm_acc[kJoin][D], sm_top[kJoin], sm_sum[kJoin];
+    const int lane = threadIdx.x & 31, col = threadIdx.x % D, way = threadIdx.x / D;
+    pdl_wait();
+    pdl_trigger();
+    const int bh = blockIdx.x / p.R, row = blockIdx.x - bh * p.R, b = bh / p.nkv, kvh = bh - b * p.nkv, rb = row / ROWS, r = row - rb * ROWS;
+    const int len = committed(p, b), nt = (entries(p, len) + kTile - 1) / kTile;
+    const int begin = tiles_before<kTile>(p, b, lane) + (kvh * p.nrb + rb) * nt;
+    const int share = share_tiles(p, tiles_before<kTile>(p, p.B, lane));
+    const int c0 = begin / share, c1 = (begin + nt - 1) / share;
+    if (c0 == c1) return;
+    // only the first of these CTAs can have begun with another job
+    auto slot = [&](int c) { return (2L * c + (c == c0 && (long)c0 * share != begin)) * ROWS + r; };
+    float top = -INFINITY;
+    for (int c = c0 + way; c <= c1; c += kJoin) top = fmaxf(top, p.part_ml[slot(c)].x);
+    if (col == 0) sm_top[way] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) top = fmaxf(top, sm_top[i]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float acc = 0.0f, sum = 0.0f;
+#pragma unroll 4
+    for (int c = c0 + way; c <= c1; c += kJoin) {
+        const float2 ml = p.part_ml[slot(c)];
+        const float f = exp2_approx(ml.x - base);
+        sum += ml.y * f;
+        acc += p.part_o[slot(c) * D + col] * f;
+    }
+    sm_acc[way][col] = acc;
+    if (col == 0) sm_sum[way] = sum;
+    __syncthreads();
+    if (way) return;
+    acc = sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) { acc += sm_acc[i][col]; sum += sm_sum[i]; }
+    const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+    store16<BF16>(p.out, (((long)b * p.S + s) * p.nh + h) * D + col, acc * row_factor(sum, sum == 0.0f && len == 0 && !drafted_bits(p, b, s, len)));
+    if (col == 0 && p.lse) p.lse[(long)bh * p.R + row] = base + log2f(sum);
+}
+
+// weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
+// 2 D for reading K again).  A thread per entry.
+constexpr int kWeightThreads = 256;
+__global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __grid_constant__ TreeAttnParams p) {
+    const int bh = blockIdx.x, t = blockIdx.y * kWeightThreads + threadIdx.x;
+    pdl_wait();
+    pdl_trigger();
+    const int b = bh / p.nkv, len = committed(p, b);
+    if (t >= entries(p, len)) return;
+    const float *sc = p.scores + (long)bh * p.R * p.score_ld + t, *lse = p.lse + (long)bh * p.R;
+    float sum = 0.0f;
+    for (int r = 0; r < p.R; ++r) {
+        if (t >= len && !((drafted_bits(p, b, r / p.g, len) >> (t - len)) & 1)) continue;         // an entry that the row does not see
+        sum += exp2_approx(fmaf(sc[r * p.score_ld], p.scale_log2, -lse[r]));
+    }
+    p.weights[(long)bh * p.T + t] += sum;
+}
+
+// The same for many rows, from K and q again: a warp keeps 16 keys in registers, the rows pass through shared memory 64 at a time.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __grid_constant__ TreeAttnParams p) {
+    constexpr int kPitch = D * 2 + 16, kKS = D / 16, kChunk = 64;
+    __shared__ __align__(16) uint8_t sm[kChunk * kPitch];
+    __shared__ float lse[kChunk];
+    __shared__ uint64_t seen[kChunk];
+    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3, t0 = blockIdx.y * 64;
+    pdl_wait();
+    pdl_trigger();
+    const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
+    if (t0 >= n) return;
+    const uint16_t *k = static_cast<const uint16_t *>(p.k) + ((long)bh * p.T + t0) * D;
+    for (int i = tid; i < 64 * (D / 8); i += kThreadsAttn) {
+        const int r = i / (D / 8), c = i - r * (D / 8);
+        *reinterpret_cast<uint4 *>(sm + r * kPitch + c * 16) = t0 + r < n ? ldg_nc_v4(k + (long)r * D + c * 8) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+    uint32_t kf[2][kKS][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int k2 = 0; k2 < kKS / 2; ++k2)
+            ldsm4(smem_u32(sm) + (warp * 16 + i * 8 + (lane & 7)) * kPitch + (k2 * 4 + (lane >> 3)) * 16, kf[i][2 * k2][0], kf[i][2 * k2][1], kf[i][2 * k2 + 1][0], kf[i][2 * k2 + 1][1]);
+    float sum[2][2] = {};
+    for (int r0 = 0; r0 < p.R; r0 += kChunk) {
+        __syncthreads();
+        for (int i = tid; i < kChunk * (D / 8); i += kThreadsAttn) {
+            const int r = i / (D / 8), c = i - r * (D / 8), row = r0 + r;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (row < p.R) {
+                const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+            }
+            *reinterpret_cast<uint4 *>(sm + r * kPitch + c * 16) = x;
+        }
+        if (tid < kChunk) {
+            const int row = r0 + tid;
+            seen[tid] = row < p.R ? drafted_bits(p, b, row / p.g, len) : 0;
+            // rows that do not exist or see nothing have no weight anywhere
+            lse[tid] = row >= p.R || (len == 0 && !seen[tid]) ? INFINITY : p.lse[(long)bh * p.R + row];
+        }
+        __syncthreads();
+        for (int t = 0; t < kChunk / 16 && r0 + t * 16 < p.R; ++t) {
+            float sc[2][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < kKS; ++ks) {
+                uint32_t a0, a1, a2, a3;
+                ldsm4(smem_u32(sm) + (t * 16 + (lane & 15)) * kPitch + (ks * 2 + (lane >> 4)) * 16, a0, a1, a2, a3);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mma16816<BF16>(sc[i], a0, a1, a2, a3, kf[i][ks][0], kf[i][ks][1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = t * 16 + grp + (e >> 1) * 8, j = t0 + warp * 16 + i * 8 + quad * 2 + (e & 1) - len;
+                    const bool none = r0 + r >= p.R || lse[r] == INFINITY || (j >= 0 && (j >= 64 || !((seen[r] >> j) & 1)));
+                    sum[i][e & 1] += none ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -lse[r]));
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = sum[i][e];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const int t = t0 + warp * 16 + i * 8 + quad * 2 + e;
+            if (grp == 0 && t < n) p.weights[(long)bh * p.T + t] += x;
+        }
+}
+
+// ---- host side ------------------------------------------------------------------------------
+struct Plan {
+    int rows, nrb, shares, min_share;
+    bool scores;
+    long score_ld;
+    size_t part_o, part_ml, lse, sc, total;        // offsets in the workspace
+};
+Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
+    Plan pl = {};
+    const int R = S * (nh / nkv);
+    pl.rows = R <= 16 ? 16 : 32;
+    pl.nrb = (R + pl.rows - 1) / pl.rows;
+    pl.shares = 2 * kNumSMs;
+    pl.min_share = kWarps;
+    pl.scores = weights && R <= 16;
+    pl.score_ld = (T + kTile - 1) / kTile * kTile;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    pl.part_o = take((size_t)2 * pl.shares * pl.rows * D * 4);
+    pl.part_ml = take((size_t)2 * pl.shares * pl.rows * 8);
+    pl.lse = take(weights ? (size_t)B * nkv * R * 4 : 0);
+    pl.sc = take(pl.scores ? (size_t)B * nkv * R * pl.score_ld * 4 : 0);
+    pl.total = at;
+    return pl;
+}
+
+int make_map(CUtensorMap *map, const void *base, bool bf16, int D, long T, long heads, int rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(FLH_B200_EUNSUPPORTED, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)heads};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)T * D * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)rows, 1}, step[3] = {1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : fail(FLH_B200_EINVAL, "the cache cannot be described to TMA (%d)", (int)r);
+}
+
+template <int D, int MT, bool BF16>
+int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
+    auto kern = attn_mma_kernel<D, MT, BF16>;
+    constexpr int smem = attn_smem<D, MT>();
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
+    int rc = cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
+    if (rc) return rc;
+    const unsigned heads = (unsigned)(p.B * p.nkv);
+    rc = cuda_status(launch_pdl(attn_join_kernel<D, 16 * MT, BF16>, dim3(heads * (unsigned)p.R), D * kJoin, 0, stream, p), "tree_attention join");
+    if (rc || !p.weights) return rc;
+    if (p.scores)
+        return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");
+    return cuda_status(launch_pdl(attn_weights_mma_kernel<D, BF16>, dim3(heads, (unsigned)((p.T + 63) / 64)), kThreadsAttn, 0, stream, p), "tree_attention weights");
+}
+
+}  // namespace
+
+size_t tree_attention_workspace_bytes(int B, int S, int nh, int nkv, int D, long T, bool weights) { return plan_of(B, S, nh, nkv, D, T, weights).total; }
+
+int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t stream) {
+    const Plan pl = plan_of(p.B, p.S, p.nh, p.nkv, p.D, p.T, p.weights != nullptr);
+    p.g = p.nh / p.nkv;
+    p.R = p.S * p.g;
+    p.nrb = pl.nrb;
+    p.shares = pl.shares;
+    p.min_share = pl.min_share;
+    p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
+    p.part_ml = reinterpret_cast<float2 *>(ws + pl.part_ml);
+    p.lse = p.weights ? reinterpret_cast<float *>(ws + pl.lse) : nullptr;
+    p.scores = pl.scores ? reinterpret_cast<float *>(ws + pl.sc) : nullptr;
+    p.score_ld = pl.score_ld;
+    CUtensorMap km, vm;
+    int rc = make_map(&km, p.k, bf16, p.D, p.T, (long)p.B * p.nkv, kTile);
+    if (!rc) rc = make_map(&vm, p.v, bf16, p.D, p.T, (long)p.B * p.nkv, kTile);
+    if (rc) return rc;
+    if (p.D == 128) {
+        if (pl.rows == 16) return bf16 ? launch_mma<128, 1, true>(p, km, vm, stream) : launch_mma<128, 1, false>(p, km, vm, stream);
+        return bf16 ? launch_mma<128, 2, true>(p, km, vm, stream) : launch_mma<128, 2, false>(p, km, vm, stream);
+    }
+    if (pl.rows == 16) return bf16 ? launch_mma<64, 1, true>(p, km, vm, stream) : launch_mma<64, 1, false>(p, km, vm, stream);
+    return bf16 ? launch_mma<64, 2, true>(p, km, vm, stream) : launch_mma<64, 2, false>(p, km, vm, stream);
+}
+
+int attn_tree_status(int *out) { return cuda_status(cudaMemcpyFromSymbol(out, g_status_attn, sizeof(int) * 4), "attn_tree_status"); }
+int attn_tree_status_clear() {
+    const int zero[4] = {};
+    return cuda_status(cudaMemcpyToSymbol(g_status_attn, zero, sizeof(zero)), "attn_tree_status");
+}
+
+}  // namespace flh

@@ -177,6 +177,53 @@ int flh_b200_rope_kv_f16(const void *qkv, const float *cos, const float *sin, vo
 int flh_b200_rope_kv_by_token_f16(const void *qkv, const float *cos, const float *sin, void *q_out, void *k_cache, void *v_cache,
                                   int B, int S, int nh, int nkv, int D, int T, int cur, void *stream);
 
+/* ---- a KV cache that is drafted into and evicted from ---------------------------------------
+ *
+ * Caches are [B, nkv, T, D], f16 or bf16 (dtype), contiguous; sequence b has lengths[b] committed entries (int32, 0 .. T; values
+ * outside are taken as the nearer end), the same for all its heads.  S drafted tokens of a tree (1 .. FLH_B200_TREE_MAX_TOKENS) lie
+ * behind them, token s in entry lengths[b] + s; entries T and up do not exist.  Entries behind the last drafted one are neither
+ * used nor changed, whatever they hold.  lengths, tree, positions, path and accepted are read on the device, when the work runs. */
+#define FLH_B200_TREE_MAX_TOKENS 64
+#define FLH_B200_CACHE_MAX_LAYERS 128
+
+/* flh_b200_rope_kv_f16 for drafted tokens: the rotary row of token (b, s) is positions[b, s] (int32 [B, S]) of cos / sin (f32
+ * [P, D / 2]), k and v go to entry lengths[b] + s, q to q_out [B, S, nh, D].  qkv [B * S, (nh + 2 nkv) * D].  D % 16 == 0.  A token
+ * whose position is not in the tables has NaN for q and k. */
+int flh_b200_rope_kv_at(const void *qkv, int dtype, const float *cos, const float *sin, long P, const int32_t *positions, const int32_t *lengths,
+                        void *q_out, void *k_cache, void *v_cache, int B, int S, int nh, int nkv, int D, long T, void *stream);
+
+/* out[b, s, h] = sum_t p[t] v[t], p = softmax(scale * q[b, s, h] . k[t]) over the entries t that token s sees: all committed ones and
+ * the drafted ones whose bit is set in tree (int64 bits [S], or [B, S] with tree_stride = S; NULL: a chain, token s sees
+ * drafted entries 0 .. s).  A token that sees nothing has zero.  S = 1 is ordinary decode.
+ *   q        [B, S, nh, D] with strides q_sb, q_ss, q_sh in elements (multiples of 8), the last dimension contiguous; nh % nkv == 0, head h
+ *            reads kv head h / (nh / nkv); D is 64 or 128; T <= 2^21; scale > 0
+ *   out      [B, S, nh, D] contiguous
+ *   weights  f32 [B, nkv, T], or NULL: to entry t is added the sum of p[t] over all tokens and the heads of the group, in an order
+ *            that is the same every time
+ *   ws       workspace of flh_b200_tree_attention_workspace_bytes bytes (16-byte aligned), any contents, of this call alone until its
+ *            work has run */
+size_t flh_b200_tree_attention_workspace_bytes(int B, int S, int nh, int nkv, int D, long T, int with_weights);
+int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache,
+                            const int32_t *lengths, const int64_t *tree, long tree_stride, float scale, void *out, float *weights,
+                            int B, int S, int nh, int nkv, int D, long T, void *ws, size_t ws_bytes, void *stream);
+/* [code, cta, 0, 0] of the attention's bounded waits, as flh_b200_gemm_status; synchronises. */
+int flh_b200_tree_attention_status(int *out);
+
+/* The accepted branch of a tree: for i < accepted[b] entry lengths[b] + path[b, i] moves to entry lengths[b] + i (path int32 [B, A], A <=
+ * drafted; in any order, as if all were read before any is written; an index outside 0 .. drafted - 1 leaves entry i as it is), in
+ * the `layers` caches k[l], v[l] (HOST arrays of device pointers).  w (or NULL): f32 [B, nkv, T] of each layer, moved along, and 0
+ * for the drafted entries behind the accepted ones.  now (int32 [B], or NULL): lengths[b] + accepted[b], at most T; it may not be
+ * `lengths` itself. */
+int flh_b200_cache_accept(void *const *k, void *const *v, float *const *w, int layers, int dtype, const int32_t *lengths, const int32_t *path,
+                          const int32_t *accepted, int32_t *now, int B, int nkv, int D, long T, int A, int drafted, void *stream);
+
+/* Down to `keep` entries a head: of every (layer, sequence, kv head) with more than that the last `recent` (<= keep) stay and, of the
+ * others, the keep - recent with the largest weights (NaN counts as the largest; ties: the lower index).  Rows of k[l] and v[l]
+ * move together in order, in place; kept (int32 [layers, B, nkv, keep]) has the entries that stay, -1 behind the last; left (f32
+ * [layers, B, nkv, T]) their weights, 0 behind the last; now (int32 [B]) the new lengths.  w[l] is only read. */
+int flh_b200_cache_evict(void *const *k, void *const *v, const float *const *w, int layers, int dtype, const int32_t *lengths, int keep, int recent,
+                         int32_t *kept, float *left, int32_t *now, int B, int nkv, int D, long T, void *stream);
+
 /* HOST helpers: build the factor table of a kfac x kfac matrix of +1/-1 (int8, row-major, host
  * memory).  Layout: bit rows out[k * words + w], bit b = 1 when signs[k][32 w + b] < 0,
  * words = (kfac + 31) / 32; then, at the next 16-byte boundary, the same matrix as bfloat16 +-1.0
