@@ -21,7 +21,7 @@ struct TreeAttnParams {
     const void *k, *v;                     // [B, nkv, T, D]
     void *out;                             // [B, S, nh, D]
     float *weights;                        // [B, nkv, T], added to; or null
-    int B, S, nh, nkv, g, D, R, nrb;       // nrb: blocks of rows
+    int B, S, nh, nkv, g, D, R, nrb, rows; // nrb: blocks of `rows` rows
     int T;
     float scale_log2;                      // scale * log2(e): scores live in powers of two
     int shares, min_share;                 // CTAs, tiles that a share has at least

@@ -14,6 +14,11 @@
 #include "tc_pair.cuh"
 
 namespace flh {
+
+int launch_attn_tc(const TreeAttnParams &, int, bool, const CUtensorMap &, const CUtensorMap &, cudaStream_t);
+int attn_tc_status(int *);
+int attn_tc_status_clear();
+
 namespace {
 
 __device__ int g_status_attn[4];
@@ -328,20 +333,20 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
 // Row (job, row of its block) of a job that several shares hold: their partial results in order.  A block per row, a thread per
 // column, kJoin groups of threads over the shares.
 constexpr int kJoin = 4;
-template <int D, int ROWS, bool BF16>
+template <int D, int TILE, bool BF16>
 __global__ void __launch_bounds__(D * kJoin) attn_join_kernel(const __grid_constant__ TreeAttnParams p) {
     __shared__ float sm_acc[kJoin][D], sm_top[kJoin], sm_sum[kJoin];
     const int lane = threadIdx.x & 31, col = threadIdx.x % D, way = threadIdx.x / D;
     pdl_wait();
     pdl_trigger();
-    const int bh = blockIdx.x / p.R, row = blockIdx.x - bh * p.R, b = bh / p.nkv, kvh = bh - b * p.nkv, rb = row / ROWS, r = row - rb * ROWS;
-    const int len = committed(p, b), nt = (entries(p, len) + kTile - 1) / kTile;
-    const int begin = tiles_before<kTile>(p, b, lane) + (kvh * p.nrb + rb) * nt;
-    const int share = share_tiles(p, tiles_before<kTile>(p, p.B, lane));
+    const int bh = blockIdx.x / p.R, row = blockIdx.x - bh * p.R, b = bh / p.nkv, kvh = bh - b * p.nkv, rb = row / p.rows, r = row - rb * p.rows;
+    const int len = committed(p, b), nt = (entries(p, len) + TILE - 1) / TILE;
+    const int begin = tiles_before<TILE>(p, b, lane) + (kvh * p.nrb + rb) * nt;
+    const int share = share_tiles(p, tiles_before<TILE>(p, p.B, lane));
     const int c0 = begin / share, c1 = (begin + nt - 1) / share;
     if (c0 == c1) return;
     // only the first of these CTAs can have begun with another job
-    auto slot = [&](int c) { return (2L * c + (c == c0 && (long)c0 * share != begin)) * ROWS + r; };
+    auto slot = [&](int c) { return (2L * c + (c == c0 && (long)c0 * share != begin)) * p.rows + r; };
     float top = -INFINITY;
     for (int c = c0 + way; c <= c1; c += kJoin) top = fmaxf(top, p.part_ml[slot(c)].x);
     if (col == 0) sm_top[way] = top;
@@ -463,6 +468,7 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
 }
 
 // ---- host side ------------------------------------------------------------------------------
+constexpr int kMmaRows = 16;
 struct Plan {
     int rows, nrb, shares, min_share;
     bool scores;
@@ -472,10 +478,10 @@ struct Plan {
 Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     Plan pl = {};
     const int R = S * (nh / nkv);
-    pl.rows = R <= 16 ? 16 : 32;
+    pl.rows = R <= 16 ? 16 : R <= kMmaRows ? 32 : R <= 128 ? 128 : 256;
     pl.nrb = (R + pl.rows - 1) / pl.rows;
-    pl.shares = 2 * kNumSMs;
-    pl.min_share = kWarps;
+    pl.shares = pl.rows >= 128 ? kNumSMs : 2 * kNumSMs;
+    pl.min_share = pl.rows >= 128 ? 1 : kWarps;
     pl.scores = weights && R <= 16;
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
@@ -503,12 +509,18 @@ template <int D, int MT, bool BF16>
 int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     auto kern = attn_mma_kernel<D, MT, BF16>;
     constexpr int smem = attn_smem<D, MT>();
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    int rc = cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
-    if (rc) return rc;
+    return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
+}
+
+template <int D, bool BF16>
+int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     const unsigned heads = (unsigned)(p.B * p.nkv);
-    rc = cuda_status(launch_pdl(attn_join_kernel<D, 16 * MT, BF16>, dim3(heads * (unsigned)p.R), D * kJoin, 0, stream, p), "tree_attention join");
+    const bool tc = p.rows >= 128;
+    int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : p.rows == 16 ? launch_mma<D, 1, BF16>(p, km, vm, stream) : launch_mma<D, 2, BF16>(p, km, vm, stream);
+    if (rc) return rc;
+    rc = cuda_status(launch_pdl(tc ? attn_join_kernel<D, 128, BF16> : attn_join_kernel<D, kTile, BF16>, dim3(heads * (unsigned)p.R), D * kJoin, 0, stream, p), "tree_attention join");
     if (rc || !p.weights) return rc;
     if (p.scores)
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");
@@ -524,6 +536,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.g = p.nh / p.nkv;
     p.R = p.S * p.g;
     p.nrb = pl.nrb;
+    p.rows = pl.rows;
     p.shares = pl.shares;
     p.min_share = pl.min_share;
     p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
@@ -532,21 +545,22 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.scores = pl.scores ? reinterpret_cast<float *>(ws + pl.sc) : nullptr;
     p.score_ld = pl.score_ld;
     CUtensorMap km, vm;
-    int rc = make_map(&km, p.k, bf16, p.D, p.T, (long)p.B * p.nkv, kTile);
-    if (!rc) rc = make_map(&vm, p.v, bf16, p.D, p.T, (long)p.B * p.nkv, kTile);
+    const int tile = pl.rows >= 128 ? 128 : kTile;
+    int rc = make_map(&km, p.k, bf16, p.D, p.T, (long)p.B * p.nkv, tile);
+    if (!rc) rc = make_map(&vm, p.v, bf16, p.D, p.T, (long)p.B * p.nkv, tile);
     if (rc) return rc;
-    if (p.D == 128) {
-        if (pl.rows == 16) return bf16 ? launch_mma<128, 1, true>(p, km, vm, stream) : launch_mma<128, 1, false>(p, km, vm, stream);
-        return bf16 ? launch_mma<128, 2, true>(p, km, vm, stream) : launch_mma<128, 2, false>(p, km, vm, stream);
-    }
-    if (pl.rows == 16) return bf16 ? launch_mma<64, 1, true>(p, km, vm, stream) : launch_mma<64, 1, false>(p, km, vm, stream);
-    return bf16 ? launch_mma<64, 2, true>(p, km, vm, stream) : launch_mma<64, 2, false>(p, km, vm, stream);
+    if (p.D == 128) return bf16 ? launch_attention<128, true>(p, km, vm, stream) : launch_attention<128, false>(p, km, vm, stream);
+    return bf16 ? launch_attention<64, true>(p, km, vm, stream) : launch_attention<64, false>(p, km, vm, stream);
 }
 
-int attn_tree_status(int *out) { return cuda_status(cudaMemcpyFromSymbol(out, g_status_attn, sizeof(int) * 4), "attn_tree_status"); }
+int attn_tree_status(int *out) {
+    const int rc = attn_tc_status(out);
+    return rc || out[0] ? rc : cuda_status(cudaMemcpyFromSymbol(out, g_status_attn, sizeof(int) * 4), "attn_tree_status");
+}
 int attn_tree_status_clear() {
     const int zero[4] = {};
-    return cuda_status(cudaMemcpyToSymbol(g_status_attn, zero, sizeof(zero)), "attn_tree_status");
+    const int rc = attn_tc_status_clear();
+    return rc ? rc : cuda_status(cudaMemcpyToSymbol(g_status_attn, zero, sizeof(zero)), "attn_tree_status");
 }
 
 }  // namespace flh
