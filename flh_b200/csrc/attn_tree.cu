@@ -330,48 +330,76 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
     }
 }
 
-// Row (job, row of its block) of a job that several shares hold: their partial results in order.  A block per row, a thread per
-// column, kJoin groups of threads over the shares.
-constexpr int kJoin = 4;
-template <int D, int TILE, bool BF16>
-__global__ void __launch_bounds__(D * kJoin) attn_join_kernel(const __grid_constant__ TreeAttnParams p) {
-    __shared__ float sm_acc[kJoin][D], sm_top[kJoin], sm_sum[kJoin];
-    const int lane = threadIdx.x & 31, col = threadIdx.x % D, way = threadIdx.x / D;
+// Jobs that several shares hold: their partial results in order.  A block for each job, or for each cut between two shares where that is
+// fewer (it takes the job that is cut there, if that is the job's first cut), and 8 of its rows; a warp per row, or, for few jobs in
+// many parts (WIDE), all warps of a block one row.
+template <int D, int TILE, bool BF16, bool WIDE>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+    __shared__ float sm_acc[WIDE ? 8 : 1][D], sm_sum[8];
+    constexpr int kCols = D / 32;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     pdl_trigger();
-    const int bh = blockIdx.x / p.R, row = blockIdx.x - bh * p.R, b = bh / p.nkv, kvh = bh - b * p.nkv, rb = row / p.rows, r = row - rb * p.rows;
-    const int len = committed(p, b), nt = (entries(p, len) + TILE - 1) / TILE;
-    const int begin = tiles_before<TILE>(p, b, lane) + (kvh * p.nrb + rb) * nt;
-    const int share = share_tiles(p, tiles_before<TILE>(p, p.B, lane));
-    const int c0 = begin / share, c1 = (begin + nt - 1) / share;
-    if (c0 == c1) return;
-    // only the first of these CTAs can have begun with another job
-    auto slot = [&](int c) { return (2L * c + (c == c0 && (long)c0 * share != begin)) * p.rows + r; };
-    float top = -INFINITY;
-    for (int c = c0 + way; c <= c1; c += kJoin) top = fmaxf(top, p.part_ml[slot(c)].x);
-    if (col == 0) sm_top[way] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kJoin; ++i) top = fmaxf(top, sm_top[i]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float acc = 0.0f, sum = 0.0f;
-#pragma unroll 4
-    for (int c = c0 + way; c <= c1; c += kJoin) {
-        const float2 ml = p.part_ml[slot(c)];
-        const float f = exp2_approx(ml.x - base);
-        sum += ml.y * f;
-        acc += p.part_o[slot(c) * D + col] * f;
+    const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
+    JobWalk<TILE> job;
+    if (by_job) {
+        const int per = p.nkv * p.nrb;
+        job.b = blockIdx.x / per;
+        job.job = blockIdx.x - job.b * per;
+        job.len = committed(p, job.b);
+        job.nt = (entries(p, job.len) + TILE - 1) / TILE;
+        job.begin = tiles_before<TILE>(p, job.b, lane) + job.job * job.nt;
+    } else {
+        const long cut = (blockIdx.x + 1L) * share;
+        if (cut >= total) return;
+        job.seek(p, (int)cut, lane);
+        if (job.begin == cut || job.begin / share != (int)blockIdx.x) return;
     }
-    sm_acc[way][col] = acc;
-    if (col == 0) sm_sum[way] = sum;
-    __syncthreads();
-    if (way) return;
-    acc = sum = 0.0f;
+    const int c0 = job.begin / share, parts = (job.begin + job.nt - 1) / share - c0 + 1;
+    if (parts == 1) return;
+    const int kvh = job.job / p.nrb, row0 = (job.job - kvh * p.nrb) * p.rows, r = WIDE ? blockIdx.y : blockIdx.y * 8 + warp, row = row0 + r, b = job.b;
+    if (r >= p.rows || row >= p.R) return;
+    // only the first of these CTAs can have begun with another job
+    const bool behind = (long)c0 * share != job.begin;
+    auto slot = [&](int i) { return (2L * (c0 + i) + (i == 0 && behind)) * p.rows + r; };
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.0f : top;
+    float acc[kCols] = {}, sum = 0.0f;
+#pragma unroll 8
+    for (int i = WIDE ? warp : 0; i < parts; i += WIDE ? 8 : 1) {
+        const float2 ml = p.part_ml[slot(i)];
+        const float f = exp2_approx(ml.x - base), *o = p.part_o + slot(i) * D + lane * kCols;
+        sum += ml.y * f;
+        float v[kCols];
+        if (D == 128) { const float4 w = *reinterpret_cast<const float4 *>(o); v[0] = w.x; v[1] = w.y; v[kCols - 2] = w.z; v[kCols - 1] = w.w; }
+        else { const float2 w = *reinterpret_cast<const float2 *>(o); v[0] = w.x; v[1] = w.y; }
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) { acc += sm_acc[i][col]; sum += sm_sum[i]; }
+        for (int c = 0; c < kCols; ++c) acc[c] += v[c] * f;
+    }
+    if (WIDE) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) sm_acc[warp][lane * kCols + c] = acc[c];
+        if (lane == 0) sm_sum[warp] = sum;
+        __syncthreads();
+        if (warp) return;
+        sum = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            sum += sm_sum[w];
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) acc[c] += sm_acc[w][lane * kCols + c];
+        }
+    }
     const int s = row / p.g, h = kvh * p.g + row - s * p.g;
-    store16<BF16>(p.out, (((long)b * p.S + s) * p.nh + h) * D + col, acc * row_factor(sum, sum == 0.0f && len == 0 && !drafted_bits(p, b, s, len)));
-    if (col == 0 && p.lse) p.lse[(long)bh * p.R + row] = base + log2f(sum);
+    const float factor = row_factor(sum, sum == 0.0f && job.len == 0 && !drafted_bits(p, b, s, job.len));
+    uint32_t *out = static_cast<uint32_t *>(p.out) + ((((long)b * p.S + s) * p.nh + h) * D + lane * kCols) / 2;
+    if (D == 128) *reinterpret_cast<uint2 *>(out) = make_uint2(narrow<BF16>(acc[0] * factor, acc[1] * factor), narrow<BF16>(acc[kCols - 2] * factor, acc[kCols - 1] * factor));
+    else *out = narrow<BF16>(acc[0] * factor, acc[1] * factor);
+    if (lane == 0 && p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum);
 }
 
 // weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
@@ -405,10 +433,17 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
     const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
     if (t0 >= n) return;
     const uint16_t *k = static_cast<const uint16_t *>(p.k) + ((long)bh * p.T + t0) * D;
-    for (int i = tid; i < 64 * (D / 8); i += kThreadsAttn) {
-        const int r = i / (D / 8), c = i - r * (D / 8);
-        *reinterpret_cast<uint4 *>(sm + r * kPitch + c * 16) = t0 + r < n ? ldg_nc_v4(k + (long)r * D + c * 8) : make_uint4(0, 0, 0, 0);
+    // pieces of 16 bytes of 64 rows: a thread has the same piece of every kStep-th row
+    constexpr int kStep = kThreadsAttn / (D / 8), kLoads = 64 / kStep;
+    const int c = tid % (D / 8), first = tid / (D / 8);
+    uint4 x[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = first + i * kStep;
+        x[i] = t0 + r < n ? ldg_nc_v4(k + (long)r * D + c * 8) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) *reinterpret_cast<uint4 *>(sm + (first + i * kStep) * kPitch + c * 16) = x[i];
     __syncthreads();
     uint32_t kf[2][kKS][2];
 #pragma unroll
@@ -419,15 +454,13 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
     float sum[2][2] = {};
     for (int r0 = 0; r0 < p.R; r0 += kChunk) {
         __syncthreads();
-        for (int i = tid; i < kChunk * (D / 8); i += kThreadsAttn) {
-            const int r = i / (D / 8), c = i - r * (D / 8), row = r0 + r;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row < p.R) {
-                const int s = row / p.g, h = kvh * p.g + row - s * p.g;
-                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
-            }
-            *reinterpret_cast<uint4 *>(sm + r * kPitch + c * 16) = x;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int row = min(r0 + first + i * kStep, p.R - 1), s = row / p.g, h = kvh * p.g + row - s * p.g;
+            x[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
         }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<uint4 *>(sm + (first + i * kStep) * kPitch + c * 16) = x[i];
         if (tid < kChunk) {
             const int row = r0 + tid;
             seen[tid] = row < p.R ? drafted_bits(p, b, row / p.g, len) : 0;
@@ -520,7 +553,13 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
     const bool tc = p.rows >= 128;
     int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : p.rows == 16 ? launch_mma<D, 1, BF16>(p, km, vm, stream) : launch_mma<D, 2, BF16>(p, km, vm, stream);
     if (rc) return rc;
-    rc = cuda_status(launch_pdl(tc ? attn_join_kernel<D, 128, BF16> : attn_join_kernel<D, kTile, BF16>, dim3(heads * (unsigned)p.R), D * kJoin, 0, stream, p), "tree_attention join");
+    const long jobs = (long)heads * p.nrb;
+    const bool by_job = jobs < p.shares, wide = jobs * 16 <= p.shares;             // 16 parts a job and more: a row's parts over the warps of a block
+    const int rows = p.R < p.rows ? p.R : p.rows;
+    const dim3 grid(by_job ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)(wide ? rows : (rows + 7) / 8));
+    auto join = tc ? (wide ? attn_join_kernel<D, 128, BF16, true> : attn_join_kernel<D, 128, BF16, false>)
+                   : (wide ? attn_join_kernel<D, kTile, BF16, true> : attn_join_kernel<D, kTile, BF16, false>);
+    rc = cuda_status(launch_pdl(join, grid, 256, 0, stream, p, (int)by_job), "tree_attention join");
     if (rc || !p.weights) return rc;
     if (p.scores)
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");

@@ -185,14 +185,19 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             const bool warp_live = myrow0 + quarter * 32 < p.R;
             // rows of q; what came before in this CTA is read out of shared and tensor memory
             if (tid == 128) bad = 0;
-            for (int i = TWO ? wg : wg + x * 128; i < kRowsTc * (D / 8); i += TWO ? 128 : 256) {
-                const int qr = i / (D / 8), c = i - qr * (D / 8), from = myrow0 + qr;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (from < p.R) {
-                    const int s = from / p.g, h = kvh * p.g + from - s * p.g;
-                    v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
-                }
-                *reinterpret_cast<uint4 *>(sm_q + (TWO ? x * kItem : 0) + (c >> 3) * kHalf + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = v;
+            constexpr int kStep = (TWO ? 128 : 256) / (D / 8), kLoads = kRowsTc / kStep;          // rows apart, and rows, of a thread
+            const int c = wg % (D / 8), qr0 = (TWO ? wg : wg + x * 128) / (D / 8);
+            uint4 qv[kLoads];
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int from = myrow0 + qr0 + i * kStep, at = min(from, p.R - 1), s = at / p.g, h = kvh * p.g + at - s * p.g;
+                qv[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+                if (from >= p.R) qv[i] = make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int qr = qr0 + i * kStep;
+                *reinterpret_cast<uint4 *>(sm_q + (TWO ? x * kItem : 0) + (c >> 3) * kHalf + qr * 128 + (((c & 7) ^ (qr & 7)) << 4)) = qv[i];
             }
             fence_proxy_async();
             tc_fence_before();
@@ -219,10 +224,10 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                             if (j >= 0 && (j >= 64 || !((seen >> j) & 1))) s[c] = 0xff800000u;
                         }
                     }
-                    float mx = -INFINITY;
+                    float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) mx = fmaxf(mx, __uint_as_float(s[c]));
-                    mx *= p.scale_log2;
+                    for (int c = 0; c < 128; ++c) mx4[c & 3] = fmaxf(mx4[c & 3], __uint_as_float(s[c]));
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
                     const bool grow = mx > m + kLag || m == -INFINITY;
                     if (mine == 0) m = mx;
                     else if (__any_sync(0xffffffffu, grow && mx != m)) {
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     }
                     const float base = m == -INFINITY ? 0.0f : -m;
                     const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), base2 = pack2(base, base);
-                    uint64_t sum2 = 0;
+                    uint64_t sum2[4] = {};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t w[16];
@@ -252,13 +257,13 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                             unpack2(fma2(pack2(__uint_as_float(s[i * 32 + 2 * c]), __uint_as_float(s[i * 32 + 2 * c + 1])), scale2, base2), e0, e1);
                             e0 = exp2_approx(e0);
                             e1 = exp2_approx(e1);
-                            sum2 = add2(sum2, pack2(e0, e1));
+                            sum2[c & 3] = add2(sum2[c & 3], pack2(e0, e1));
                             w[c] = narrow<BF16>(e0, e1);
                         }
                         tc_st16(ts + i * 16, w);
                     }
                     float a, c;
-                    unpack2(sum2, a, c);
+                    unpack2(add2(add2(sum2[0], sum2[1]), add2(sum2[2], sum2[3])), a, c);
                     l += a + c;
                     tc_wait_st();
                 }
