@@ -22,10 +22,11 @@ struct TreeAttnParams {
     void *out;                             // [B, S, nh, D]
     float *weights;                        // [B, nkv, T], added to; or null
     int B, S, nh, nkv, g, D, R, nrb, rows; // nrb: blocks of `rows` rows
+    uint32_t g_inverse;                    // 2^32 / g, rounded up (g > 1)
     int T;
     float scale_log2;                      // scale * log2(e): scores live in powers of two
     int shares, min_share;                 // CTAs, tiles that a share has at least
-    float *part_o;                         // [2 shares][rows of a block][D]
+    float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
     float *scores;                         // [B, nkv, R, score_ld] (with weights and few rows), or null
@@ -40,6 +41,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ int committed(const TreeAttnParams &p, int b) { return min(max(p.lengths[b], 0), p.T); }
 __device__ __forceinline__ int entries(const TreeAttnParams &p, int len) { return min(len + p.S, p.T); }    // len <= T < 2^30
 
+// row / g: exact for row < 64 g with g <= 4096, where row * (g_inverse * g - 2^32) < 64 g * g < 2^32
+__device__ __forceinline__ int token_of(const TreeAttnParams &p, int row) { return p.g == 1 ? row : (int)__umulhi((uint32_t)row, p.g_inverse); }
+// element offset of a row of q
+__device__ __forceinline__ long q_offset(const TreeAttnParams &p, int b, int kvh, int row) {
+    const int s = token_of(p, row);
+    return b * p.q_sb + s * p.q_ss + (long)(kvh * p.g + row - s * p.g) * p.q_sh;
+}
+// A value that is the same in all lanes, where the compiler knows it too: what MMAs and TMA loads are issued with has to be in uniform
+// registers, and a value out of a shuffle or a load is moved there anew for every instruction (measured: 900 clocks for eight MMAs).
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+
 // The drafted entries that a token sees, as bits; those behind the end of the cache do not exist.
 __device__ __forceinline__ uint64_t drafted_bits(const TreeAttnParams &p, int b, int s, int len) {
     const int n = entries(p, len) - len;
@@ -53,7 +65,7 @@ __device__ __forceinline__ int tiles_before(const TreeAttnParams &p, int upto, i
     int sum = 0;
     for (int i = lane; i < upto; i += 32) sum += (entries(p, committed(p, i)) + TILE - 1) / TILE;
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum * p.nkv * p.nrb;
+    return uniform(sum) * p.nkv * p.nrb;
 }
 __device__ __forceinline__ int share_tiles(const TreeAttnParams &p, int total) { return max((total + p.shares - 1) / p.shares, p.min_share); }
 
@@ -80,7 +92,9 @@ struct JobWalk {
             base += __shfl_sync(0xffffffffu, incl, 31);
             b0 += 32;
         }
-        len = committed(p, b);
+        b = uniform(b);
+        base = uniform(base);
+        len = uniform(committed(p, b));
         nt = (entries(p, len) + TILE - 1) / TILE;
         job = (u - base) / nt;
         begin = base + job * nt;
@@ -90,7 +104,7 @@ struct JobWalk {
         if (++job == p.nkv * p.nrb) {
             job = 0;
             if (++b < p.B) {
-                len = committed(p, b);
+                len = uniform(committed(p, b));
                 nt = (entries(p, len) + TILE - 1) / TILE;
             } else {
                 b = p.B;                   // behind the last job: no tile comes here
@@ -129,7 +143,7 @@ __device__ __forceinline__ float row_factor(float l, bool empty) { return l == 0
 // maximum that the sum is relative to.
 template <bool BF16>
 __device__ __noinline__ float nonfinite_part(const TreeAttnParams &p, uint64_t bad, uint64_t seen, int b, int kvh, int row, int d, int len, float m) {
-    const long q0 = b * p.q_sb + (row / p.g) * p.q_ss + (long)(kvh * p.g + row % p.g) * p.q_sh;
+    const long q0 = q_offset(p, b, kvh, row);
     float sum = 0.0f;
     for (uint64_t left = bad & seen; left; left &= left - 1) {
         const long at = (((long)b * p.nkv + kvh) * p.T + len + __ffsll((long long)left) - 1) * p.D;

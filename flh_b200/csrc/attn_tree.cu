@@ -117,12 +117,11 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const int r = i / (D / 8), c = i - r * (D / 8), row = row0 + r;
             uint4 x = make_uint4(0, 0, 0, 0);
             if (row < p.R) {
-                const int s = row / p.g, h = kvh * p.g + row - s * p.g;
-                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, row) + c * 8);
             }
             *reinterpret_cast<uint4 *>(sm_q + r * q_pitch<D, MT>() + c * 16) = x;
         }
-        if (tid < kRows) seen[tid] = row0 + tid < p.R ? drafted_bits(p, b, (row0 + tid) / p.g, len) : 0;
+        if (tid < kRows) seen[tid] = row0 + tid < p.R ? drafted_bits(p, b, token_of(p, row0 + tid), len) : 0;
         if (tid == 0) bad = 0;
         __syncthreads();
         float o[MT][kDT][4], m[MT][2], l[MT][2];
@@ -314,10 +313,10 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
                 const int d = c * 32 + col;
                 if (bad) acc += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, row, d, len, base);
                 if (whole) {
-                    const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+                    const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
                     store16<BF16>(p.out, (((long)b * p.S + s) * p.nh + h) * D + d, acc * row_factor(sum, len == 0 && !seen[r]));
                 } else {
-                    p.part_o[(part * kRows + r) * D + d] = acc;
+                    p.part_o[part * kRows * D + (d >> 2) * (kRows * 4) + r * 4 + (d & 3)] = acc;
                 }
                 if (d == 0) {
                     if (whole) { if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum); }
@@ -331,13 +330,14 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
 }
 
 // Jobs that several shares hold: their partial results in order.  A block for each job, or for each cut between two shares where that is
-// fewer (it takes the job that is cut there, if that is the job's first cut), and 8 of its rows; a warp per row, or, for few jobs in
-// many parts (WIDE), all warps of a block one row.
-template <int D, int TILE, bool BF16, bool WIDE>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
-    __shared__ float sm_acc[WIDE ? 8 : 1][D], sm_sum[8];
-    constexpr int kCols = D / 32;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// fewer (it takes the job that is cut there, if that is the job's first cut), and a few of its rows: a thread for four columns of a
+// row, 8 rows next to one another in a warp so that it reads whole lines.  WAYS groups of threads share out the parts of a job.
+template <int D> constexpr int join_rows() { return 1024 / D; }
+template <int D, int TILE, bool BF16, int WAYS>
+__global__ void __launch_bounds__(256 * WAYS) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+    __shared__ float sm_acc[WAYS > 1 ? WAYS - 1 : 1][5][256];
+    const int lane = threadIdx.x & 31, way = threadIdx.x >> 8, t = threadIdx.x & 255;
+    const int group = t / join_rows<D>(), r = blockIdx.y * join_rows<D>() + t % join_rows<D>();
     pdl_wait();
     pdl_trigger();
     const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
@@ -357,49 +357,41 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     }
     const int c0 = job.begin / share, parts = (job.begin + job.nt - 1) / share - c0 + 1;
     if (parts == 1) return;
-    const int kvh = job.job / p.nrb, row0 = (job.job - kvh * p.nrb) * p.rows, r = WIDE ? blockIdx.y : blockIdx.y * 8 + warp, row = row0 + r, b = job.b;
-    if (r >= p.rows || row >= p.R) return;
+    const int kvh = job.job / p.nrb, row0 = (job.job - kvh * p.nrb) * p.rows, row = row0 + r, b = job.b;
+    const bool live = r < p.rows && row < p.R;
     // only the first of these CTAs can have begun with another job
     const bool behind = (long)c0 * share != job.begin;
-    auto slot = [&](int i) { return (2L * (c0 + i) + (i == 0 && behind)) * p.rows + r; };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.0f : top;
-    float acc[kCols] = {}, sum = 0.0f;
+    auto slot = [&](int i) { return 2L * (c0 + i) + (i == 0 && behind); };
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+    if (live) {
 #pragma unroll 8
-    for (int i = WIDE ? warp : 0; i < parts; i += WIDE ? 8 : 1) {
-        const float2 ml = p.part_ml[slot(i)];
-        const float f = exp2_approx(ml.x - base), *o = p.part_o + slot(i) * D + lane * kCols;
-        sum += ml.y * f;
-        float v[kCols];
-        if (D == 128) { const float4 w = *reinterpret_cast<const float4 *>(o); v[0] = w.x; v[1] = w.y; v[kCols - 2] = w.z; v[kCols - 1] = w.w; }
-        else { const float2 w = *reinterpret_cast<const float2 *>(o); v[0] = w.x; v[1] = w.y; }
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) acc[c] += v[c] * f;
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, p.part_ml[slot(i) * p.rows + r].x);
     }
-    if (WIDE) {
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) sm_acc[warp][lane * kCols + c] = acc[c];
-        if (lane == 0) sm_sum[warp] = sum;
-        __syncthreads();
-        if (warp) return;
-        sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) acc[c] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            sum += sm_sum[w];
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) acc[c] += sm_acc[w][lane * kCols + c];
+    const float base = top == -INFINITY ? 0.0f : top;
+    if (live) {
+#pragma unroll 8
+        for (int i = way; i < parts; i += WAYS) {
+            const float2 ml = p.part_ml[slot(i) * p.rows + r];
+            const float4 v = *reinterpret_cast<const float4 *>(p.part_o + slot(i) * p.rows * D + ((long)group * p.rows + r) * 4);
+            const float f = exp2_approx(ml.x - base);
+            sum += ml.y * f;
+            acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
     }
-    const int s = row / p.g, h = kvh * p.g + row - s * p.g;
+    if (WAYS > 1) {
+        if (way) { float(*x)[256] = sm_acc[way - 1]; x[0][t] = acc.x; x[1][t] = acc.y; x[2][t] = acc.z; x[3][t] = acc.w; x[4][t] = sum; }
+        __syncthreads();
+        if (way) return;
+#pragma unroll
+        for (int w = 0; w < WAYS - 1; ++w) { acc.x += sm_acc[w][0][t]; acc.y += sm_acc[w][1][t]; acc.z += sm_acc[w][2][t]; acc.w += sm_acc[w][3][t]; sum += sm_acc[w][4][t]; }
+    }
+    if (!live) return;
+    const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
     const float factor = row_factor(sum, sum == 0.0f && job.len == 0 && !drafted_bits(p, b, s, job.len));
-    uint32_t *out = static_cast<uint32_t *>(p.out) + ((((long)b * p.S + s) * p.nh + h) * D + lane * kCols) / 2;
-    if (D == 128) *reinterpret_cast<uint2 *>(out) = make_uint2(narrow<BF16>(acc[0] * factor, acc[1] * factor), narrow<BF16>(acc[kCols - 2] * factor, acc[kCols - 1] * factor));
-    else *out = narrow<BF16>(acc[0] * factor, acc[1] * factor);
-    if (lane == 0 && p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum);
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + s) * p.nh + h) * D + group * 4) =
+        make_uint2(narrow<BF16>(acc.x * factor, acc.y * factor), narrow<BF16>(acc.z * factor, acc.w * factor));
+    if (group == 0 && p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum);
 }
 
 // weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
@@ -414,7 +406,7 @@ __global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __gr
     const float *sc = p.scores + (long)bh * p.R * p.score_ld + t, *lse = p.lse + (long)bh * p.R;
     float sum = 0.0f;
     for (int r = 0; r < p.R; ++r) {
-        if (t >= len && !((drafted_bits(p, b, r / p.g, len) >> (t - len)) & 1)) continue;         // an entry that the row does not see
+        if (t >= len && !((drafted_bits(p, b, token_of(p, r), len) >> (t - len)) & 1)) continue;         // an entry that the row does not see
         sum += exp2_approx(fmaf(sc[r * p.score_ld], p.scale_log2, -lse[r]));
     }
     p.weights[(long)bh * p.T + t] += sum;
@@ -456,14 +448,14 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int row = min(r0 + first + i * kStep, p.R - 1), s = row / p.g, h = kvh * p.g + row - s * p.g;
-            x[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+            const int row = min(r0 + first + i * kStep, p.R - 1);
+            x[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, row) + c * 8);
         }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) *reinterpret_cast<uint4 *>(sm + (first + i * kStep) * kPitch + c * 16) = x[i];
         if (tid < kChunk) {
             const int row = r0 + tid;
-            seen[tid] = row < p.R ? drafted_bits(p, b, row / p.g, len) : 0;
+            seen[tid] = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
             // rows that do not exist or see nothing have no weight anywhere
             lse[tid] = row >= p.R || (len == 0 && !seen[tid]) ? INFINITY : p.lse[(long)bh * p.R + row];
         }
@@ -554,12 +546,12 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
     int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : p.rows == 16 ? launch_mma<D, 1, BF16>(p, km, vm, stream) : launch_mma<D, 2, BF16>(p, km, vm, stream);
     if (rc) return rc;
     const long jobs = (long)heads * p.nrb;
-    const bool by_job = jobs < p.shares, wide = jobs * 16 <= p.shares;             // 16 parts a job and more: a row's parts over the warps of a block
+    const bool by_job = jobs < p.shares, wide = jobs * 16 <= p.shares;             // 16 parts a job and more
     const int rows = p.R < p.rows ? p.R : p.rows;
-    const dim3 grid(by_job ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)(wide ? rows : (rows + 7) / 8));
-    auto join = tc ? (wide ? attn_join_kernel<D, 128, BF16, true> : attn_join_kernel<D, 128, BF16, false>)
-                   : (wide ? attn_join_kernel<D, kTile, BF16, true> : attn_join_kernel<D, kTile, BF16, false>);
-    rc = cuda_status(launch_pdl(join, grid, 256, 0, stream, p, (int)by_job), "tree_attention join");
+    const dim3 grid(by_job ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + join_rows<D>() - 1) / join_rows<D>()));
+    auto join = tc ? (wide ? attn_join_kernel<D, 128, BF16, 4> : attn_join_kernel<D, 128, BF16, 1>)
+                   : (wide ? attn_join_kernel<D, kTile, BF16, 4> : attn_join_kernel<D, kTile, BF16, 1>);
+    rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)by_job), "tree_attention join");
     if (rc || !p.weights) return rc;
     if (p.scores)
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");
@@ -573,6 +565,7 @@ size_t tree_attention_workspace_bytes(int B, int S, int nh, int nkv, int D, long
 int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t stream) {
     const Plan pl = plan_of(p.B, p.S, p.nh, p.nkv, p.D, p.T, p.weights != nullptr);
     p.g = p.nh / p.nkv;
+    p.g_inverse = p.g > 1 ? (uint32_t)(((1ull << 32) + p.g - 1) / p.g) : 0;
     p.R = p.S * p.g;
     p.nrb = pl.nrb;
     p.rows = pl.rows;

@@ -123,49 +123,61 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
         // ---------------------------------------------------------------------- products
         const uint32_t fmt = BF16 ? 1u : 0u, base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRowsTc >> 4) << 24);
         const uint32_t id_qk = base | ((uint32_t)(kTileTc >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-        int pn[2] = {0, 0}, pieces = 0;                                          // tiles of a stream so far; pieces so far
-        for (int piece = u0; piece < u1 && ok; ++pieces) {
+        // slots and phases of the next K and the next V of the ring; phases of the streams' barriers, a bit each
+        uint32_t ks = 0, kph = 0, vs = 1, vph = 0, qph = 0, pph = 0;
+        const uint32_t ring = uniform(smem_u32(smem)), qbase = uniform(smem_u32(sm_q)), tm = uniform(tmem);
+        const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
+        auto wait_u = [&](uint32_t bar, uint32_t phase, int code) {
+            if (ok) ok = mbar_wait_warp(g_status_attn_tc, bar, phase, &abort_flag, code);
+            return ok;
+        };
+        for (int piece = u0; piece < u1 && ok;) {
             while (piece >= job.begin + job.nt) job.next(p);
             const int end = min(u1, job.begin + job.nt), tiles = end - piece;
             const bool second = !TWO || (job.job % p.nrb) * kJobRows + kRowsTc < p.R;
             const int live = second ? 2 : 1, steps = TWO ? tiles * live : tiles;
-            auto tile_of = [&](int k) { return TWO ? k / live : k; };
-            auto stream_of = [&](int k) { return second ? k & 1 : 0; };
-            auto qk = [&](int k) {
-                const int x = stream_of(k), item = 2 * (piece - u0 + tile_of(k)), slot = item % kItems;
-                if (!wait(&full[slot], item / kItems, 42)) return;
+            // stream x: step parity where there are two
+            auto qk = [&](uint32_t x) {
+                if (!wait_u(fulls + 8 * ks, kph, 42)) return;
                 tc_fence_after();
+                const uint64_t a = make_smem_desc(qbase + (TWO ? x * kItem : 0)), b = make_smem_desc(ring + ks * kItem);
+                const uint32_t d = tm + x * 128;
+                const bool free = !TWO || x == (uint32_t)live - 1;
                 if (elect_one()) {
-                    const uint32_t a = smem_u32(sm_q + (TWO ? x * kItem : 0)), b = smem_u32(smem + slot * kItem);
 #pragma unroll
-                    for (int s = 0; s < D / 16; ++s)
-                        mma_f16<false>(tmem + x * 128, make_smem_desc(a + (s >> 2) * kHalf + (s & 3) * 32), make_smem_desc(b + (s >> 2) * kHalf + (s & 3) * 32), id_qk, s > 0);
-                    tc_commit(smem_u32(&s_full[x]));
-                    if (!TWO || x == live - 1) tc_commit(smem_u32(&empty[slot]));
+                    for (int s = 0; s < D / 16; ++s) {
+                        const uint64_t off = ((s >> 2) * kHalf + (s & 3) * 32) >> 4;
+                        mma_f16<false>(d, a + off, b + off, id_qk, s > 0);
+                    }
+                    tc_commit(smem_u32(&s_full[0]) + 8 * x);
+                    if (free) tc_commit(empties + 8 * ks);
                 }
                 __syncwarp();
+                if (free) { ks += 2; if (ks >= kItems) { ks -= kItems; kph ^= 1; } }
             };
-            for (int x = 0; x < 2; ++x) wait(&q_full[x], pieces, 43);
+            for (int x = 0; x < 2; ++x) wait_u(smem_u32(&q_full[x]), qph, 43);
+            qph ^= 1;
             tc_fence_after();
-            int done[2] = {0, 0};                                                // tiles of a stream in this piece
-            for (int k = 0; k < min(live, steps) && ok; ++k) qk(k);
+            uint32_t begun = 0;                                                  // streams that have a sum in this piece, a bit each
+            for (int k = 0; k < min(live, steps) && ok; ++k) qk(second ? k & 1 : 0);
             for (int k = 0; k < steps && ok; ++k) {
-                const int x = stream_of(k), item = 2 * (piece - u0 + tile_of(k)) + 1, slot = item % kItems;
-                if (!wait(&p_full[x], pn[x], 44) || !wait(&full[slot], item / kItems, 45)) break;
+                const uint32_t x = second ? k & 1 : 0;
+                if (!wait_u(smem_u32(&p_full[0]) + 8 * x, (pph >> x) & 1, 44) || !wait_u(fulls + 8 * vs, vph, 45)) break;
                 tc_fence_after();
-                const bool last = k + live >= steps;
+                const bool last = k + live >= steps, free = !TWO || x == (uint32_t)live - 1;
+                const uint64_t b = umma_desc_tc(ring + vs * kItem, kHalf, 1024);
+                const uint32_t d = tm + 256 + x * 128, a = tm + x * 128, more = (begun >> x) & 1;
                 if (elect_one()) {
-                    const uint32_t b = smem_u32(smem + slot * kItem);
 #pragma unroll
-                    for (int s = 0; s < kTileTc / 16; ++s)
-                        mma_f16<true>(tmem + 256 + x * 128, tmem + x * 128 + s * 8, umma_desc_tc(b + s * 2048, kHalf, 1024), id_pv, s > 0 || done[x] > 0);
-                    if (!TWO || x == live - 1) tc_commit(smem_u32(&empty[slot]));
-                    if (last) tc_commit(smem_u32(&o_full[x]));
+                    for (int s = 0; s < kTileTc / 16; ++s) mma_f16<true>(d, a + s * 8, b + ((s * 2048) >> 4), id_pv, s > 0 ? 1 : more);
+                    if (free) tc_commit(empties + 8 * vs);
+                    if (last) tc_commit(smem_u32(&o_full[0]) + 8 * x);
                 }
                 __syncwarp();
-                ++done[x];
-                ++pn[x];
-                if (!last) qk(k + live);
+                begun |= 1u << x;
+                pph ^= 1u << x;
+                if (free) { vs += 2; if (vs >= kItems) { vs -= kItems; vph ^= 1; } }
+                if (!last) qk(x);
             }
             piece = end;
         }
@@ -190,8 +202,8 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             uint4 qv[kLoads];
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int from = myrow0 + qr0 + i * kStep, at = min(from, p.R - 1), s = at / p.g, h = kvh * p.g + at - s * p.g;
-                qv[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + b * p.q_sb + s * p.q_ss + h * p.q_sh + c * 8);
+                const int from = myrow0 + qr0 + i * kStep, at = min(from, p.R - 1);
+                qv[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, at) + c * 8);
                 if (from >= p.R) qv[i] = make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
@@ -203,7 +215,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full[x]));
-            const uint64_t seen = row < p.R ? drafted_bits(p, b, row / p.g, len) : 0;
+            const uint64_t seen = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
             const bool stream = !TWO || warp_live || myrow0 < p.R;               // this stream has rows
             float m = -INFINITY, l = 0.0f;
             int mine = 0;                                                        // tiles of this stream in this piece
@@ -317,7 +329,6 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             tc_fence_after();
             const uint64_t nonfinite = bad;
             if (warp_live && ok) {
-                const int s = row / p.g, h = kvh * p.g + row - s * p.g;
                 const float factor = row_factor(sum, len == 0 && !seen), base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 1
                 for (int c0 = col0; c0 < col0 + cols; c0 += 32) {
@@ -340,15 +351,31 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                                 for (int e = 0; e < 32; ++e)
                                     if (e == c) v[e] += add;
                             }
-                        if (whole) {
+                        if (!whole) {
+                            float *dst = p.part_o + part * kJobRows * D + ((c0 >> 2) * kJobRows + (row - row0)) * 4;
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) v[c] *= factor;
-                            store_row_chunk(p.out, BF16, (((long)b * p.S + s) * p.nh + h) * D + c0, v);
-                        } else {
-                            float *dst = p.part_o + (part * kJobRows + (row - row0)) * D + c0;
-#pragma unroll
-                            for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4 *>(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+                            for (int c = 0; c < 32; c += 4) *reinterpret_cast<float4 *>(dst + c * kJobRows) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
                         }
+                    }
+                    if (whole) {
+                        // through the rows' own place in the buffer of q, which is not read any more: a warp then writes whole lines
+                        uint8_t *dst = sm_q + (TWO ? x * kItem : 0) + (c0 >> 6) * kHalf + r * 128;
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+                            *reinterpret_cast<uint4 *>(dst + (((((c0 & 32) + c) >> 3) ^ (r & 7)) << 4)) =
+                                make_uint4(narrow<BF16>(v[c] * factor, v[c + 1] * factor), narrow<BF16>(v[c + 2] * factor, v[c + 3] * factor),
+                                           narrow<BF16>(v[c + 4] * factor, v[c + 5] * factor), narrow<BF16>(v[c + 6] * factor, v[c + 7] * factor));
+                    }
+                }
+                if (whole) {
+                    __syncwarp();
+                    constexpr int kPieces = (TWO ? D : D / 2) / 8, kRowsAtOnce = 32 / kPieces;       // of 16 bytes, of this warp's rows
+                    const int piece_of = col0 / 8 + lane % kPieces;
+#pragma unroll
+                    for (int i = 0; i < 32; i += kRowsAtOnce) {
+                        const int rr = quarter * 32 + i + lane / kPieces, orow = myrow0 + rr, os = token_of(p, orow), oh = kvh * p.g + orow - os * p.g;
+                        const uint4 w = *reinterpret_cast<const uint4 *>(sm_q + (TWO ? x * kItem : 0) + (piece_of >> 3) * kHalf + rr * 128 + (((piece_of & 7) ^ (rr & 7)) << 4));
+                        if (orow < p.R) *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + os) * p.nh + oh) * D + piece_of * 8) = w;
                     }
                 }
                 if (row < p.R && col0 == 0) {
