@@ -12,6 +12,8 @@
 
 namespace flh {
 
+constexpr int kTreeTcTile = 64;            // entries of a key tile of attn_tc_kernel
+
 struct TreeAttnParams {
     const void *q;
     long q_sb, q_ss, q_sh;                 // strides in elements; the head's values are contiguous

@@ -506,7 +506,7 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     pl.rows = R <= 16 ? 16 : R <= kMmaRows ? 32 : R <= 128 ? 128 : 256;
     pl.nrb = (R + pl.rows - 1) / pl.rows;
     pl.shares = pl.rows >= 128 ? kNumSMs : 2 * kNumSMs;
-    pl.min_share = pl.rows >= 128 ? 1 : kWarps;
+    pl.min_share = pl.rows >= 128 ? 2 : kWarps;
     pl.scores = weights && R <= 16;
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
@@ -549,7 +549,7 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
     const bool by_job = jobs < p.shares, wide = jobs * 16 <= p.shares;             // 16 parts a job and more
     const int rows = p.R < p.rows ? p.R : p.rows;
     const dim3 grid(by_job ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + join_rows<D>() - 1) / join_rows<D>()));
-    auto join = tc ? (wide ? attn_join_kernel<D, 128, BF16, 4> : attn_join_kernel<D, 128, BF16, 1>)
+    auto join = tc ? (wide ? attn_join_kernel<D, kTreeTcTile, BF16, 4> : attn_join_kernel<D, kTreeTcTile, BF16, 1>)
                    : (wide ? attn_join_kernel<D, kTile, BF16, 4> : attn_join_kernel<D, kTile, BF16, 1>);
     rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)by_job), "tree_attention join");
     if (rc || !p.weights) return rc;
@@ -577,7 +577,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.scores = pl.scores ? reinterpret_cast<float *>(ws + pl.sc) : nullptr;
     p.score_ld = pl.score_ld;
     CUtensorMap km, vm;
-    const int tile = pl.rows >= 128 ? 128 : kTile;
+    const int tile = pl.rows >= 128 ? kTreeTcTile : kTile;
     int rc = make_map(&km, p.k, bf16, p.D, p.T, (long)p.B * p.nkv, tile);
     if (!rc) rc = make_map(&vm, p.v, bf16, p.D, p.T, (long)p.B * p.nkv, tile);
     if (rc) return rc;

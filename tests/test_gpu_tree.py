@@ -69,6 +69,17 @@ def test_many_sequences_of_uneven_lengths(cuda, S, nh, nkv):
     _check_attention(cuda, q, k, v, _ints(lengths), None)
 
 
+@pytest.mark.parametrize("S,nh", [(3, 4), (9, 4), (20, 4), (33, 8)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_shares(cuda, S, nh, D):
+    """Hundreds of thousands of entries: every ring, barrier and tile of scores is gone around many times, with rows that change their maximum."""
+    lengths = [150001, 90007, 33]
+    T = lengths[0] + S
+    q, k, v = _normal(1, 3, S, nh, D, scale=1.5), _normal(2, 3, 1, T, D), _normal(3, 3, 1, T, D)
+    k[0, 0, :lengths[0]] *= torch.linspace(0.2, 3.0, lengths[0], device="cuda")[:, None].half()
+    _check_attention(cuda, q, k, v, _ints(lengths), None)
+
+
 def test_one_long_sequence(cuda):
     q, k, v = _normal(1, 1, 2, 8, 128, dtype=torch.bfloat16), _normal(2, 1, 1, 70003, 128, dtype=torch.bfloat16), _normal(3, 1, 1, 70003, 128, dtype=torch.bfloat16)
     _check_attention(cuda, q, k, v, _ints([70001]), None)

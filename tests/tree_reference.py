@@ -58,9 +58,11 @@ def attention(q, k, v, lengths, tree=None, scale=None):
             p = torch.where(some, torch.softmax(torch.where(some, x, 0.0), -1), 0.0)
             d = torch.where(seen[:, None] & size.isfinite(), size, 0.0).amax(-1, keepdim=True) * (D + 1) * 2.0 ** -24 + 2.0 ** -21
             # a weight of zero on an entry that is not seen adds nothing, whatever lies there
-            pv = torch.where(seen[:, None, :, None], p[..., None] * vh[None, None], 0.0)
-            o = pv.sum(2)
-            size_o, size_v = pv.abs().sum(2), torch.where(seen[:, None, :, None], vh.abs()[None, None], 0.0).sum(2)
+            o, size_o, size_v = (torch.empty(S, g, D, dtype=torch.float64, device=q.device) for _ in range(3))
+            for s in range(S):
+                at = seen[s].nonzero()[:, 0]
+                pv = p[s][:, at, None] * vh[at]
+                o[s], size_o[s], size_v[s] = pv.sum(1), pv.abs().sum(1), vh[at].abs().sum(0)
             out[b, :, h * g:(h + 1) * g] = o
             tol[b, :, h * g:(h + 1) * g] = u * o.abs() * 1.01 + (u + 2 * d) * size_o * 1.01 + (2.0 ** -25 * (size_v + 1) if q.dtype == torch.float16 else 0.0) + 1e-30
             w[b, h, :total] = torch.where(seen[:, None], p, 0.0).sum((0, 1))
