@@ -370,6 +370,10 @@ def rope_kv_at(qkv, cos, sin, positions, lengths, k_cache, v_cache, nh):
     lengths[b] + s of the caches [B, nkv, T, D]; entries T and up do not exist.  qkv [B*S, (nh + 2 nkv) * D] contiguous, float16 or
     bfloat16; cos, sin f32 [P, D/2]; positions int32 [B, S]; lengths int32 [B].  -> q [B, S, nh, D].  A position that the tables
     do not have makes that token's q and k NaN."""
+    if _host is not None:
+        r = _host.rope_kv_at(qkv, cos, sin, positions, lengths, k_cache, v_cache, nh)
+        if r is not None:
+            return r
     _check_caches(k_cache, v_cache)
     B, nkv, T, D = k_cache.shape
     _check(positions.dim() == 2, "positions must be int32 [B, S]")
@@ -394,6 +398,10 @@ def tree_attention(q, k_cache, v_cache, lengths, tree=None, weights=None, scale=
     nkv; lengths int32 [B]; tree int64 [S] or [B, S], or None for a chain (S = 1: ordinary decode).  scale: 1 / sqrt(D) by default.
     weights (f32 [B, nkv, T]): to every entry is added what all tokens and heads of the group gave it, what
     cache_evict goes by.  -> [B, S, nh, D].  A token that sees no entry has zeros."""
+    if _host is not None:
+        r = _host.tree_attention(q, k_cache, v_cache, lengths, tree, weights, scale)
+        if r is not None:
+            return r
     _check_caches(k_cache, v_cache)
     B, nkv, T, D = k_cache.shape
     _check(q.dim() == 4 and q.shape[0] == B and q.shape[3] == D, "q must be [B, S, heads, D] for caches [B, kv heads, T, D]")
@@ -451,6 +459,10 @@ def cache_accept(k_caches, v_caches, lengths, path, accepted, drafted, weights=N
     accepted[b] entry lengths[b] + path[b, i] moves to lengths[b] + i (path int32 [B, A], accepted int32 [B]), in place and as if
     all were read before any is written.  An index outside 0 .. drafted - 1 leaves entry i as it is.  weights (a list of f32 [B, nkv, T]): moved along, and zero for the drafted
     entries behind the accepted ones.  -> the new lengths, lengths + accepted (int32 [B])."""
+    if _host is not None:
+        r = _host.cache_accept(k_caches, v_caches, weights, lengths, path, accepted, drafted)
+        if r is not None:
+            return r
     B, nkv, T, D, dtype = _check_layers(k_caches, v_caches, weights, lengths)
     _check(1 <= drafted <= _TREE_MAX, f"drafted must be 1 .. {_TREE_MAX}")
     _check(path.dim() == 2 and path.shape[1] <= drafted, "path must be int32 [B, A] with A <= drafted")
@@ -470,6 +482,10 @@ def cache_evict(k_caches, v_caches, weights, lengths, keep, recent):
     stay and, of the others, the keep - recent with the largest weights (lists of f32 [B, nkv, T]; NaN is the largest, ties go to the
     lower index).  What stays moves together in order, in place.  -> (kept int32 [layers, B, nkv, keep]: the entries that
     stayed, -1 behind the last; their weights f32 [layers, B, nkv, T], 0 behind the last; the new lengths int32 [B])."""
+    if _host is not None:
+        r = _host.cache_evict(k_caches, v_caches, weights, lengths, keep, recent)
+        if r is not None:
+            return r
     _check(weights is not None, "weights must be lists of float32 [B, kv heads, T]")
     B, nkv, T, D, dtype = _check_layers(k_caches, v_caches, weights, lengths)
     _check(1 <= keep <= T and 0 <= recent <= keep, "keep must be 1 .. T and recent 0 .. keep")

@@ -30,10 +30,10 @@ namespace {
 bool observed() {
     return at::impl::torch_function_mode_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
 }
-// a contiguous CUDA tensor on `device` (the current one, which is asked for only once a tensor is known to be a CUDA tensor: there may
+// a contiguous (or, with `strides`, any strided) CUDA tensor on `device` (the current one, which is asked for only once a tensor is known to be a CUDA tensor: there may
 // be no driver) with memory of its own kind and nothing wrapped around it
-bool plain(const at::Tensor &t, c10::DeviceIndex device) {
-    if (!t.is_cuda() || t.device().index() != device || t.layout() != at::kStrided || !t.is_contiguous() || t.is_neg() || t.is_conj()) return false;
+bool plain(const at::Tensor &t, c10::DeviceIndex device, bool strides = false) {
+    if (!t.is_cuda() || t.device().index() != device || t.layout() != at::kStrided || (!strides && !t.is_contiguous()) || t.is_neg() || t.is_conj()) return false;
     const c10::DispatchKeySet ks = t.key_set();
     return !ks.has_any(c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched,
                                             c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Batched, c10::DispatchKey::ZeroTensor}));
@@ -209,7 +209,196 @@ PyObject *square(PyObject *, PyObject *x_) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- a KV cache that is drafted into and evicted from -----------------------------------------
+bool is_cache(const at::Tensor &t) { return t.dim() == 4 && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16); }
+int dtype_of(const at::Tensor &t) { return t.scalar_type() == at::kBFloat16 ? FLH_B200_BF16 : FLH_B200_F16; }
+bool ints(const at::Tensor &t, at::IntArrayRef sizes) { return t.scalar_type() == at::kInt && t.sizes() == sizes; }
+
+// tree_attention(q, k, v, lengths, tree or None, weights or None, scale or None) -> out
+PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) Py_RETURN_NONE;
+    const at::Tensor *t[6];
+    for (int i = 0; i < 6; ++i) {
+        t[i] = tensor(args[i]);
+        if (!t[i] && (args[i] != Py_None || i < 4)) Py_RETURN_NONE;
+    }
+    const double given = args[6] == Py_None ? 0 : PyFloat_AsDouble(args[6]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2];
+    if (!q.is_cuda() || observed() || q.dim() != 4 || !is_cache(k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) Py_RETURN_NONE;
+    const c10::DeviceIndex dev = c10::cuda::current_device();
+    for (int i = 0; i < 6; ++i)
+        if (t[i] && !plain(*t[i], dev, i == 0)) Py_RETURN_NONE;
+    const int64_t B = k.size(0), nkv = k.size(1), T = k.size(2), D = k.size(3), S = q.size(1), nh = q.size(2);
+    if (q.size(0) != B || q.size(3) != D || B == 0 || S == 0 || S > FLH_B200_TREE_MAX_TOKENS || nkv == 0 || nh == 0 || nh % nkv || T == 0 || q.stride(3) != 1 || !ints(*t[3], {B}) ||
+        B * nh * S >= 1L << 31)
+        Py_RETURN_NONE;
+    long st[3];
+    for (int i = 0; i < 3; ++i) {
+        st[i] = q.size(i) > 1 ? q.stride(i) : 0;
+        if (st[i] % 8) Py_RETURN_NONE;
+    }
+    if (t[4] && (t[4]->scalar_type() != at::kLong || (t[4]->sizes() != at::IntArrayRef({S}) && t[4]->sizes() != at::IntArrayRef({B, S})))) Py_RETURN_NONE;
+    if (t[5] && (t[5]->scalar_type() != at::kFloat || t[5]->sizes() != at::IntArrayRef({B, nkv, T}))) Py_RETURN_NONE;
+    const float scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)given;
+    const long tree_stride = t[4] && t[4]->dim() == 2 ? S : 0;
+    at::Tensor held[6], out, ws;
+    void *ptr[6] = {};
+    for (int i = 0; i < 6; ++i)
+        if (t[i]) { held[i] = *t[i]; ptr[i] = t[i]->data_ptr(); }
+    const size_t need = flh_b200_tree_attention_workspace_bytes((int)B, (int)S, (int)nh, (int)nkv, (int)D, T, ptr[5] != nullptr);
+    if (!need) Py_RETURN_NONE;
+    int rc;
+    {
+        const Unlocked unlocked;
+        out = empty({B, S, nh, D}, held[0].scalar_type(), held[0]);
+        ws = empty({(int64_t)need}, at::kByte, held[0]);                // of this call alone, freed in stream order when it returns
+        rc = flh_b200_tree_attention(ptr[0], st[0], st[1], st[2], dtype_of(held[0]), ptr[1], ptr[2], static_cast<const int32_t *>(ptr[3]), static_cast<const int64_t *>(ptr[4]),
+                                     tree_stride, scale, out.data_ptr(), static_cast<float *>(ptr[5]), (int)B, (int)S, (int)nh, (int)nkv, (int)D, T, ws.data_ptr(), need,
+                                     c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    if (rc) return failed("tree_attention", rc);
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// rope_kv_at(qkv, cos, sin, positions, lengths, k_cache, v_cache, nh) -> q
+PyObject *rope_kv_at(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 8) Py_RETURN_NONE;
+    const at::Tensor *t[7];
+    for (int i = 0; i < 7; ++i)
+        if (!(t[i] = tensor(args[i]))) Py_RETURN_NONE;
+    const long nh = PyLong_AsLong(args[7]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    const at::Tensor &qkv = *t[0], &cos = *t[1], &sin = *t[2], &pos = *t[3], &k = *t[5], &v = *t[6];
+    if (!qkv.is_cuda() || observed() || !is_cache(k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || qkv.scalar_type() != k.scalar_type()) Py_RETURN_NONE;
+    const c10::DeviceIndex dev = c10::cuda::current_device();
+    for (int i = 0; i < 7; ++i)
+        if (!plain(*t[i], dev)) Py_RETURN_NONE;
+    const int64_t B = k.size(0), nkv = k.size(1), T = k.size(2), D = k.size(3);
+    if (pos.dim() != 2 || B == 0 || nh <= 0 || nh >= 1L << 24) Py_RETURN_NONE;
+    const int64_t S = pos.size(1);
+    if (S == 0 || !ints(pos, {B, S}) || !ints(*t[4], {B}) || qkv.sizes() != at::IntArrayRef({B * S, (nh + 2 * nkv) * D}) || cos.scalar_type() != at::kFloat ||
+        sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.size(1) * 2 != D || sin.sizes() != cos.sizes())
+        Py_RETURN_NONE;
+    at::Tensor held[7], q;
+    void *ptr[7];
+    for (int i = 0; i < 7; ++i) { held[i] = *t[i]; ptr[i] = t[i]->data_ptr(); }
+    const long P = cos.size(0);
+    int rc;
+    {
+        const Unlocked unlocked;
+        q = empty({B, S, nh, D}, held[0].scalar_type(), held[0]);
+        rc = flh_b200_rope_kv_at(ptr[0], dtype_of(held[0]), static_cast<const float *>(ptr[1]), static_cast<const float *>(ptr[2]), P, static_cast<const int32_t *>(ptr[3]),
+                                 static_cast<const int32_t *>(ptr[4]), q.data_ptr(), ptr[5], ptr[6], (int)B, (int)S, (int)nh, (int)nkv, (int)D, T,
+                                 c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    if (rc) return failed("rope_kv_at", rc);
+    return THPVariable_Wrap(std::move(q));
+    END_HANDLE_TH_ERRORS
+}
+
+// the caches of all layers: lists of plain tensors that are alike, weights a list or None
+struct Layers {
+    at::Tensor held[3][FLH_B200_CACHE_MAX_LAYERS];
+    void *ptr[3][FLH_B200_CACHE_MAX_LAYERS];
+    int layers = 0;
+    bool weights = false;
+    // args: lists of k, of v and, at `w`, of the weights
+    bool take(PyObject *k, PyObject *v, PyObject *w, c10::DeviceIndex dev) {
+        PyObject *lists[3] = {k, v, w};
+        weights = w != Py_None;
+        for (int i = 0; i < (weights ? 3 : 2); ++i) {
+            if (!PyList_CheckExact(lists[i])) return false;
+            const Py_ssize_t n = PyList_GET_SIZE(lists[i]);
+            if (i == 0) {
+                if (n < 1 || n > FLH_B200_CACHE_MAX_LAYERS) return false;
+                layers = (int)n;
+            }
+            if (n != layers) return false;
+            for (int j = 0; j < layers; ++j) {
+                const at::Tensor *t = tensor(PyList_GET_ITEM(lists[i], j));
+                if (!t || !plain(*t, dev)) return false;
+                const at::Tensor &first = i || j ? held[0][0] : *t;
+                if (i < 2 ? !is_cache(*t) || t->sizes() != first.sizes() || t->scalar_type() != first.scalar_type()
+                          : t->scalar_type() != at::kFloat || t->sizes() != first.sizes().slice(0, 3))
+                    return false;
+                held[i][j] = *t;                                        // alive while the lock is given up
+                ptr[i][j] = t->data_ptr();
+            }
+        }
+        return true;
+    }
+};
+
+// cache_accept(k list, v list, weights list or None, lengths, path, accepted, drafted) -> now
+PyObject *cache_accept(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 7) Py_RETURN_NONE;
+    const at::Tensor *t[3];
+    for (int i = 0; i < 3; ++i)
+        if (!(t[i] = tensor(args[3 + i])) || !t[i]->is_cuda()) Py_RETURN_NONE;
+    const long drafted = PyLong_AsLong(args[6]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (observed() || drafted < 1 || drafted > FLH_B200_TREE_MAX_TOKENS) Py_RETURN_NONE;
+    const c10::DeviceIndex dev = c10::cuda::current_device();
+    Layers c;
+    if (!plain(*t[0], dev) || !plain(*t[1], dev) || !plain(*t[2], dev) || !c.take(args[0], args[1], args[2], dev)) Py_RETURN_NONE;
+    const at::Tensor lengths = *t[0], path = *t[1], accepted = *t[2], &k = c.held[0][0];
+    const int64_t B = k.size(0), nkv = k.size(1), T = k.size(2), D = k.size(3);
+    if (B == 0 || path.dim() != 2 || path.size(1) > drafted || !ints(lengths, {B}) || !ints(path, {B, path.size(1)}) || !ints(accepted, {B})) Py_RETURN_NONE;
+    void *len_p = lengths.data_ptr(), *path_p = path.data_ptr(), *acc_p = accepted.data_ptr();
+    at::Tensor now;
+    int rc;
+    {
+        const Unlocked unlocked;
+        now = empty({B}, at::kInt, lengths);
+        rc = flh_b200_cache_accept(c.ptr[0], c.ptr[1], c.weights ? reinterpret_cast<float *const *>(c.ptr[2]) : nullptr, c.layers, dtype_of(k), static_cast<const int32_t *>(len_p),
+                                   static_cast<const int32_t *>(path_p), static_cast<const int32_t *>(acc_p), static_cast<int32_t *>(now.data_ptr()), (int)B, (int)nkv, (int)D,
+                                   T, (int)path.size(1), (int)drafted, c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    if (rc) return failed("cache_accept", rc);
+    return THPVariable_Wrap(std::move(now));
+    END_HANDLE_TH_ERRORS
+}
+
+// cache_evict(k list, v list, weights list, lengths, keep, recent) -> (kept, left, now)
+PyObject *cache_evict(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 6) Py_RETURN_NONE;
+    const at::Tensor *len = tensor(args[3]);
+    if (!len || !len->is_cuda()) Py_RETURN_NONE;
+    const long keep = PyLong_AsLong(args[4]), recent = PyLong_AsLong(args[5]);
+    if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (observed() || args[2] == Py_None) Py_RETURN_NONE;
+    const c10::DeviceIndex dev = c10::cuda::current_device();
+    Layers c;
+    if (!plain(*len, dev) || !c.take(args[0], args[1], args[2], dev)) Py_RETURN_NONE;
+    const at::Tensor lengths = *len, &k = c.held[0][0];
+    const int64_t B = k.size(0), nkv = k.size(1), T = k.size(2), D = k.size(3);
+    if (B == 0 || !ints(lengths, {B}) || keep < 1 || keep > T || recent < 0 || recent > keep) Py_RETURN_NONE;
+    void *len_p = lengths.data_ptr();
+    at::Tensor kept, left, now;
+    int rc;
+    {
+        const Unlocked unlocked;
+        kept = empty({c.layers, B, nkv, keep}, at::kInt, lengths);
+        left = empty({c.layers, B, nkv, T}, at::kFloat, lengths);
+        now = empty({B}, at::kInt, lengths);
+        rc = flh_b200_cache_evict(c.ptr[0], c.ptr[1], reinterpret_cast<const float *const *>(c.ptr[2]), c.layers, dtype_of(k), static_cast<const int32_t *>(len_p), (int)keep,
+                                  (int)recent, static_cast<int32_t *>(kept.data_ptr()), static_cast<float *>(left.data_ptr()), static_cast<int32_t *>(now.data_ptr()), (int)B,
+                                  (int)nkv, (int)D, T, c10::cuda::getCurrentCUDAStream(dev).stream());
+    }
+    if (rc) return failed("cache_evict", rc);
+    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(kept)), THPVariable_Wrap(std::move(left)), THPVariable_Wrap(std::move(now)));
+    END_HANDLE_TH_ERRORS
+}
+
+#define FASTCALL(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
+    FASTCALL(tree_attention), FASTCALL(rope_kv_at), FASTCALL(cache_accept), FASTCALL(cache_evict),
     {"square", square, METH_O, nullptr},
     {"act_quant_group", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(act_quant_group)), METH_FASTCALL, nullptr},
     {"act_quant_token", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(act_quant_token)), METH_FASTCALL, nullptr},
