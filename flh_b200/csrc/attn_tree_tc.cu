@@ -9,8 +9,8 @@
 //                    written over S
 //   O += P V         P from tensor memory, V from shared memory as it lies there, read along the entries
 // The scores of the next tile are made while the threads are at this one, so that they wait for a product only when the tensor cores are
-// what bounds the pass.  (128 entries and one tile of scores a stream took 2,300 clocks for 128 x 128 scores, of which the products
-// were 1,090 and the softmax 1,900 with its stream's products behind it; an issuing warp for both streams spent 1,560 on the issue.)
+// what bounds the pass.  What goes from the softmax to the products is a named barrier (56 clocks there and back; a wait on an
+// mbarrier is 120 - 160 even where it does not have to wait, so those that remain are asked before their time has come).
 // With more than 128 rows the two streams are two blocks of rows that share every tile (half the shared-memory traffic and half
 // the reads of K and V); with up to 128 they are the same rows over every other tile, and their results become one at the end of a
 // piece, straight from tensor memory.
@@ -28,6 +28,9 @@ __device__ int g_status_attn_tc[4];
 
 constexpr int kTileTc = kTreeTcTile, kRowsTc = 128;
 constexpr int kThreadsTcA = 384;           // warp 0 TMA, warps 1 and 2 MMA, warps 4 - 7 and 8 - 11 softmax
+// registers: 384 threads are launched with 168; 128 * 112 + 256 * 192 are less than those 64,512
+constexpr int kRegsIssue = 112, kRegsSoftmax = 192;
+static_assert(128 * kRegsIssue + 256 * kRegsSoftmax <= kThreadsTcA * 168, "more registers than the CTA was launched with");
 constexpr float kLag = 8.0f;               // powers of two that the true maximum may be ahead
 
 template <int D> constexpr int item_bytes() { return kTileTc * D * 2; }                         // K or V of a tile
@@ -75,7 +78,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sm_q = smem + kItems * kItem;
-    __shared__ uint64_t full[kItems], empty[kItems], s_full[2][2], p_full[2][2], o_full[2][2], q_full[2];  // [stream][its tiles in turn]
+    __shared__ uint64_t full[kItems], empty[kItems], s_full[2][2], o_full[2][2], q_full[2];  // [stream][its tiles in turn]
     __shared__ unsigned long long bad[2];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
@@ -83,7 +86,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     if (tid == 0) {
         for (int i = 0; i < kItems; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), TWO ? 2 : 1); }
         for (int i = 0; i < 2; ++i) {
-            for (int j = 0; j < 2; ++j) { mbar_init(smem_u32(&s_full[i][j]), 1); mbar_init(smem_u32(&p_full[i][j]), 4); mbar_init(smem_u32(&o_full[i][j]), 1); }
+            for (int j = 0; j < 2; ++j) { mbar_init(smem_u32(&s_full[i][j]), 1); mbar_init(smem_u32(&o_full[i][j]), 1); }
             mbar_init(smem_u32(&q_full[i]), TWO ? 4 : 8);
         }
         abort_flag = 0;
@@ -115,6 +118,8 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     if (u0 < u1) job.seek(p, u0, lane);
 
     // Items 2 i and 2 i + 1 of the ring are K and V of the CTA's tile u0 + i, in slot item % kItems.
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsIssue));
     if (warp == 0) {
         // ---------------------------------------------------------------------- loads
         int item = 0, slot = 0;
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
         const uint32_t fmt = BF16 ? 1u : 0u, base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(kRowsTc >> 4) << 24);
         const uint32_t id_qk = base | ((uint32_t)(kTileTc >> 3) << 17), id_pv = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
         const uint32_t ring = uniform(smem_u32(smem)), qbase = uniform(smem_u32(sm_q) + (TWO ? x * kQ : 0)), tm = uniform(tmem + x * 128);
-        const uint32_t s_bar = uniform(smem_u32(&s_full[x][0])), p_bar = uniform(smem_u32(&p_full[x][0])), o_bar = uniform(smem_u32(&o_full[x][0]));
+        const uint32_t s_bar = uniform(smem_u32(&s_full[x][0])), o_bar = uniform(smem_u32(&o_full[x][0]));
         // the stream's next K and next V: slots 2 i and 2 i + 1 of the ring's kItems, i counting its tiles
         constexpr int kAdvance = TWO ? 2 : 4;
         uint32_t ks = TWO ? 0 : 2 * x, kph = 0, vs = ks + 1, vph = 0, qph = 0, nk = 0, nv = 0;           // nk, nv: tiles so far
@@ -163,8 +168,9 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             qph ^= 1;
             tc_fence_after();
             if (!live) {                                                         // the other stream's tiles: they are not waited for here
-                for (int i = 0; i < 2 * tiles && wait(fulls + 8 * (i & 1 ? vs : ks), i & 1 ? vph : kph, 42); ++i) {
-                    if (elect_one()) mbar_arrive(empties + 8 * (i & 1 ? vs : ks));
+                for (int i = 0; i < 2 * tiles; ++i) {
+                    wait(fulls + 8 * (i & 1 ? vs : ks), i & 1 ? vph : kph, 42);
+                    if (ok && elect_one()) mbar_arrive(empties + 8 * (i & 1 ? vs : ks));
                     __syncwarp();
                     if (i & 1) advance(vs, vph, kAdvance);
                     else advance(ks, kph, kAdvance);
@@ -173,12 +179,12 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 piece = end;
                 continue;
             }
+            // the tile's K is there
             auto qk = [&]() {
-                if (!wait(fulls + 8 * ks, kph, 42)) return;
                 tc_fence_after();
                 const uint64_t a = make_smem_desc(qbase), b = make_smem_desc(ring + ks * kItem);
                 const uint32_t d = tm + (nk & 1) * kTileTc;
-                if (elect_one()) {
+                if (ok && elect_one()) {
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s)
                         mma_f16<false>(d, a + (((s >> 2) * kQHalf + (s & 3) * 32) >> 4), b + (((s >> 2) * kHalf + (s & 3) * 32) >> 4), id_qk, s > 0);
@@ -189,13 +195,18 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 ++nk;
                 advance(ks, kph, kAdvance);
             };
-            for (int i = 0; i < min(mine, 2) && ok; ++i) qk();
-            for (int i = 0; i < mine && ok; ++i) {
-                if (!wait(p_bar + 8 * (nv & 1), nv >> 1, 44) || !wait(fulls + 8 * vs, vph, 45)) break;
+            for (int i = 0; i < min(mine, 2); ++i) {
+                wait(fulls + 8 * ks, kph, 42);
+                qk();
+            }
+            for (int i = 0; i < mine; ++i) {
+                wait(fulls + 8 * vs, vph, 45);
+                if (i + 2 < mine) wait(fulls + 8 * ks, kph, 42);
+                bar_sync_named(3 + 2 * x + (nv & 1), 160);                       // the weights are written
                 tc_fence_after();
                 const uint64_t b = umma_desc_tc(ring + vs * kItem, kHalf, 1024);
                 const uint32_t d = tm + 256, a = tm + (nv & 1) * kTileTc, more = i > 0;
-                if (elect_one()) {
+                if (ok && elect_one()) {
 #pragma unroll
                     for (int s = 0; s < kTileTc / 16; ++s) mma_f16<true>(d, a + s * 8, b + ((s * 2048) >> 4), id_pv, s > 0 ? 1 : more);
                     tc_commit(o_bar + 8 * (nv & 1));
@@ -209,11 +220,13 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
             bar_arrive_named(2, 320);                                            // this warp has seen the piece's q: the next may come (also after a wait that ran out)
             piece = end;
         }
-    } else if (warp >= 4) {
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         // ---------------------------------------------------------------------- softmax of stream x
         const int x = (warp >> 2) - 1, quarter = warp & 3, r = quarter * 32 + lane, wg = tid - 128 - x * 128;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16, ts = tmem + x * 128 + lanes, to = tmem + 256 + x * 128 + lanes;
-        const uint32_t s_bar = smem_u32(&s_full[x][0]), p_bar = smem_u32(&p_full[x][0]), o_bar = smem_u32(&o_full[x][0]);
+        const uint32_t s_bar = smem_u32(&s_full[x][0]), o_bar = smem_u32(&o_full[x][0]);
         uint32_t count = 0, which = 0;                                           // this stream's tiles so far; piece parity
         for (int piece = u0; piece < u1; which ^= 1) {
             while (piece >= job.begin + job.nt) job.next(p);
@@ -253,7 +266,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 const int t = TWO ? i : first_tile + 2 * i, key0 = (piece + t - job.begin) * kTileTc;
                 const bool tail = key0 + kTileTc > len;
                 const uint32_t tile = ts + (count & 1) * kTileTc;
-                if (!wait(s_bar + 8 * (count & 1), count >> 1, 46)) break;
+                wait(s_bar + 8 * (count & 1), count >> 1, 46);
                 tc_fence_after();
                 if (warp_live) {
                     uint32_t s[64];
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     if (i == 0) m = mx;
                     else if (__any_sync(0xffffffffu, (mx > m + kLag || m == -INFINITY) && mx != m)) {
                         // the product before this one has to be done (the one before that is: these scores were made behind it)
-                        if (!wait(o_bar + 8 * ((count - 1) & 1), (count - 1) >> 1, 49)) break;
+                        wait(o_bar + 8 * ((count - 1) & 1), (count - 1) >> 1, 49);
                         tc_fence_after();
                         const float up = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : exp2_approx(m - up);
                         l *= f;
@@ -344,8 +357,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     }
                 }
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_bar + 8 * (count & 1));
+                bar_arrive_named(3 + 2 * x + (count & 1), 160);
             }
             // ------------------------------------------------------------------ the piece's result
             const long part = 2L * blockIdx.x + (piece != u0);
