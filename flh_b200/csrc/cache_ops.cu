@@ -151,14 +151,16 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
-constexpr int kCopies = 8;                 // of each histogram: the weights' leading bits are much alike
+constexpr int kSelKeys = 45056;            // in shared memory, 176 KB
 
 // A block per row.  The smallest key that is kept is found digit by digit, eight bits at a time, by counting the keys that agree with
 // the digits found so far; then the row is walked in order, every warp over a stretch of its own, and what lies above that key is
-// kept, of the equal ones the first few.  The keys stay in shared memory (cap: how many fit; the rest is read again).
+// kept, of the equal ones the first few.  The keys stay in shared memory (cap: how many fit; the rest is read again).  Every lane counts in
+// a histogram of its own: weights are much alike in their leading bits, and with 8 copies of the counters 256 rows of 8,192 took 31 us.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
     extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[256 * kCopies];
+    __shared__ uint32_t hist[256 * 32];    // [digit][lane]
+    __shared__ uint32_t digits[256];
     __shared__ uint32_t found[2];          // prefix, how many of the keys that match it are to be kept
     __shared__ uint32_t above[kSelWarps], equal[kSelWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -183,24 +185,26 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
     for (int i = tid; i < min(cand, cap); i += kSelThreads) keys[i] = order_key(w[i]);
     if (need) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256 * kCopies; i += kSelThreads) hist[i] = 0;
+            for (int i = tid; i < 256 * 32; i += kSelThreads) hist[i] = 0;
             __syncthreads();
             const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
             for (int i = tid; i < cand; i += kSelThreads) {
                 const uint32_t u = key(i);
-                if ((u & mask) == prefix) atomicAdd(&hist[((u >> shift) & 255u) * kCopies + (lane & (kCopies - 1))], 1u);
+                if ((u & mask) == prefix) atomicAdd(&hist[((u >> shift) & 255u) * 32 + lane], 1u);
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 256 / kSelWarps; ++i) {
+                uint32_t c = hist[(warp * (256 / kSelWarps) + i) * 32 + lane];
+                c = __reduce_add_sync(0xffffffffu, c);
+                if (lane == 0) digits[warp * (256 / kSelWarps) + i] = c;
             }
             __syncthreads();
             if (warp == 0) {
                 // lane l: digits 255 - 8 l .. 248 - 8 l, from the largest down
                 uint32_t c[8], sum = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    c[e] = 0;
-#pragma unroll
-                    for (int q = 0; q < kCopies; ++q) c[e] += hist[(255 - 8 * lane - e) * kCopies + q];
-                    sum += c[e];
-                }
+                for (int e = 0; e < 8; ++e) { c[e] = digits[255 - 8 * lane - e]; sum += c[e]; }
                 uint32_t before = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -250,9 +254,10 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
 }
 
 // Rows kept[0 .. m) of K and V to rows 0 .. m - 1, in place.  kept rises, so kept[d] >= d: rows that a batch writes are read by
-// that batch and by earlier ones only.  A block owns a column of a row's 16-byte pieces, reads a batch, then the next one, and
-// writes the first when all its threads have read theirs.
-constexpr int kMoveThreads = 512, kMovePieces = 4;
+// that batch and by earlier ones only.  A block owns a column of a row's 16-byte pieces; while it has one batch of rows to write it
+// reads the next one and the indices of the one after that, and it writes when all its threads have read theirs.  8 pieces a thread:
+// with 4 the move of 512 MB took 131 us, with 8 it is 100 (256 threads; 512 threads and 8 pieces as fast, 1,024 and 2 slower).
+constexpr int kMoveThreads = 256, kMovePieces = 8;
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p, int slab) {
     const int layer = blockIdx.y, unit = blockIdx.x, slabs = p.chunks / slab;
     const int bh = unit / (2 * slabs), sub = unit - bh * 2 * slabs, isv = sub / slabs, c0 = (sub - isv * slabs) * slab;
@@ -267,18 +272,25 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
     uint4 *base = static_cast<uint4 *>(isv ? p.v[layer] : p.k[layer]) + (long)bh * p.T * p.chunks + c;
     const int batch = rows * kMovePieces;
     uint4 x[kMovePieces], y[kMovePieces];
-    int fx[kMovePieces], fy[kMovePieces];
-    auto load = [&](int d0, uint4 (&v)[kMovePieces], int (&f)[kMovePieces]) {
+    int fx[kMovePieces], fy[kMovePieces], fz[kMovePieces];
+    auto indices = [&](int d0, int (&f)[kMovePieces]) {
 #pragma unroll
         for (int j = 0; j < kMovePieces; ++j) {
             const int d = d0 + r + j * rows;
             f[j] = d < end ? kept[d] : d;
-            if (f[j] != d) v[j] = base[(long)f[j] * p.chunks];
         }
     };
-    load(0, x, fx);
+    auto load = [&](int d0, const int (&f)[kMovePieces], uint4 (&v)[kMovePieces]) {
+#pragma unroll
+        for (int j = 0; j < kMovePieces; ++j)
+            if (f[j] != d0 + r + j * rows) v[j] = base[(long)f[j] * p.chunks];
+    };
+    indices(0, fx);
+    indices(batch, fy);
+    load(0, fx, x);
     for (int d0 = 0; d0 < p.keep; d0 += batch) {
-        load(d0 + batch, y, fy);
+        indices(d0 + 2 * batch, fz);
+        load(d0 + batch, fy, y);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kMovePieces; ++j) {
@@ -286,6 +298,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
             if (fx[j] != d) base[(long)d * p.chunks] = x[j];
             x[j] = y[j];
             fx[j] = fy[j];
+            fy[j] = fz[j];
         }
     }
 }
@@ -321,8 +334,8 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     for (int i = 0; i < layers; ++i) { p.k[i] = k[i]; p.v[i] = v[i]; p.w[i] = w[i]; }
     p.lengths = lengths; p.kept = kept; p.now = now; p.left = left;
     p.B = B; p.nkv = nkv; p.keep = keep; p.recent = recent; p.chunks = D / 8; p.T = T;
-    const int cap = (int)(T < 49152 ? T : 49152);
-    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 49152 * 4);
+    const int cap = (int)(T < kSelKeys ? T : kSelKeys);
+    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
     if (e != cudaSuccess) return cuda_status(e, "cache_evict shared memory");
     int rc = cuda_status(launch_pdl(evict_select_kernel, dim3((unsigned)(B * nkv), (unsigned)layers), kSelThreads, (size_t)cap * 4, stream, p, cap), "cache_evict select");
     if (rc) return rc;
