@@ -28,6 +28,7 @@ struct TreeAttnParams {
     int T;
     float scale_log2;                      // scale * log2(e): scores live in powers of two
     int shares, min_share;                 // CTAs, tiles that a share has at least
+    int by_job;                            // a CTA per job: nothing is cut, and there is no join
     float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
@@ -75,6 +76,15 @@ __device__ __forceinline__ int share_tiles(const TreeAttnParams &p, int total) {
 template <int TILE>
 struct JobWalk {
     int b, job, nt, len, begin;            // sequence; job within the sequence (head * nrb + block of rows); its tiles; first tile
+    // job `index` in order; warp-uniform
+    __device__ void at(const TreeAttnParams &p, int index, int lane) {
+        const int per = p.nkv * p.nrb;
+        b = index / per;
+        job = index - b * per;
+        len = uniform(committed(p, b));
+        nt = (entries(p, len) + TILE - 1) / TILE;
+        begin = tiles_before<TILE>(p, b, lane) + job * nt;
+    }
     // from the start of the order to the job of tile u (u < total); warp-uniform
     __device__ void seek(const TreeAttnParams &p, int u, int lane) {
         const int per = p.nkv * p.nrb;
@@ -115,6 +125,22 @@ struct JobWalk {
         }
     }
 };
+
+// Tiles [u0, u1) of this CTA, and the walk at the first of them (u0 < u1)
+template <int TILE>
+__device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, JobWalk<TILE> &job, int &u0, int &u1) {
+    if (p.by_job) {
+        job.at(p, blockIdx.x, lane);
+        u0 = job.begin;
+        u1 = u0 + job.nt;
+        return;
+    }
+    const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
+    const long first = (long)blockIdx.x * share;
+    u0 = (int)min(first, (long)total);
+    u1 = (int)min((long)total, first + share);
+    if (u0 < u1) job.seek(p, u0, lane);
+}
 
 // Two 16-bit values of the tensors' type as binary32, and back.
 template <bool BF16> __device__ __forceinline__ float2 widen(uint32_t w) {

@@ -26,10 +26,11 @@ __device__ int g_status_attn[4];
 constexpr int kTile = 32;                  // keys of a tile
 constexpr int kWarps = 4, kThreadsAttn = kWarps * 32;
 
-template <int MT> constexpr int ring_slots() { return MT == 1 ? 3 : 2; }    // of a warp, so that two CTAs fit an SM; a slot is the K or the V part of a tile
+constexpr int kRows = 16;                  // of a job
+constexpr int kSlots = 3;                  // ring slots of a warp, so that two CTAs fit an SM; a slot is the K or the V part of a tile
 template <int D> constexpr int slot_bytes() { return kTile * D * 2; }
-template <int D, int MT> constexpr int q_pitch() { return D * 2 + 16; }                       // bytes; the 16 keep ldmatrix free of conflicts
-template <int D, int MT> constexpr int attn_smem() { return 1024 + kWarps * ring_slots<MT>() * slot_bytes<D>() + 16 * MT * q_pitch<D, MT>() + kWarps * 16 * MT * 32 * 4; }
+template <int D> constexpr int q_pitch() { return D * 2 + 16; }                       // bytes; the 16 keep ldmatrix free of conflicts
+template <int D> constexpr int attn_smem() { return 1024 + kWarps * kSlots * slot_bytes<D>() + kRows * q_pitch<D>() + kWarps * 4 * 128 * 4; }
 
 __device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -55,15 +56,14 @@ template <int ROWS> __device__ __forceinline__ uint32_t swizzled(int row, int ch
     return (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// MT: blocks of 16 rows of a job.
-template <int D, int MT, bool BF16>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap) {
-    constexpr int kRows = 16 * MT, kNT = kTile / 8, kKS = D / 16, kDT = D / 8, kSlot = slot_bytes<D>(), kSlots = ring_slots<MT>();
+    constexpr int kNT = kTile / 8, kKS = D / 16, kDT = D / 8, kSlot = slot_bytes<D>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t *sm_q = smem + kWarps * kSlots * kSlot;
-    float *sm_o = reinterpret_cast<float *>(sm_q + kRows * q_pitch<D, MT>());      // [warp][row][32 columns]
+    float *sm_o = reinterpret_cast<float *>(sm_q + kRows * q_pitch<D>());      // [warp][rows][D], 512 values a warp
     __shared__ uint64_t full[kWarps][kSlots];
     __shared__ uint64_t seen[kRows];
     __shared__ unsigned long long bad;
@@ -80,12 +80,10 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
     pdl_wait();
     pdl_trigger();
 
-    const int total = tiles_before<kTile>(p, p.B, lane), share = share_tiles(p, total);
-    const long first = (long)blockIdx.x * share;
-    if (first >= total) return;
-    const int u0 = (int)first, u1 = (int)min((long)total, first + share);
     JobWalk<kTile> cur, ahead;             // the job worked on, and the one that the loads have come to
-    cur.seek(p, u0, lane);
+    int u0, u1;
+    take_share(p, lane, cur, u0, u1);
+    if (u0 >= u1) return;
     ahead = cur;
 
     // item i of this warp: K (i even) or V (i odd) of its tile i / 2, into slot i % kSlots
@@ -104,65 +102,61 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
         ++item;
     };
     for (int i = 0; i < kSlots; ++i) issue();
+    const bool few = p.R <= 8;
     int used = 0;                          // items taken from the ring
     bool alive = true;
 
+    // rows of q of a job: 16-byte piece q_c of every kQStep-th row, fetched while the job before is finished
+    constexpr int kQStep = kThreadsAttn / (D / 8), kQLoads = kRows / kQStep;
+    const int q_c = tid % (D / 8), q_r = tid / (D / 8);
+    uint4 qv[kQLoads];
+    auto fetch_q = [&](const JobWalk<kTile> &j) {
+        const int kvh = j.job / p.nrb, row0 = (j.job - kvh * p.nrb) * kRows;
+#pragma unroll
+        for (int i = 0; i < kQLoads; ++i) {
+            const int row = row0 + q_r + i * kQStep;
+            qv[i] = row < p.R ? ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, j.b, kvh, row) + q_c * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    fetch_q(cur);
     for (int piece = u0; piece < u1;) {
-        while (piece >= cur.begin + cur.nt) cur.next(p);
         const int piece_end = min(u1, cur.begin + cur.nt);
         const int b = cur.b, kvh = cur.job / p.nrb, row0 = (cur.job - kvh * p.nrb) * kRows, len = cur.len, n = entries(p, len);
-        // rows of q, and what they see of the drafted entries
         __syncthreads();                   // the piece before is written out
-        for (int i = tid; i < kRows * (D / 8); i += kThreadsAttn) {
-            const int r = i / (D / 8), c = i - r * (D / 8), row = row0 + r;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (row < p.R) {
-                x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, row) + c * 8);
-            }
-            *reinterpret_cast<uint4 *>(sm_q + r * q_pitch<D, MT>() + c * 16) = x;
-        }
+#pragma unroll
+        for (int i = 0; i < kQLoads; ++i) *reinterpret_cast<uint4 *>(sm_q + (q_r + i * kQStep) * q_pitch<D>() + q_c * 16) = qv[i];
         if (tid < kRows) seen[tid] = row0 + tid < p.R ? drafted_bits(p, b, token_of(p, row0 + tid), len) : 0;
         if (tid == 0) bad = 0;
         __syncthreads();
-        float o[MT][kDT][4], m[MT][2], l[MT][2];
+        float o[kDT][4], m[2], l[2];
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            m[t][0] = m[t][1] = -INFINITY;
-            l[t][0] = l[t][1] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kDT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.0f;
-        }
+        for (int i = 0; i < kDT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
         int u = piece + ((u0 + warp - piece) % kWarps + kWarps) % kWarps;
         for (; u < piece_end && alive; u += kWarps) {
             const int key0 = (u - cur.begin) * kTile;
-            // scores: 16 MT rows by 32 keys
-            float sc[MT][kNT][4];
+            // scores: 16 rows by 32 keys
+            float sc[kNT][4];
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int i = 0; i < kNT; ++i) sc[t][i][0] = sc[t][i][1] = sc[t][i][2] = sc[t][i][3] = 0.0f;
+            for (int i = 0; i < kNT; ++i) sc[i][0] = sc[i][1] = sc[i][2] = sc[i][3] = 0.0f;
             int slot = used % kSlots;
             alive = mbar_wait_warp(g_status_attn, full_u + 8 * slot, (used / kSlots) & 1, &abort_flag, 31);
             if (!alive) break;
             const uint32_t ks = ring_u + slot * kSlot;
 #pragma unroll
             for (int k2 = 0; k2 < kKS / 2; ++k2) {                              // 32 values of the heads at a time
-                uint32_t a[MT][8];
+                uint32_t a[8];
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-                        ldsm4(smem_u32(sm_q) + (t * 16 + (lane & 15)) * q_pitch<D, MT>() + (k2 * 4 + hh * 2 + (lane >> 4)) * 16,
-                              a[t][4 * hh], a[t][4 * hh + 1], a[t][4 * hh + 2], a[t][4 * hh + 3]);
+                for (int hh = 0; hh < 2; ++hh)
+                    ldsm4(smem_u32(sm_q) + (lane & 15) * q_pitch<D>() + (k2 * 4 + hh * 2 + (lane >> 4)) * 16,
+                          a[4 * hh], a[4 * hh + 1], a[4 * hh + 2], a[4 * hh + 3]);
 #pragma unroll
                 for (int i = 0; i < kNT; ++i) {
                     uint32_t b0, b1, b2, b3;
                     ldsm4(ks + swizzled<kTile>(i * 8 + (lane & 7), k2 * 4 + (lane >> 3)), b0, b1, b2, b3);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        mma16816<BF16>(sc[t][i], a[t][0], a[t][1], a[t][2], a[t][3], b0, b1);
-                        mma16816<BF16>(sc[t][i], a[t][4], a[t][5], a[t][6], a[t][7], b2, b3);
-                    }
+                    mma16816<BF16>(sc[i], a[0], a[1], a[2], a[3], b0, b1);
+                    mma16816<BF16>(sc[i], a[4], a[5], a[6], a[7], b2, b3);
                 }
             }
             __syncwarp();
@@ -171,59 +165,57 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const bool tail = key0 + kTile > len;                              // drafted entries, or none at all, in this tile
             if (tail) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
+                for (int hh = 0; hh < 2; ++hh) {
+                    // a bit for each of the 32 entries: committed, or drafted and seen
+                    const uint64_t bits = seen[grp + hh * 8];
+                    const int j0 = key0 - len;
+                    const uint32_t vis = (j0 >= 64 ? 0u : j0 >= 0 ? (uint32_t)(bits >> j0) : ((uint32_t)bits << -j0) | ((1u << -j0) - 1)) >> (quad * 2);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint64_t bits = seen[t * 16 + grp + (e >> 1) * 8];
+                    for (int i = 0; i < kNT; ++i)
 #pragma unroll
-                        for (int i = 0; i < kNT; ++i) {
-                            const int j = key0 + i * 8 + quad * 2 + (e & 1) - len;
-                            if (j >= 0 && (j >= 64 || !((bits >> j) & 1))) sc[t][i][e] = -INFINITY;
-                        }
-                    }
+                        for (int e = 0; e < 2; ++e)
+                            if (!((vis >> (i * 8 + e)) & 1)) sc[i][2 * hh + e] = -INFINITY;
+                }
             }
             if (p.scores) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {
-                        const int row = row0 + t * 16 + grp + hh * 8;
-                        if (row < p.R) {
-                            float *dst = p.scores + (((long)b * p.nkv + kvh) * p.R + row) * p.score_ld + key0 + quad * 2;
-#pragma unroll
-                            for (int i = 0; i < kNT; ++i)
-                                *reinterpret_cast<float2 *>(dst + i * 8) = make_float2(sc[t][i][2 * hh], sc[t][i][2 * hh + 1]);
-                        }
-                    }
-            }
-            // running maximum and sum; the sum is of the exponentials in binary32, before they are rounded for the product
-            uint32_t pr[MT][kNT][2];
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    float mx = -INFINITY;
+                    const int row = row0 + grp + hh * 8;
+                    if (row < p.R) {
+                        float *dst = p.scores + (((long)b * p.nkv + kvh) * p.R + row) * p.score_ld + key0 + quad * 2;
 #pragma unroll
-                    for (int i = 0; i < kNT; ++i) mx = fmaxf(mx, fmaxf(sc[t][i][2 * hh], sc[t][i][2 * hh + 1]));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    mx *= p.scale_log2;                                         // scale > 0
-                    const float was = m[t][hh], now = fmaxf(was, mx), base = now == -INFINITY ? 0.0f : now;
-                    m[t][hh] = now;
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kNT; ++i) {
-                        const float x = exp2_approx(fmaf(sc[t][i][2 * hh], p.scale_log2, -base)), y = exp2_approx(fmaf(sc[t][i][2 * hh + 1], p.scale_log2, -base));
-                        sum += x + y;
-                        pr[t][i][hh] = narrow<BF16>(x, y);
-                    }
-                    const float keep = exp2_approx(was - base);
-                    l[t][hh] = l[t][hh] * keep + sum;
-                    if (__any_sync(0xffffffffu, now != was)) {
-#pragma unroll
-                        for (int i = 0; i < kDT; ++i) { o[t][i][2 * hh] *= keep; o[t][i][2 * hh + 1] *= keep; }
+                        for (int i = 0; i < kNT; ++i)
+                            *reinterpret_cast<float2 *>(dst + i * 8) = make_float2(sc[i][2 * hh], sc[i][2 * hh + 1]);
                     }
                 }
+            }
+            // running maximum and sum; the sum is of the exponentials in binary32, before they are rounded for the product
+            uint32_t pr[kNT][2] = {};
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                if (hh && few) break;                                            // rows 8 and up do not exist
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kNT; ++i) mx = fmaxf(mx, fmaxf(sc[i][2 * hh], sc[i][2 * hh + 1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                mx *= p.scale_log2;                                         // scale > 0
+                const float was = m[hh], now = fmaxf(was, mx), base = now == -INFINITY ? 0.0f : now;
+                m[hh] = now;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kNT; ++i) {
+                    const float x = exp2_approx(fmaf(sc[i][2 * hh], p.scale_log2, -base)), y = exp2_approx(fmaf(sc[i][2 * hh + 1], p.scale_log2, -base));
+                    sum += x + y;
+                    pr[i][hh] = narrow<BF16>(x, y);
+                }
+                const float keep = exp2_approx(was - base);
+                l[hh] = l[hh] * keep + sum;
+                if (__any_sync(0xffffffffu, now != was)) {
+#pragma unroll
+                    for (int i = 0; i < kDT; ++i) { o[i][2 * hh] *= keep; o[i][2 * hh + 1] *= keep; }
+                }
+            }
             slot = used % kSlots;
             alive = mbar_wait_warp(g_status_attn, full_u + 8 * slot, (used / kSlots) & 1, &abort_flag, 32);
             if (!alive) break;
@@ -251,11 +243,8 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
                 for (int i = 0; i < kDT; i += 2) {
                     uint32_t b0, b1, b2, b3;
                     ldsm4t(vs + swizzled<kTile>(k * 16 + (lane & 15), i + (lane >> 4)), b0, b1, b2, b3);
-#pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        mma16816<BF16>(o[t][i], pr[t][2 * k][0], pr[t][2 * k][1], pr[t][2 * k + 1][0], pr[t][2 * k + 1][1], b0, b1);
-                        mma16816<BF16>(o[t][i + 1], pr[t][2 * k][0], pr[t][2 * k][1], pr[t][2 * k + 1][0], pr[t][2 * k + 1][1], b2, b3);
-                    }
+                    mma16816<BF16>(o[i], pr[2 * k][0], pr[2 * k][1], pr[2 * k + 1][0], pr[2 * k + 1][1], b0, b1);
+                    mma16816<BF16>(o[i + 1], pr[2 * k][0], pr[2 * k][1], pr[2 * k + 1][0], pr[2 * k + 1][1], b2, b3);
                 }
             }
             if (tail) fence_proxy_async();                                      // the slot was written here: TMA writes it next
@@ -265,41 +254,46 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
         }
         // the warps' results, each relative to its own maximum, become one
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                float sum = l[t][hh];
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (quad == 0) { sm_m[warp][t * 16 + grp + hh * 8] = m[t][hh]; sm_l[warp][t * 16 + grp + hh * 8] = sum; }
-            }
+        for (int hh = 0; hh < 2; ++hh) {
+            float sum = l[hh];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (quad == 0) { sm_m[warp][grp + hh * 8] = m[hh]; sm_l[warp][grp + hh * 8] = sum; }
+        }
         __syncthreads();
-        float mine[MT][2];
+        float mine[2];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int hh = 0; hh < 2; ++hh) {
+            const int r = grp + hh * 8;
+            float top = sm_m[0][r];
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const int r = t * 16 + grp + hh * 8;
-                float top = sm_m[0][r];
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-                mine[t][hh] = exp2_approx(m[t][hh] - (top == -INFINITY ? 0.0f : top));
-            }
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
+            mine[hh] = exp2_approx(m[hh] - (top == -INFINITY ? 0.0f : top));
+        }
         const bool whole = piece == cur.begin && piece_end == cur.begin + cur.nt;
         const long part = 2L * blockIdx.x + (piece != u0);
+        JobWalk<kTile> next = cur;
+        if (piece_end < u1) {
+            next.next(p);
+            fetch_q(next);
+        }
+        constexpr int kChunk = 4 * 128 / D;                                      // rows whose sums of all warps fit the buffer (8 KB)
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {                                      // 32 columns at a time
+        for (int r0 = 0; r0 < kRows; r0 += kChunk) {
+            if (row0 + r0 >= p.R) break;
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+            for (int hh = 0; hh < 2; ++hh) {
+                const int r = hh * 8 + grp;
+                if (r / kChunk == r0 / kChunk) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-                        *reinterpret_cast<float2 *>(sm_o + (warp * kRows + t * 16 + grp + hh * 8) * 32 + ((i * 8 + quad * 2) ^ ((grp & 3) * 8))) =
-                            make_float2(o[t][c * 4 + i][2 * hh] * mine[t][hh], o[t][c * 4 + i][2 * hh + 1] * mine[t][hh]);
+                    for (int i = 0; i < kDT; ++i)
+                        *reinterpret_cast<float2 *>(sm_o + (warp * kChunk + r - r0) * D + i * 8 + quad * 2) = make_float2(o[i][2 * hh] * mine[hh], o[i][2 * hh + 1] * mine[hh]);
+                }
+            }
             __syncthreads();
-            for (int i = tid; i < kRows * 32; i += kThreadsAttn) {
-                const int r = i >> 5, col = i & 31, row = row0 + r;
+#pragma unroll
+            for (int i = tid; i < kChunk * D; i += kThreadsAttn) {
+                const int r = r0 + i / D, d = i % D, row = row0 + r;
                 if (row >= p.R) continue;
                 float top = sm_m[0][r], sum = 0.0f, acc = 0.0f;
 #pragma unroll
@@ -308,9 +302,8 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
                     sum += sm_l[w][r] * exp2_approx(sm_m[w][r] - base);
-                    acc += sm_o[(w * kRows + r) * 32 + (col ^ ((r & 3) * 8))];
+                    acc += sm_o[(w * kChunk + r - r0) * D + d];
                 }
-                const int d = c * 32 + col;
                 if (bad) acc += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, row, d, len, base);
                 if (whole) {
                     const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
@@ -323,32 +316,31 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
                     else p.part_ml[part * kRows + r] = make_float2(top, sum);
                 }
             }
-            __syncthreads();
+            if (r0 + kChunk < kRows) __syncthreads();
         }
         piece = piece_end;
+        cur = next;
     }
 }
 
 // Jobs that several shares hold: their partial results in order.  A block for each job, or for each cut between two shares where that is
-// fewer (it takes the job that is cut there, if that is the job's first cut), and a few of its rows: a thread for four columns of a
-// row, 8 rows next to one another in a warp so that it reads whole lines.  WAYS groups of threads share out the parts of a job.
-template <int D> constexpr int join_rows() { return 1024 / D; }
-template <int D, int TILE, bool BF16, int WAYS>
-__global__ void __launch_bounds__(256 * WAYS) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
-    __shared__ float sm_acc[WAYS > 1 ? WAYS - 1 : 1][5][256];
-    const int lane = threadIdx.x & 31, way = threadIdx.x >> 8, t = threadIdx.x & 255;
-    const int group = t / join_rows<D>(), r = blockIdx.y * join_rows<D>() + t % join_rows<D>();
+// fewer (it takes the job that is cut there, if that is the job's first cut), for 8 of its rows and 4 GROUPS columns; a thread for four
+// columns of a row, the 8 rows next to one another in a warp so that it reads whole lines, and WAYS sets of threads that share
+// out the parts.  The parts' factors come first, each from one thread.  Few jobs in many parts take 32 columns a block and 16 ways (one
+// sequence of 60,000 entries, 8 rows: 59 -> 19 us with its attention), others all columns and 256 threads (16 jobs of 256 rows: 94 -> 84 us).
+constexpr int kJoinRows = 8, kMaxParts = 2 * kNumSMs;
+template <int D, int TILE, bool BF16, int GROUPS, int WAYS>
+__global__ void __launch_bounds__(8 * GROUPS * WAYS) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+    __shared__ float factor_of[kMaxParts][kJoinRows], reduced[GROUPS * WAYS / 4][kJoinRows];
+    __shared__ float4 sm_acc[WAYS][8 * GROUPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, way = tid / (8 * GROUPS);
+    const int r_in = tid & 7, r = blockIdx.y * kJoinRows + r_in, group = blockIdx.z * GROUPS + (tid >> 3) % GROUPS;
     pdl_wait();
     pdl_trigger();
     const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
     JobWalk<TILE> job;
     if (by_job) {
-        const int per = p.nkv * p.nrb;
-        job.b = blockIdx.x / per;
-        job.job = blockIdx.x - job.b * per;
-        job.len = committed(p, job.b);
-        job.nt = (entries(p, job.len) + TILE - 1) / TILE;
-        job.begin = tiles_before<TILE>(p, job.b, lane) + job.job * job.nt;
+        job.at(p, blockIdx.x, lane);
     } else {
         const long cut = (blockIdx.x + 1L) * share;
         if (cut >= total) return;
@@ -362,31 +354,53 @@ __global__ void __launch_bounds__(256 * WAYS) attn_join_kernel(const __grid_cons
     // only the first of these CTAs can have begun with another job
     const bool behind = (long)c0 * share != job.begin;
     auto slot = [&](int i) { return 2L * (c0 + i) + (i == 0 && behind); };
+    // a row's values in lanes 8 apart, then over the warps
+    auto over_block = [&](float x, bool max) {
+        for (int o = 8; o < 32; o <<= 1) { const float y = __shfl_xor_sync(0xffffffffu, x, o); x = max ? fmaxf(x, y) : x + y; }
+        if (lane < 8) reduced[warp][lane] = x;
+        __syncthreads();
+        x = reduced[0][r_in];
+#pragma unroll
+        for (int w = 1; w < GROUPS * WAYS / 4; ++w) x = max ? fmaxf(x, reduced[w][r_in]) : x + reduced[w][r_in];
+        __syncthreads();
+        return x;
+    };
+    // a thread for every kThreads-th part of a row
+    constexpr int kThreads = GROUPS * WAYS, kEach = (kMaxParts + kThreads - 1) / kThreads;
+    float2 ml[kEach];
     float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int i = (tid >> 3) + k * kThreads;
+        ml[k] = live && i < parts ? p.part_ml[slot(i) * p.rows + r] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[k].x);
+    }
+    top = over_block(top, true);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int i = (tid >> 3) + k * kThreads;
+        const float f = exp2_approx(ml[k].x - base);
+        if (i < parts) factor_of[i][r_in] = f;
+        sum += ml[k].y * f;
+    }
+    sum = over_block(sum, false);
     float4 acc = make_float4(0, 0, 0, 0);
     if (live) {
 #pragma unroll 8
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, p.part_ml[slot(i) * p.rows + r].x);
-    }
-    const float base = top == -INFINITY ? 0.0f : top;
-    if (live) {
-#pragma unroll 8
         for (int i = way; i < parts; i += WAYS) {
-            const float2 ml = p.part_ml[slot(i) * p.rows + r];
             const float4 v = *reinterpret_cast<const float4 *>(p.part_o + slot(i) * p.rows * D + ((long)group * p.rows + r) * 4);
-            const float f = exp2_approx(ml.x - base);
-            sum += ml.y * f;
+            const float f = factor_of[i][r_in];
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
     }
     if (WAYS > 1) {
-        if (way) { float(*x)[256] = sm_acc[way - 1]; x[0][t] = acc.x; x[1][t] = acc.y; x[2][t] = acc.z; x[3][t] = acc.w; x[4][t] = sum; }
+        sm_acc[way][tid % (8 * GROUPS)] = acc;
         __syncthreads();
-        if (way) return;
-#pragma unroll
-        for (int w = 0; w < WAYS - 1; ++w) { acc.x += sm_acc[w][0][t]; acc.y += sm_acc[w][1][t]; acc.z += sm_acc[w][2][t]; acc.w += sm_acc[w][3][t]; sum += sm_acc[w][4][t]; }
     }
-    if (!live) return;
+    if (way || !live) return;
+#pragma unroll
+    for (int w = 1; w < WAYS; ++w) { const float4 v = sm_acc[w][tid]; acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w; }
     const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
     const float factor = row_factor(sum, sum == 0.0f && job.len == 0 && !drafted_bits(p, b, s, job.len));
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + s) * p.nh + h) * D + group * 4) =
@@ -493,20 +507,24 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
 }
 
 // ---- host side ------------------------------------------------------------------------------
-constexpr int kMmaRows = 16;
 struct Plan {
     int rows, nrb, shares, min_share;
-    bool scores;
+    bool by_job, scores;
     long score_ld;
     size_t part_o, part_ml, lse, sc, total;        // offsets in the workspace
 };
 Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     Plan pl = {};
     const int R = S * (nh / nkv);
-    pl.rows = R <= 16 ? 16 : R <= kMmaRows ? 32 : R <= 128 ? 128 : 256;
+    pl.rows = R <= 16 ? 16 : R <= 128 ? 128 : 256;
     pl.nrb = (R + pl.rows - 1) / pl.rows;
     pl.shares = pl.rows >= 128 ? kNumSMs : 2 * kNumSMs;
     pl.min_share = pl.rows >= 128 ? 2 : kWarps;
+    // A CTA per job where the longest job (of a full cache) would not take much longer than an even share: what is saved is the join
+    // and the second piece of most CTAs.  In tiles of that share: 24 of 32 entries (one sequence of 500 entries, 32 heads: 13.7 -> 10.1 us),
+    // 12 of 64 entries on the tensor cores.
+    const long jobs = (long)B * nkv * pl.nrb, tile = pl.rows >= 128 ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile;
+    pl.by_job = jobs <= pl.shares && nt - nt * jobs / pl.shares <= (pl.rows >= 128 ? 12 : 24);
     pl.scores = weights && R <= 16;
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
@@ -530,28 +548,30 @@ int make_map(CUtensorMap *map, const void *base, bool bf16, int D, long T, long 
     return r == CUDA_SUCCESS ? 0 : fail(FLH_B200_EINVAL, "the cache cannot be described to TMA (%d)", (int)r);
 }
 
-template <int D, int MT, bool BF16>
+template <int D, bool BF16>
 int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
-    auto kern = attn_mma_kernel<D, MT, BF16>;
-    constexpr int smem = attn_smem<D, MT>();
+    auto kern = attn_mma_kernel<D, BF16>;
+    constexpr int smem = attn_smem<D>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.by_job ? p.B * p.nkv * p.nrb : p.shares)), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 template <int D, bool BF16>
 int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     const unsigned heads = (unsigned)(p.B * p.nkv);
     const bool tc = p.rows >= 128;
-    int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : p.rows == 16 ? launch_mma<D, 1, BF16>(p, km, vm, stream) : launch_mma<D, 2, BF16>(p, km, vm, stream);
+    int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : launch_mma<D, BF16>(p, km, vm, stream);
     if (rc) return rc;
     const long jobs = (long)heads * p.nrb;
-    const bool by_job = jobs < p.shares, wide = jobs * 16 <= p.shares;             // 16 parts a job and more
-    const int rows = p.R < p.rows ? p.R : p.rows;
-    const dim3 grid(by_job ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + join_rows<D>() - 1) / join_rows<D>()));
-    auto join = tc ? (wide ? attn_join_kernel<D, kTreeTcTile, BF16, 4> : attn_join_kernel<D, kTreeTcTile, BF16, 1>)
-                   : (wide ? attn_join_kernel<D, kTile, BF16, 4> : attn_join_kernel<D, kTile, BF16, 1>);
-    rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)by_job), "tree_attention join");
+    if (!p.by_job) {
+        const bool each = jobs < p.shares, wide = jobs * 16 <= p.shares;           // a block per job; 16 parts a job and more
+        const int rows = p.R < p.rows ? p.R : p.rows;
+        const dim3 grid(each ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + kJoinRows - 1) / kJoinRows), wide ? D / 32 : 1);
+        auto join = tc ? (wide ? attn_join_kernel<D, kTreeTcTile, BF16, 8, 16> : attn_join_kernel<D, kTreeTcTile, BF16, D / 4, 128 / D>)
+                       : (wide ? attn_join_kernel<D, kTile, BF16, 8, 16> : attn_join_kernel<D, kTile, BF16, D / 4, 128 / D>);
+        rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)each), "tree_attention join");
+    }
     if (rc || !p.weights) return rc;
     if (p.scores)
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");
@@ -571,6 +591,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.rows = pl.rows;
     p.shares = pl.shares;
     p.min_share = pl.min_share;
+    p.by_job = pl.by_job;
     p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + pl.part_ml);
     p.lse = p.weights ? reinterpret_cast<float *>(ws + pl.lse) : nullptr;

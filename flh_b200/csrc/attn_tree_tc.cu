@@ -105,9 +105,6 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     pdl_wait();
     pdl_trigger();
 
-    const int total = tiles_before<kTileTc>(p, p.B, lane), share = share_tiles(p, total);
-    const long first = (long)blockIdx.x * share;
-    const int u0 = (int)min(first, (long)total), u1 = (int)min((long)total, first + share);
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t phase, int code) {
         if (ok) ok = mbar_wait_warp(g_status_attn_tc, bar, phase & 1, &abort_flag, code);
@@ -115,7 +112,8 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     };
     const uint32_t fulls = smem_u32(full), empties = smem_u32(empty);
     JobWalk<kTileTc> job;
-    if (u0 < u1) job.seek(p, u0, lane);
+    int u0, u1;
+    take_share(p, lane, job, u0, u1);
 
     // Items 2 i and 2 i + 1 of the ring are K and V of the CTA's tile u0 + i, in slot item % kItems.
     if (warp < 4) {
@@ -465,7 +463,7 @@ int launch_tc(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap 
     constexpr int smem = smem_tc<D, TWO>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.by_job ? p.B * p.nkv * p.nrb : p.shares)), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 }  // namespace
