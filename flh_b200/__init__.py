@@ -16,6 +16,6 @@ from . import _lib
 if "flh_b200.build" not in getattr(sys, "orig_argv", []):
     _lib.load()
 
-from . import _CUDA, functional, hadamard, nn  # noqa: E402
+from . import _CUDA, draft, functional, hadamard, nn  # noqa: E402
 
-__all__ = ["_CUDA", "functional", "hadamard", "nn"]
+__all__ = ["_CUDA", "draft", "functional", "hadamard", "nn"]

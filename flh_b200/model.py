@@ -37,6 +37,8 @@ class DecoderConfig:
     n_layers: int = 32
     vocab: int = 32000
     rope_theta: float = 10000.0
+    max_positions: int = 32768           # rows of the rotary tables that Decoder.draft reads (built at its first call): tokens behind
+                                         # them come out as NaN
     eps: float = 1e-5
     act_mode: str = "group_sym"          # or "token_asym"
     tp: int = 1
@@ -142,14 +144,24 @@ class DecoderLayer(torch.nn.Module):
             return s.view(lead + (cfg.hidden // 128,)), None, q.view(lead + (cfg.hidden // 2,))
         return quant(norm(x))
 
-    def forward(self, x, pos, cache=None, tables=None, shape=None, pre=None, next_layer=None):
+    def _attend_drafted(self, qkv, cache, tables, draft):
+        """Attention of drafted tokens behind sequences of their own lengths (Decoder.draft): [B, S, heads * D]."""
+        lengths, positions, bits = draft
+        q = _CUDA.rope_kv_at(qkv.view(-1, qkv.shape[-1]), tables[0], tables[1], positions, lengths, cache[0], cache[1], self.nh)
+        att = _CUDA.tree_attention(q, cache[0], cache[1], lengths, tree=bits, weights=cache[3] if len(cache) > 3 else None)
+        return att.view(qkv.shape[0], qkv.shape[1], -1)
+
+    def forward(self, x, pos, cache=None, tables=None, shape=None, pre=None, next_layer=None, draft=None):
         """x [B, S, hidden] f16 (or, sequence-parallel, this rank's B S / tp rows with shape = (B, S, blocks)); pos [S]
         absolute positions; cache = (k, v) [B, nkv, T, D] with a write cursor `cache[2]`, or None for a cache-less prefill;
         tables = rope_tables(pos, ...) shared by the layers.
         Tensor-parallel decode with tp.enable_one_shot(): the all-reduce behind o_proj / down_proj, the residual add, the
         RMS-norm and the quantiser of the next linear's input run as ONE launch, and x is then updated in place.  For
         down_proj the next linear belongs to `next_layer`: the layer returns (x, pre) and the caller hands `pre` (that
-        layer's quantised input) to it."""
+        layer's quantised input) to it.
+        draft = (lengths, positions, tree bits): the tokens are drafted ones behind entries lengths[b] of the cache, tables are
+        over all positions (Decoder.draft).  A cache with accumulated weights (Decoder.new_cache(observe=True)) gets those of the
+        last 64 tokens of a call."""
         cfg = self.cfg
         sp = x.dim() == 2                                # sequence-parallel: x holds this rank's T / tp of the B * S rows (tp.local_rows)
         if sp:
@@ -167,9 +179,14 @@ class DecoderLayer(torch.nn.Module):
             q, s = q.view(B, S, -1), s.view(B, S, -1)
             z = None if z is None else z.view(B, S, -1)
         qkv = self.qkv(q, s, z)
+        if draft is not None:
+            with timing.region("attention"):
+                att = self._attend_drafted(qkv, cache, tables, draft)
+            return self._after_attention(x, att, sp, blocks if sp else None, next_layer)
         with timing.region("glue"):
             mask, causal = None, S > 1
             cur = 0 if cache is None else cache[2]
+            observe = cache is not None and len(cache) > 3
             if cfg.fuse_glue and qkv.dtype == torch.float16:
                 # one kernel: rotary embedding of q and k, q laid out for the attention call, k and v written at their cache positions
                 if tables is None:
@@ -182,9 +199,14 @@ class DecoderLayer(torch.nn.Module):
                 # q stays in token order: the attention output follows its layout and needs no transposing copy
                 qh = torch.empty((B, S, self.nh, hd), dtype=qkv.dtype, device=qkv.device)
                 _CUDA.rope_kv(qkv.view(B * S, -1), tables[0], tables[1], qh, kc, vc, B, S, self.nh, self.nkv, cur, q_by_token=True)
+                if observe:
+                    last = min(S, 64)
+                    seen = _CUDA.tree_attention(qh[:, S - last:], kc, vc, torch.full((B,), cur + S - last, dtype=torch.int32, device=x.device), weights=cache[3])
                 qh = qh.transpose(1, 2)
                 kh, vh = kc[:, :, :cur + S], vc[:, :, :cur + S]
             else:
+                if observe:
+                    raise RuntimeError("a cache with accumulated weights needs fuse_glue and float16")
                 qh, kh, vh = qkv.split((self.nh * hd, self.nkv * hd, self.nkv * hd), dim=-1)
                 qh = rope(qh.view(B, S, self.nh, hd), pos, cfg.rope_theta).transpose(1, 2)
                 kh = rope(kh.view(B, S, self.nkv, hd), pos, cfg.rope_theta).transpose(1, 2)
@@ -199,8 +221,17 @@ class DecoderLayer(torch.nn.Module):
                 # triangle with the top-left corner, which is only right for cur = 0)
                 mask, causal = torch.ones(S, cur + S, dtype=torch.bool, device=x.device).tril(diagonal=cur), False
         with timing.region("attention"):
-            att = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=causal, enable_gqa=self.nh != self.nkv)
-            att = att.transpose(1, 2).reshape(B, S, self.nh * hd)
+            if observe and S <= 64:
+                att = seen.view(B, S, self.nh * hd)      # all of the call's tokens: the same attention
+            else:
+                att = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=causal, enable_gqa=self.nh != self.nkv)
+                att = att.transpose(1, 2).reshape(B, S, self.nh * hd)
+        return self._after_attention(x, att, sp, blocks if sp else None, next_layer)
+
+    def _after_attention(self, x, att, sp, blocks, next_layer):
+        """o_proj, the residual, the MLP: what follows the attention output att [B, S, heads * D] in forward()."""
+        cfg = self.cfg
+        S = att.shape[1]
         with timing.region("quant"):
             s, z, q = self.q_attn(att)
         fused = None
@@ -262,6 +293,7 @@ class Decoder(torch.nn.Module):
         self.embed.weight.data.copy_(torch.randn(cfg.vocab, cfg.hidden, device=device, generator=rep).half())
         self.layers = torch.nn.ModuleList(DecoderLayer(cfg, device, gen, group) for _ in range(cfg.n_layers))
         self.norm = RMSNorm(cfg.hidden, cfg.eps).to(device)
+        self._tables = None                              # rotary tables of draft()
         self.head = torch.nn.Linear(cfg.hidden, cfg.vocab, bias=False, device=device, dtype=torch.float16) if with_head else None
         if self.head is not None:
             self.head.weight.data.copy_((torch.randn(cfg.vocab, cfg.hidden, device=device, generator=rep) * cfg.hidden ** -0.5).half())
@@ -273,12 +305,55 @@ class Decoder(torch.nn.Module):
                 m.prepack_int8()
         return self
 
-    def new_cache(self, batch, max_len):
+    def new_cache(self, batch, max_len, observe=False):
+        """A list of [k, v, cursor] per layer.  observe: [k, v, cursor, weights], where every call adds to weights (f32 [B, kv heads,
+        max_len]) the attention that its last 64 tokens gave each entry, which evict() goes by."""
         c = self.cfg
         nkv = max(c.n_kv_heads // c.tp, 1)
         return [[torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device),
                  torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device), 0]
+                + ([torch.zeros(batch, nkv, max_len, dtype=torch.float32, device=self.device)] if observe else [])
                 for _ in range(c.n_layers)]
+
+    @torch.no_grad()
+    def draft(self, ids, cache, lengths, tree=None, positions=None):
+        """One pass over drafted tokens ids [B, S] (S = 1 .. 64): token s of sequence b goes to entry lengths[b] + s of the cache and sees
+        the entries before lengths[b] and its ancestors in `tree` (a DraftTree; None: a chain, each token the child of the one
+        before).  lengths int32 [B]: entries that the sequences have, each its own.  positions int32 [B]: how many tokens they are
+        long, where entries were evicted (default: lengths).  -> logits [B, S, vocab] of all tokens (the normed hidden states without
+        a head).  lengths and positions are read on the device: a recorded step follows them.  What is kept of the tokens is
+        what accept() is told."""
+        B, S = ids.shape
+        if self._tables is None:
+            self._tables = rope_tables(torch.arange(self.cfg.max_positions, device=self.device), self.cfg.head_dim, self.cfg.rope_theta)
+        at = lengths if positions is None else positions
+        at = at[:, None] + (torch.arange(S, dtype=torch.int32, device=self.device) if tree is None else tree.depth)
+        bits = None if tree is None else tree.bits
+        x, pre = self.embed(ids), None
+        for i, layer in enumerate(self.layers):
+            out = layer(x, None, cache[i], self._tables, pre=pre, next_layer=self.layers[i + 1] if i + 1 < len(self.layers) else None,
+                        draft=(lengths, at, bits))
+            x, pre = out if isinstance(out, tuple) else (out, None)
+        x = self.norm(x)
+        return x if self.head is None else self.head(x)
+
+    @torch.no_grad()
+    def accept(self, cache, lengths, path, accepted, drafted):
+        """Keeps entries path[b, :accepted[b]] (int32 [B, A], from the root down) of the `drafted` ones behind lengths[b], in all
+        layers.  -> the new lengths."""
+        return _CUDA.cache_accept([c[0] for c in cache], [c[1] for c in cache], lengths, path, accepted, drafted,
+                                  weights=[c[3] for c in cache] if len(cache[0]) > 3 else None)
+
+    @torch.no_grad()
+    def evict(self, cache, lengths, keep, recent):
+        """Down to `keep` entries of each head in a cache made with observe=True: the last `recent` and those that got the most attention.
+        -> the new lengths; the tokens that follow go through draft() with the positions they would have had."""
+        if len(cache[0]) < 4:
+            raise RuntimeError("evict needs a cache with accumulated weights (new_cache(observe=True))")
+        _, left, now = _CUDA.cache_evict([c[0] for c in cache], [c[1] for c in cache], [c[3] for c in cache], lengths, keep, recent)
+        for c, w in zip(cache, left.unbind(0)):
+            c[3].copy_(w)                                # in place: a recorded step goes on adding to it
+        return now
 
     @torch.no_grad()
     def forward(self, ids, cache=None, start=0):

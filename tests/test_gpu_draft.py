@@ -1,0 +1,158 @@
+"""Decoder.draft / accept / evict: drafted tokens through the whole decoder against the plain forward of each branch."""
+import pytest
+import torch
+
+from flh_b200.draft import DraftTree
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(mode="group_sym", **other):
+    from flh_b200.model import Decoder, DecoderConfig
+    cfg = dict(hidden=256, n_heads=4, n_kv_heads=2, ffn=512, n_layers=2, vocab=128, act_mode=mode, max_positions=512)
+    return Decoder(DecoderConfig(**{**cfg, **other}), torch.device("cuda"), seed=5)
+
+
+def _ids(seed, *shape):
+    return torch.randint(0, 128, shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def _near(a, b):
+    # a code of the second layer that flips by one step with the last bit of the first layer's attention moves the logits by a
+    # percent or two of their range (tests/test_gpu_model.py)
+    err = (a.float() - b.float()).abs().max() / b.float().abs().max()
+    assert err < 3e-2, err
+
+
+@pytest.mark.parametrize("mode,hidden", [("group_sym", 256), ("token_asym", 256), ("group_sym", 512)])
+def test_tree_equals_every_branch(cuda, mode, hidden):
+    m = _model(mode, hidden=hidden)
+    prompt, tree = _ids(2, 2, 20), DraftTree([-1, 0, 0, 1, 1, 2, 4], "cuda")
+    ids = _ids(3, 2, tree.size)
+    cache = m.new_cache(2, 64)
+    m(prompt, cache=cache, start=0)
+    lengths = torch.tensor([20, 20], dtype=torch.int32, device="cuda")
+    logits = m.draft(ids, cache, lengths, tree)
+    assert logits.shape == (2, tree.size, 128)
+    for i in range(tree.size):
+        branch = [j for j in range(tree.size) if (int(tree.bits[i]) >> j) & 1]
+        _near(logits[:, i:i + 1], m(torch.cat((prompt, ids[:, branch]), dim=1)))
+
+
+def test_sequences_of_their_own_lengths_and_the_next_step(cuda):
+    """Two sequences accept different branches; the step behind them sees what they accepted."""
+    m = _model()
+    prompt, tree = _ids(4, 2, 12), DraftTree([-1, 0, 0, 2, 3], "cuda")
+    ids, nxt = _ids(5, 2, 5), _ids(6, 2, 3)
+    cache = m.new_cache(2, 40)
+    m(prompt, cache=cache, start=0)
+    lengths = torch.tensor([12, 9], dtype=torch.int32, device="cuda")          # the second sequence is shorter
+    m.draft(ids, cache, lengths, tree)
+    path = torch.tensor([[0, 2, 3, 4], [0, 1, 0, 0]], dtype=torch.int32, device="cuda")
+    now = m.accept(cache, lengths, path, torch.tensor([4, 2], dtype=torch.int32, device="cuda"), tree.size)
+    assert now.tolist() == [16, 11]
+    logits = m.draft(nxt, cache, now)                                          # a chain
+    for b, (n, branch) in enumerate(((12, [0, 2, 3, 4]), (9, [0, 1]))):
+        whole = torch.cat((prompt[b, :n], ids[b, branch], nxt[b]))[None]
+        for i in range(3):
+            _near(logits[b:b + 1, i:i + 1], m(whole[:, :n + len(branch) + 1 + i]))
+
+
+def test_a_recorded_draft_follows_the_lengths(cuda):
+    m = _model()
+    prompt, tree = _ids(7, 2, 24), DraftTree([-1, 0, 0], "cuda")
+    cache = m.new_cache(2, 64)
+    m(prompt, cache=cache, start=0)
+    ids, lengths = _ids(8, 2, 3), torch.tensor([24, 24], dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.draft(ids, cache, lengths, tree)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = m.draft(ids, cache, lengths, tree)
+    for n in ([10, 17], [24, 1]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        ids.copy_(_ids(sum(n), 2, 3))
+        kv = [[c[0].clone(), c[1].clone()] for c in cache]
+        g.replay()
+        got = out.clone()
+        for c, (k, v) in zip(cache, kv):
+            c[0].copy_(k), c[1].copy_(v)
+        assert torch.equal(got, m.draft(ids, cache, lengths, tree))
+        for c, (k, v) in zip(cache, kv):
+            c[0].copy_(k), c[1].copy_(v)
+
+
+@pytest.mark.parametrize("S", [1, 30, 100])
+def test_observed_weights(cuda, S):
+    """They sum to the tokens and heads that were counted, and the logits are those of a cache without them."""
+    m = _model(n_heads=4, n_kv_heads=2)
+    first, then = _ids(9, 2, 40), _ids(10, 2, S)
+    plain, cache = m.new_cache(2, 160), m.new_cache(2, 160, observe=True)
+    m(first, cache=plain, start=0), m(first, cache=cache, start=0)
+    _near(m(then, cache=cache, start=40), m(then, cache=plain, start=40))
+    for c in cache:
+        total = 2.0 * (40 + min(S, 64))                                        # two query heads a kv head; 40 tokens, then the last 64
+        assert torch.allclose(c[3].sum(-1), torch.full((2, 2), total, device="cuda"), rtol=1e-4)
+        assert not c[3][:, :, 40 + S:].any() and bool((c[3][:, :, :40 + S] > 0).all())
+
+
+def test_evict_and_go_on(cuda):
+    """What was evicted is not seen any more, tokens keep their positions, and evicting nothing changes nothing."""
+    m = _model()
+    prompt = _ids(11, 2, 60)
+    cache, same = m.new_cache(2, 100, observe=True), m.new_cache(2, 100, observe=True)
+    m(prompt, cache=cache, start=0), m(prompt, cache=same, start=0)
+    lengths = torch.tensor([60, 60], dtype=torch.int32, device="cuda")
+    assert m.evict(same, lengths, 60, 10).tolist() == [60, 60]
+    for a, b in zip(cache, same):
+        assert all(torch.equal(x, y) for x, y in zip((a[0], a[1], a[3]), (b[0], b[1], b[3])))
+    before = [[c[0].clone(), c[1].clone(), c[3].clone()] for c in cache]
+    now = m.evict(cache, lengths, 24, 8)
+    assert now.tolist() == [24, 24]
+    step, positions = _ids(12, 2, 1), torch.tensor([60, 60], dtype=torch.int32, device="cuda")
+    for c, (k, v, w) in zip(cache, before):
+        assert torch.equal(c[0][:, :, 16:24], k[:, :, 52:60]) and not c[3][:, :, 24:].any()
+        # the 16 heaviest of the first 52
+        heavy = w[:, :, :52].topk(16, dim=-1).indices.sort(dim=-1).values
+        assert torch.equal(c[1][:, :, :16], v.gather(2, heavy[..., None].expand(2, 2, 16, v.shape[-1])))
+    got = m.draft(step, cache, now, positions=positions)
+    # the same step on a cache where the others were never there
+    clean = m.new_cache(2, 100, observe=True)
+    for c, d in zip(cache, clean):
+        d[0][:, :, :24], d[1][:, :, :24] = c[0][:, :, :24], c[1][:, :, :24]
+    assert torch.equal(got, m.draft(step, clean, now, positions=positions))
+    with pytest.raises(RuntimeError, match="observe"):
+        m.evict(m.new_cache(2, 10), lengths, 5, 1)
+
+
+def test_speculative_run_equals_one_token_at_a_time(cuda):
+    """Greedy decoding with trees that hold the right token now and then gives the tokens of greedy decoding without them."""
+    m = _model()
+    prompt = _ids(13, 1, 16)
+    lengths = torch.tensor([16], dtype=torch.int32, device="cuda")
+    one, cache = m.new_cache(1, 128), m.new_cache(1, 128)
+    first = m(prompt, cache=one, start=0)[:, -1].argmax(-1)
+    m(prompt, cache=cache, start=0)
+    # greedy, a token at a time, through draft() with one token: the same kernels and row order of the quantisers
+    want, tok, at = [], first, lengths.clone()
+    for _ in range(24):
+        logits = m.draft(tok[:, None], one, at)
+        want.append((int(tok), logits[0, 0].float().topk(2).values))
+        tok, at = logits[:, 0].argmax(-1), at + 1
+    tree, got, tok, step = DraftTree([-1, 0, 0, 1, 2], "cuda"), [], first, 0
+    while len(got) < 20:
+        guess = [w[0] for w in want[len(got) + 1:len(got) + 3]]
+        wrong = [(g + 1) % 128 for g in guess]
+        ids = [int(tok)] + ([guess[0], wrong[0], guess[1] if step % 2 else wrong[1], guess[1]] if step % 3 else [wrong[0], wrong[0], guess[1], guess[1]])
+        ids = torch.tensor([ids], device="cuda")
+        logits = m.draft(ids, cache, lengths, tree)
+        path, accepted, tok = tree.accept_greedy(ids, logits)
+        n = int(accepted)
+        assert n == (1 if step % 3 == 0 else 3 if step % 2 else 2)
+        got += [int(ids[0, int(i)]) for i in path[0, :n]]
+        lengths = m.accept(cache, lengths, path, accepted, tree.size)
+        step += 1
+        assert got == [w[0] for w in want[:len(got)]]
