@@ -2,16 +2,21 @@
 // the join of partial results.
 //
 // Rows: the S drafted tokens of a sequence times the g query heads that share a kv head are R = S g rows over the same keys;
-// row r is token r / g, head r % g of the group.  A job is a block of rows of one (sequence, kv head); its keys come in tiles.  All
-// tiles of all jobs in a row (sequence, then head, then block of rows) are cut into equal shares, one for each CTA, wherever the
-// cuts fall: a batch of uneven lengths is as balanced as one long sequence, and the lengths are read on the device, so that a
-// recorded launch follows them.  A job that lies within one share is finished there; of a job that was cut each CTA
-// writes a partial result (sum of exponentials, maximum, weighted sum of V) to a slot of its own and the join kernel adds them in order.
+// row r is token r / g, head r % g of the group.  A job is a block of rows of one (sequence, kv head); its keys come in tiles.  The
+// lengths are read on the device, so that a recorded launch follows them, and so is the division of the work among the CTAs:
+//   kEven   all tiles of all jobs in a row (sequence, then head, then block of rows) are cut into equal shares, wherever the cuts fall:
+//           a batch of uneven lengths is as balanced as one long sequence.  For more jobs than CTAs, or many sequences.
+//   kParts  every job is cut into parts of nearly the same size, as many as its length is worth, a CTA for each: no CTA has
+//           parts of two jobs, whose second one costs it what several tiles do (q, the ramp of the rings, the result).
+//   kJobs   a CTA for each job; nothing is cut.
+// A job that lies within one CTA is finished there; of a job that was cut each CTA writes a partial result (sum of exponentials,
+// maximum, weighted sum of V) to a slot of its own and the join kernel adds them in order.
 #pragma once
 #include "tc_common.cuh"
 
 namespace flh {
 
+enum { kEven, kParts, kJobs };
 constexpr int kTreeTcTile = 64;            // entries of a key tile of attn_tc_kernel
 
 struct TreeAttnParams {
@@ -28,7 +33,7 @@ struct TreeAttnParams {
     int T;
     float scale_log2;                      // scale * log2(e): scores live in powers of two
     int shares, min_share;                 // CTAs, tiles that a share has at least
-    int by_job;                            // a CTA per job: nothing is cut, and there is no join
+    int split;                             // kEven, kParts, kJobs
     float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
@@ -126,20 +131,64 @@ struct JobWalk {
     }
 };
 
+// kParts: the parts that the jobs of a sequence are cut into.  Lane l has those of sequence l (at most 32, and no more jobs than CTAs).
+template <int TILE>
+struct Parts {
+    int nt, parts, size, first;            // tiles of a job, its parts, tiles of a part (the last may have fewer), first CTA of the sequence
+    __device__ __forceinline__ void find(const TreeAttnParams &p, int lane) {
+        const int per = p.nkv * p.nrb;
+        nt = lane < p.B ? (entries(p, committed(p, lane)) + TILE - 1) / TILE : 0;
+        int total = nt, longest = nt;
+        for (int o = 16; o; o >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, o);
+            longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+        }
+        // the smallest size for which there are CTAs enough, of 32 between an even share and the longest job (which always is)
+        const int even = max((total * per + p.shares - 1) / p.shares, p.min_share);
+        const int tried = lane == 31 ? max(longest, 1) : even + even * lane / 16;
+        int count = 0;
+        for (int i = 0; i < p.B; ++i) count += (__shfl_sync(0xffffffffu, nt, i) + tried - 1) / tried;
+        const unsigned fits = __ballot_sync(0xffffffffu, (long)count * per <= p.shares);
+        size = __shfl_sync(0xffffffffu, tried, __ffs(fits) - 1);
+        parts = (nt + size - 1) / size;
+        size = nt ? (nt + parts - 1) / parts : 1;
+        parts = (nt + size - 1) / size;
+        int incl = parts * per;
+        for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += t; }
+        first = incl - parts * per;
+    }
+};
+
 // Tiles [u0, u1) of this CTA, and the walk at the first of them (u0 < u1)
 template <int TILE>
 __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, JobWalk<TILE> &job, int &u0, int &u1) {
-    if (p.by_job) {
+    if (p.split == kJobs) {
         job.at(p, blockIdx.x, lane);
         u0 = job.begin;
         u1 = u0 + job.nt;
-        return;
+    } else if (p.split == kParts) {
+        Parts<TILE> c;
+        c.find(p, lane);
+        const int per = p.nkv * p.nrb, cta = blockIdx.x;
+        const unsigned at = __ballot_sync(0xffffffffu, lane < p.B && cta < c.first + c.parts * per);
+        u0 = u1 = 0;
+        if (!at) return;
+        const int b = __ffs(at) - 1;
+        const int first = uniform(__shfl_sync(0xffffffffu, c.first, b)), parts = uniform(__shfl_sync(0xffffffffu, c.parts, b)), size = uniform(__shfl_sync(0xffffffffu, c.size, b));
+        job.b = b;
+        job.job = (cta - first) / parts;
+        job.len = uniform(committed(p, b));
+        job.nt = (entries(p, job.len) + TILE - 1) / TILE;
+        job.begin = 0;                     // its own count of tiles
+        u0 = (cta - first - job.job * parts) * size;
+        u1 = min(u0 + size, job.nt);
+    } else {
+        const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
+        const long first = (long)blockIdx.x * share;
+        u0 = (int)min(first, (long)total);
+        u1 = (int)min((long)total, first + share);
+        if (u0 < u1) job.seek(p, u0, lane);
     }
-    const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
-    const long first = (long)blockIdx.x * share;
-    u0 = (int)min(first, (long)total);
-    u1 = (int)min((long)total, first + share);
-    if (u0 < u1) job.seek(p, u0, lane);
 }
 
 // Two 16-bit values of the tensors' type as binary32, and back.

@@ -337,22 +337,35 @@ __global__ void __launch_bounds__(8 * GROUPS * WAYS) attn_join_kernel(const __gr
     const int r_in = tid & 7, r = blockIdx.y * kJoinRows + r_in, group = blockIdx.z * GROUPS + (tid >> 3) % GROUPS;
     pdl_wait();
     pdl_trigger();
-    const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
     JobWalk<TILE> job;
-    if (by_job) {
-        job.at(p, blockIdx.x, lane);
+    int c0, parts;                         // CTAs c0 .. c0 + parts - 1 have the job
+    bool behind = false;                   // the first of them has begun with another job: the only one that can have
+    if (p.split == kParts) {
+        Parts<TILE> c;
+        c.find(p, lane);
+        const int per = p.nkv * p.nrb;
+        job.b = blockIdx.x / per;
+        job.job = blockIdx.x - job.b * per;
+        job.len = committed(p, job.b);
+        parts = __shfl_sync(0xffffffffu, c.parts, job.b);
+        c0 = __shfl_sync(0xffffffffu, c.first, job.b) + job.job * parts;
     } else {
-        const long cut = (blockIdx.x + 1L) * share;
-        if (cut >= total) return;
-        job.seek(p, (int)cut, lane);
-        if (job.begin == cut || job.begin / share != (int)blockIdx.x) return;
+        const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
+        if (by_job) {
+            job.at(p, blockIdx.x, lane);
+        } else {
+            const long cut = (blockIdx.x + 1L) * share;
+            if (cut >= total) return;
+            job.seek(p, (int)cut, lane);
+            if (job.begin == cut || job.begin / share != (int)blockIdx.x) return;
+        }
+        c0 = job.begin / share;
+        parts = (job.begin + job.nt - 1) / share - c0 + 1;
+        behind = (long)c0 * share != job.begin;
     }
-    const int c0 = job.begin / share, parts = (job.begin + job.nt - 1) / share - c0 + 1;
     if (parts == 1) return;
     const int kvh = job.job / p.nrb, row0 = (job.job - kvh * p.nrb) * p.rows, row = row0 + r, b = job.b;
     const bool live = r < p.rows && row < p.R;
-    // only the first of these CTAs can have begun with another job
-    const bool behind = (long)c0 * share != job.begin;
     auto slot = [&](int i) { return 2L * (c0 + i) + (i == 0 && behind); };
     // a row's values in lanes 8 apart, then over the warps
     auto over_block = [&](float x, bool max) {
@@ -509,7 +522,8 @@ __global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __
 // ---- host side ------------------------------------------------------------------------------
 struct Plan {
     int rows, nrb, shares, min_share;
-    bool by_job, scores;
+    int split;
+    bool scores;
     long score_ld;
     size_t part_o, part_ml, lse, sc, total;        // offsets in the workspace
 };
@@ -522,9 +536,9 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     pl.min_share = pl.rows >= 128 ? 2 : kWarps;
     // A CTA per job where the longest job (of a full cache) would not take much longer than an even share: what is saved is the join
     // and the second piece of most CTAs.  In tiles of that share: 24 of 32 entries (one sequence of 500 entries, 32 heads: 13.7 -> 10.1 us),
-    // 12 of 64 entries on the tensor cores.
+    // 12 of 64 entries on the tensor cores.  Else parts of the jobs, where that is worked out quickly.
     const long jobs = (long)B * nkv * pl.nrb, tile = pl.rows >= 128 ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile;
-    pl.by_job = jobs <= pl.shares && nt - nt * jobs / pl.shares <= (pl.rows >= 128 ? 12 : 24);
+    pl.split = jobs > pl.shares ? kEven : nt - nt * jobs / pl.shares <= (pl.rows >= 128 ? 12 : 24) ? kJobs : B <= 32 ? kParts : kEven;
     pl.scores = weights && R <= 16;
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
@@ -554,7 +568,7 @@ int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap
     constexpr int smem = attn_smem<D>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.by_job ? p.B * p.nkv * p.nrb : p.shares)), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.split == kJobs ? p.B * p.nkv * p.nrb : p.shares)), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 template <int D, bool BF16>
@@ -564,8 +578,8 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
     int rc = tc ? launch_attn_tc(p, p.rows, BF16, km, vm, stream) : launch_mma<D, BF16>(p, km, vm, stream);
     if (rc) return rc;
     const long jobs = (long)heads * p.nrb;
-    if (!p.by_job) {
-        const bool each = jobs < p.shares, wide = jobs * 16 <= p.shares;           // a block per job; 16 parts a job and more
+    if (p.split != kJobs) {
+        const bool each = p.split == kParts || jobs < p.shares, wide = jobs * 16 <= p.shares;           // a block per job; 16 parts a job and more
         const int rows = p.R < p.rows ? p.R : p.rows;
         const dim3 grid(each ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + kJoinRows - 1) / kJoinRows), wide ? D / 32 : 1);
         auto join = tc ? (wide ? attn_join_kernel<D, kTreeTcTile, BF16, 8, 16> : attn_join_kernel<D, kTreeTcTile, BF16, D / 4, 128 / D>)
@@ -591,7 +605,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.rows = pl.rows;
     p.shares = pl.shares;
     p.min_share = pl.min_share;
-    p.by_job = pl.by_job;
+    p.split = pl.split;
     p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + pl.part_ml);
     p.lse = p.weights ? reinterpret_cast<float *>(ws + pl.lse) : nullptr;

@@ -463,7 +463,7 @@ int launch_tc(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap 
     constexpr int smem = smem_tc<D, TWO>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.by_job ? p.B * p.nkv * p.nrb : p.shares)), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.split == kJobs ? p.B * p.nkv * p.nrb : p.shares)), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 }  // namespace
