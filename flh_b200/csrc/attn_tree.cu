@@ -422,101 +422,141 @@ __global__ void __launch_bounds__(8 * GROUPS * WAYS) attn_join_kernel(const __gr
 }
 
 // weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
-// 2 D for reading K again).  A thread per entry.
-constexpr int kWeightThreads = 256;
+// 2 D for reading K again).  A thread has four entries, 256 apart, so that it waits for memory once for all of them.
+constexpr int kWeightThreads = 256, kWeightEach = 4;
 __global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __grid_constant__ TreeAttnParams p) {
-    const int bh = blockIdx.x, t = blockIdx.y * kWeightThreads + threadIdx.x;
+    const int bh = blockIdx.x, t0 = blockIdx.y * kWeightThreads * kWeightEach + threadIdx.x;
     pdl_wait();
     pdl_trigger();
-    const int b = bh / p.nkv, len = committed(p, b);
-    if (t >= entries(p, len)) return;
-    const float *sc = p.scores + (long)bh * p.R * p.score_ld + t, *lse = p.lse + (long)bh * p.R;
-    float sum = 0.0f;
-    for (int r = 0; r < p.R; ++r) {
-        if (t >= len && !((drafted_bits(p, b, token_of(p, r), len) >> (t - len)) & 1)) continue;         // an entry that the row does not see
-        sum += exp2_approx(fmaf(sc[r * p.score_ld], p.scale_log2, -lse[r]));
+    const int b = bh / p.nkv, len = committed(p, b), n = entries(p, len);
+    if (t0 >= n) return;
+    const float *sc = p.scores + (long)bh * p.R * p.score_ld, *lse = p.lse + (long)bh * p.R;
+    float *w = p.weights + (long)bh * p.T, was[kWeightEach], sum[kWeightEach] = {};
+#pragma unroll
+    for (int k = 0; k < kWeightEach; ++k) {
+        const int t = t0 + k * kWeightThreads;
+        was[k] = t < n ? w[t] : 0.0f;
     }
-    p.weights[(long)bh * p.T + t] += sum;
+    for (int r = 0; r < p.R; ++r) {
+        const float at = lse[r];
+#pragma unroll
+        for (int k = 0; k < kWeightEach; ++k) {
+            const int t = t0 + k * kWeightThreads;
+            if (t >= n || (t >= len && !((drafted_bits(p, b, token_of(p, r), len) >> (t - len)) & 1))) continue;      // an entry that the row does not see
+            sum[k] += exp2_approx(fmaf(sc[r * p.score_ld + t], p.scale_log2, -at));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kWeightEach; ++k) {
+        const int t = t0 + k * kWeightThreads;
+        if (t < n) w[t] = was[k] + sum[k];
+    }
 }
 
-// The same for many rows, from K and q again: a warp keeps 16 keys in registers, the rows pass through shared memory 64 at a time.
+// The same for many rows, from K and q again: a block has 128 entries, a warp keeps 16 of them in registers, the rows pass through
+// shared memory 64 at a time, fetched while the 64 before are worked on.
+constexpr int kWeightKeys = 128, kWeightMmaThreads = 256;
+template <int D> constexpr int weights_smem() { return (kWeightKeys + 64) * (D * 2 + 16); }
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreadsAttn) attn_weights_mma_kernel(const __grid_constant__ TreeAttnParams p) {
+__global__ void __launch_bounds__(kWeightMmaThreads) attn_weights_mma_kernel(const __grid_constant__ TreeAttnParams p) {
     constexpr int kPitch = D * 2 + 16, kKS = D / 16, kChunk = 64;
-    __shared__ __align__(16) uint8_t sm[kChunk * kPitch];
+    extern __shared__ __align__(16) uint8_t sm_k[];
+    uint8_t *sm_q = sm_k + kWeightKeys * kPitch;
     __shared__ float lse[kChunk];
     __shared__ uint64_t seen[kChunk];
-    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3, t0 = blockIdx.y * 64;
+    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3, t0 = blockIdx.y * kWeightKeys;
     pdl_wait();
     pdl_trigger();
     const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
     if (t0 >= n) return;
-    const uint16_t *k = static_cast<const uint16_t *>(p.k) + ((long)bh * p.T + t0) * D;
-    // pieces of 16 bytes of 64 rows: a thread has the same piece of every kStep-th row
-    constexpr int kStep = kThreadsAttn / (D / 8), kLoads = 64 / kStep;
+    // pieces of 16 bytes: a thread has the same piece of every kStep-th row
+    constexpr int kStep = kWeightMmaThreads / (D / 8), kKLoads = kWeightKeys / kStep, kQLoads = kChunk / kStep;
     const int c = tid % (D / 8), first = tid / (D / 8);
-    uint4 x[kLoads];
+    const uint16_t *k = static_cast<const uint16_t *>(p.k) + ((long)bh * p.T + t0) * D + c * 8;
+    uint4 x[kKLoads], q[kQLoads];
+    float at = 0.0f;
+    uint64_t bits = 0;
+    auto fetch = [&](int r0) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int r = first + i * kStep;
-        x[i] = t0 + r < n ? ldg_nc_v4(k + (long)r * D + c * 8) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) *reinterpret_cast<uint4 *>(sm + (first + i * kStep) * kPitch + c * 16) = x[i];
-    __syncthreads();
-    uint32_t kf[2][kKS][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int k2 = 0; k2 < kKS / 2; ++k2)
-            ldsm4(smem_u32(sm) + (warp * 16 + i * 8 + (lane & 7)) * kPitch + (k2 * 4 + (lane >> 3)) * 16, kf[i][2 * k2][0], kf[i][2 * k2][1], kf[i][2 * k2 + 1][0], kf[i][2 * k2 + 1][1]);
-    float sum[2][2] = {};
-    for (int r0 = 0; r0 < p.R; r0 += kChunk) {
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int row = min(r0 + first + i * kStep, p.R - 1);
-            x[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, row) + c * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) *reinterpret_cast<uint4 *>(sm + (first + i * kStep) * kPitch + c * 16) = x[i];
+        for (int i = 0; i < kQLoads; ++i)
+            q[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, min(r0 + first + i * kStep, p.R - 1)) + c * 8);
         if (tid < kChunk) {
             const int row = r0 + tid;
-            seen[tid] = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
+            bits = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
             // rows that do not exist or see nothing have no weight anywhere
-            lse[tid] = row >= p.R || (len == 0 && !seen[tid]) ? INFINITY : p.lse[(long)bh * p.R + row];
+            at = row >= p.R || (len == 0 && !bits) ? INFINITY : p.lse[(long)bh * p.R + row];
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kKLoads; ++i) x[i] = t0 + first + i * kStep < n ? ldg_nc_v4(k + (long)(first + i * kStep) * D) : make_uint4(0, 0, 0, 0);
+    fetch(0);
+    // the entries that this lane adds to, at the end
+    const int mine = t0 + warp * 16 + (grp & 1) * 8 + quad * 2;
+    float was[2] = {};
+    if (grp < 2) {
+        if (mine < n) was[0] = p.weights[(long)bh * p.T + mine];
+        if (mine + 1 < n) was[1] = p.weights[(long)bh * p.T + mine + 1];
+    }
+#pragma unroll
+    for (int i = 0; i < kKLoads; ++i) *reinterpret_cast<uint4 *>(sm_k + (first + i * kStep) * kPitch + c * 16) = x[i];
+    uint32_t kf[2][kKS][2];
+    float sum[2][2] = {};
+    for (int r0 = 0; r0 < p.R; r0 += kChunk) {
+        if (r0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kQLoads; ++i) *reinterpret_cast<uint4 *>(sm_q + (first + i * kStep) * kPitch + c * 16) = q[i];
+        if (tid < kChunk) { seen[tid] = bits; lse[tid] = at; }
         __syncthreads();
+        if (r0 == 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int k2 = 0; k2 < kKS / 2; ++k2)
+                    ldsm4(smem_u32(sm_k) + (warp * 16 + i * 8 + (lane & 7)) * kPitch + (k2 * 4 + (lane >> 3)) * 16, kf[i][2 * k2][0], kf[i][2 * k2][1], kf[i][2 * k2 + 1][0], kf[i][2 * k2 + 1][1]);
+        }
+        if (r0 + kChunk < p.R) fetch(r0 + kChunk);
         for (int t = 0; t < kChunk / 16 && r0 + t * 16 < p.R; ++t) {
             float sc[2][4] = {};
 #pragma unroll
             for (int ks = 0; ks < kKS; ++ks) {
                 uint32_t a0, a1, a2, a3;
-                ldsm4(smem_u32(sm) + (t * 16 + (lane & 15)) * kPitch + (ks * 2 + (lane >> 4)) * 16, a0, a1, a2, a3);
+                ldsm4(smem_u32(sm_q) + (t * 16 + (lane & 15)) * kPitch + (ks * 2 + (lane >> 4)) * 16, a0, a1, a2, a3);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) mma16816<BF16>(sc[i], a0, a1, a2, a3, kf[i][ks][0], kf[i][ks][1]);
             }
+            if (t0 + kWeightKeys <= len) {
+                // committed entries; a row without weight has an infinite logarithm, and q of the last row
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = t * 16 + grp + (e >> 1) * 8, j = t0 + warp * 16 + i * 8 + quad * 2 + (e & 1) - len;
-                    const bool none = r0 + r >= p.R || lse[r] == INFINITY || (j >= 0 && (j >= 64 || !((seen[r] >> j) & 1)));
-                    sum[i][e & 1] += none ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -lse[r]));
-                }
+                    for (int e = 0; e < 4; ++e) {
+                        const float l = lse[t * 16 + grp + (e >> 1) * 8];
+                        sum[i][e & 1] += l == INFINITY ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -l));
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = t * 16 + grp + (e >> 1) * 8, j = t0 + warp * 16 + i * 8 + quad * 2 + (e & 1) - len;
+                        const bool none = lse[r] == INFINITY || (j >= 0 && (j >= 64 || !((seen[r] >> j) & 1)));
+                        sum[i][e & 1] += none ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -lse[r]));
+                    }
+            }
         }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float x = sum[i][e];
-            x += __shfl_xor_sync(0xffffffffu, x, 4);
-            x += __shfl_xor_sync(0xffffffffu, x, 8);
-            x += __shfl_xor_sync(0xffffffffu, x, 16);
-            const int t = t0 + warp * 16 + i * 8 + quad * 2 + e;
-            if (grp == 0 && t < n) p.weights[(long)bh * p.T + t] += x;
+            sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 4);
+            sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 8);
+            sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 16);
         }
+    if (grp < 2) {
+        if (mine < n) p.weights[(long)bh * p.T + mine] = was[0] + (grp ? sum[1][0] : sum[0][0]);
+        if (mine + 1 < n) p.weights[(long)bh * p.T + mine + 1] = was[1] + (grp ? sum[1][1] : sum[0][1]);
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------
@@ -587,9 +627,14 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
         rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)each), "tree_attention join");
     }
     if (rc || !p.weights) return rc;
-    if (p.scores)
-        return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + kWeightThreads - 1) / kWeightThreads)), kWeightThreads, 0, stream, p), "tree_attention weights");
-    return cuda_status(launch_pdl(attn_weights_mma_kernel<D, BF16>, dim3(heads, (unsigned)((p.T + 63) / 64)), kThreadsAttn, 0, stream, p), "tree_attention weights");
+    if (p.scores) {
+        const int each = kWeightThreads * kWeightEach;
+        return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + each - 1) / each)), kWeightThreads, 0, stream, p), "tree_attention weights");
+    }
+    const cudaError_t e = cudaFuncSetAttribute(attn_weights_mma_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem<D>());
+    if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
+    return cuda_status(launch_pdl(attn_weights_mma_kernel<D, BF16>, dim3(heads, (unsigned)((p.T + kWeightKeys - 1) / kWeightKeys)), kWeightMmaThreads, weights_smem<D>(), stream, p),
+                       "tree_attention weights");
 }
 
 }  // namespace
