@@ -150,61 +150,101 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
-constexpr int kSelKeys = 45056;            // in shared memory, 176 KB
+constexpr int kSelKeys = 45056;            // of a block in shared memory, 176 KB
+constexpr int kMaxCluster = 8;
+constexpr int kSelAhead = 4;               // times 32 entries that a warp has under way
 
-// A block per row.  The smallest key that is kept is found digit by digit, eight bits at a time, by counting the keys that agree with
-// the digits found so far; then the row is walked in order, every warp over a stretch of its own, and what lies above that key is
-// kept, of the equal ones the first few.  The keys stay in shared memory (cap: how many fit; the rest is read again).  Every lane counts in
-// a histogram of its own: weights are much alike in their leading bits, and with 8 copies of the counters 256 rows of 8,192 took 31 us.
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
+__device__ __forceinline__ uint32_t cluster_rank_of() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size_of() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_sync_of() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of shared memory of another CTA of the cluster, at the place that `local` has in this one
+__device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t rank) {
+    uint32_t at, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// A block per row, or a cluster of blocks that have a stretch of it each.  The smallest key that is kept is found digit by digit, eight
+// bits at a time, by counting the keys that agree with the digits found so far; then the row is walked in order, every warp over a
+// part of its own, and what lies above that key is kept, of the equal ones the first few.  The keys stay in shared memory (cap: how
+// many fit; the rest is read again).  Every lane counts in a histogram of its own: weights are much alike in their leading bits.  (With 8
+// copies of the counters 256 rows of 8,192 took 31 us, finding the key two bits at a time by comparisons in registers 33, counting
+// equal digits of a warp once 28; this 25.)
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
+    constexpr int kWarps = THREADS / 32;
     extern __shared__ uint32_t keys[];
-    __shared__ uint32_t hist[256 * 32];    // [digit][lane]
-    __shared__ uint32_t digits[256];
+    __shared__ __align__(16) uint32_t hist[256 * 32];     // [digit][lane]
+    __shared__ uint32_t digits[2][256];    // of one digit and the next, in turn: the cluster may still read the last ones
+    __shared__ uint32_t total[256];
     __shared__ uint32_t found[2];          // prefix, how many of the keys that match it are to be kept
-    __shared__ uint32_t above[kSelWarps], equal[kSelWarps];
+    __shared__ uint32_t above[kWarps], equal[kWarps], sides[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int layer = blockIdx.y, b = blockIdx.x / p.nkv;
+    const int blocks = cluster_size_of(), rank = cluster_rank_of();
+    const int layer = blockIdx.y, head = blockIdx.x / blocks, b = head / p.nkv;
     pdl_wait();
     pdl_trigger();
-    const long row = (long)layer * gridDim.x + blockIdx.x;
-    const float *w = p.w[layer] + (long)blockIdx.x * p.T;
+    const long row = (long)layer * (gridDim.x / blocks) + head;
+    const float *w = p.w[layer] + (long)head * p.T;
     float *left = p.left + row * p.T;
     int32_t *kept = p.kept + row * p.keep;
     const int n = (int)min(max((long)p.lengths[b], 0L), p.T), m = min(n, p.keep);
-    if (tid == 0 && layer == 0 && blockIdx.x % p.nkv == 0) p.now[b] = m;
-    for (int i = m + tid; i < p.keep; i += kSelThreads) kept[i] = -1;
-    for (long i = m + tid; i < p.T; i += kSelThreads) left[i] = 0.0f;
+    const int all = blocks * THREADS, me = rank * THREADS + tid;
+    if (me == 0 && layer == 0 && head % p.nkv == 0) p.now[b] = m;
+    for (int i = m + me; i < p.keep; i += all) kept[i] = -1;
+    for (long i = m + me; i < p.T; i += all) left[i] = 0.0f;
     if (n <= p.keep) {
-        for (int i = tid; i < n; i += kSelThreads) { kept[i] = i; left[i] = w[i]; }
-        return;
+        for (int i = me; i < n; i += all) { kept[i] = i; left[i] = w[i]; }
+        return;                            // the whole cluster
     }
     const int cand = n - p.recent;         // recent <= keep < n
     uint32_t need = p.keep - p.recent, prefix = 0;
-    auto key = [&](int i) { return i < cap ? keys[i] : order_key(w[i]); };
-    for (int i = tid; i < min(cand, cap); i += kSelThreads) keys[i] = order_key(w[i]);
+    // this block's stretch of the row (whole warps' spans), and its warps'
+    const int span = ((n + blocks * kWarps - 1) / (blocks * kWarps) + 31) / 32 * 32;
+    const int lo = min(rank * kWarps * span, n), hi = min(lo + kWarps * span, n), own = min(hi, cand) - lo;      // entries to choose from: may be none
+    auto key = [&](int i) { return i < cap ? keys[i] : order_key(w[lo + i]); };
+#pragma unroll 8
+    for (int i = tid; i < min(own, cap); i += THREADS) keys[i] = order_key(w[lo + i]);
     if (need) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256 * 32; i += kSelThreads) hist[i] = 0;
+        for (int shift = 24, turn = 0; shift >= 0; shift -= 8, turn ^= 1) {
+#pragma unroll
+            for (int i = 0; i < 256 * 8 / THREADS; ++i) reinterpret_cast<uint4 *>(hist)[tid + i * THREADS] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-            for (int i = tid; i < cand; i += kSelThreads) {
+#pragma unroll 4
+            for (int i = tid; i < own; i += THREADS) {
                 const uint32_t u = key(i);
                 if ((u & mask) == prefix) atomicAdd(&hist[((u >> shift) & 255u) * 32 + lane], 1u);
             }
             __syncthreads();
+            // four lanes have eight of a digit's counts each
 #pragma unroll
-            for (int i = 0; i < 256 / kSelWarps; ++i) {
-                uint32_t c = hist[(warp * (256 / kSelWarps) + i) * 32 + lane];
-                c = __reduce_add_sync(0xffffffffu, c);
-                if (lane == 0) digits[warp * (256 / kSelWarps) + i] = c;
+            for (int i = 0; i < 256 / kWarps; i += 8) {
+                const int d = warp * (256 / kWarps) + i + (lane >> 2);
+                const uint4 u = *reinterpret_cast<const uint4 *>(&hist[d * 32 + (lane & 3) * 4]), v = *reinterpret_cast<const uint4 *>(&hist[d * 32 + 16 + (lane & 3) * 4]);
+                uint32_t c = u.x + u.y + u.z + u.w + v.x + v.y + v.z + v.w;
+                c += __shfl_xor_sync(0xffffffffu, c, 1);
+                c += __shfl_xor_sync(0xffffffffu, c, 2);
+                if ((lane & 3) == 0) digits[turn][d] = c;
+            }
+            if (blocks > 1) {
+                cluster_sync_of();
+                for (int i = tid; i < 256; i += THREADS) {
+                    uint32_t c = 0;
+                    for (int r = 0; r < blocks; ++r) c += peer_u32(&digits[turn][i], r);
+                    total[i] = c;
+                }
             }
             __syncthreads();
             if (warp == 0) {
                 // lane l: digits 255 - 8 l .. 248 - 8 l, from the largest down
                 uint32_t c[8], sum = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) { c[e] = digits[255 - 8 * lane - e]; sum += c[e]; }
+                for (int e = 0; e < 8; ++e) { c[e] = blocks > 1 ? total[255 - 8 * lane - e] : digits[turn][255 - 8 * lane - e]; sum += c[e]; }
                 uint32_t before = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -227,62 +267,76 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const __grid_
         __syncthreads();
     }
     // a warp walks entries [from, to) of the row, 32 at a time; the recent ones are above everything
-    const int span = (n + kSelWarps * 32 - 1) / (kSelWarps * 32) * 32, from = min(warp * span, n), to = min(from + span, n);
-    auto side = [&](int i) { return i >= to ? 0 : i >= cand ? 2 : key(i) > prefix ? 2 : key(i) == prefix ? 1 : 0; };
+    const int from = min(lo + warp * span, hi), to = min(from + span, hi);
+    auto side = [&](int i) { return i >= to ? 0 : i >= cand ? 2 : key(i - lo) > prefix ? 2 : key(i - lo) == prefix ? 1 : 0; };
     uint32_t na = 0, ne = 0;
-    for (int i = from; i < to; i += 32) {
-        const int s = side(i + lane);
-        na += __popc(__ballot_sync(0xffffffffu, s == 2));
-        ne += __popc(__ballot_sync(0xffffffffu, s == 1));
+    for (int i = from; i < to; i += 32 * kSelAhead) {
+#pragma unroll
+        for (int k = 0; k < kSelAhead; ++k) {
+            const int s = side(i + k * 32 + lane);
+            na += __popc(__ballot_sync(0xffffffffu, s == 2));
+            ne += __popc(__ballot_sync(0xffffffffu, s == 1));
+        }
     }
     if (lane == 0) { above[warp] = na; equal[warp] = ne; }
     __syncthreads();
     uint32_t a0 = 0, e0 = 0;               // what lies before this warp's stretch
     for (int i = 0; i < warp; ++i) { a0 += above[i]; e0 += equal[i]; }
-    for (int i = from; i < to; i += 32) {
-        const int s = side(i + lane);
-        const uint32_t ba = __ballot_sync(0xffffffffu, s == 2), be = __ballot_sync(0xffffffffu, s == 1), low = (1u << lane) - 1;
-        const uint32_t ea = e0 + __popc(be & low);
-        if (s == 2 || (s == 1 && ea < need)) {
-            const uint32_t at = a0 + __popc(ba & low) + min(ea, need);
-            kept[at] = i + lane;
-            left[at] = w[i + lane];
-        }
-        a0 += __popc(ba);
-        e0 += __popc(be);
+    if (blocks > 1) {
+        if (warp == kWarps - 1 && lane == 0) { sides[0] = a0 + na; sides[1] = e0 + ne; }
+        cluster_sync_of();
+        for (int r = 0; r < rank; ++r) { a0 += peer_u32(&sides[0], r); e0 += peer_u32(&sides[1], r); }
     }
+    for (int i = from; i < to; i += 32 * kSelAhead) {
+        float x[kSelAhead];                // fetched together
+#pragma unroll
+        for (int k = 0; k < kSelAhead; ++k) x[k] = i + k * 32 + lane < to ? w[i + k * 32 + lane] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < kSelAhead; ++k) {
+            const int s = side(i + k * 32 + lane);
+            const uint32_t ba = __ballot_sync(0xffffffffu, s == 2), be = __ballot_sync(0xffffffffu, s == 1), low = (1u << lane) - 1;
+            const uint32_t ea = e0 + __popc(be & low);
+            if (s == 2 || (s == 1 && ea < need)) {
+                const uint32_t at = a0 + __popc(ba & low) + min(ea, need);
+                kept[at] = i + k * 32 + lane;
+                left[at] = x[k];
+            }
+            a0 += __popc(ba);
+            e0 += __popc(be);
+        }
+    }
+    if (blocks > 1) cluster_sync_of();     // the others have read this block's counts
 }
 
 // Rows kept[0 .. m) of K and V to rows 0 .. m - 1, in place.  kept rises, so kept[d] >= d: rows that a batch writes are read by
 // that batch and by earlier ones only.  A block owns a column of a row's 16-byte pieces; while it has one batch of rows to write it
-// reads the next one and the indices of the one after that, and it writes when all its threads have read theirs.  8 pieces a thread:
-// with 4 the move of 512 MB took 131 us, with 8 it is 100 (256 threads; 512 threads and 8 pieces as fast, 1,024 and 2 slower).
-constexpr int kMoveThreads = 256, kMovePieces = 8;
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p, int slab) {
+// reads the next one and the indices of the one after that, and it writes when all its threads have read theirs.
+template <int THREADS, int PIECES>
+__global__ void __launch_bounds__(THREADS) evict_move_kernel(const __grid_constant__ EvictParams p, int slab) {
     const int layer = blockIdx.y, unit = blockIdx.x, slabs = p.chunks / slab;
     const int bh = unit / (2 * slabs), sub = unit - bh * 2 * slabs, isv = sub / slabs, c0 = (sub - isv * slabs) * slab;
     pdl_wait();
     pdl_trigger();
-    const int rows = kMoveThreads / slab, r = threadIdx.x / slab, c = c0 + threadIdx.x - r * slab;
+    const int rows = THREADS / slab, r = threadIdx.x / slab, c = c0 + threadIdx.x - r * slab;
     const int heads = gridDim.x / (2 * slabs), b = bh / p.nkv;
     const int n = (int)min(max((long)p.lengths[b], 0L), p.T);
     if (n <= p.keep) return;               // the whole block
     const int end = r < rows ? p.keep : 0; // threads that a slab of odd width leaves over have nothing to move
     const int32_t *kept = p.kept + ((long)layer * heads + bh) * p.keep;
     uint4 *base = static_cast<uint4 *>(isv ? p.v[layer] : p.k[layer]) + (long)bh * p.T * p.chunks + c;
-    const int batch = rows * kMovePieces;
-    uint4 x[kMovePieces], y[kMovePieces];
-    int fx[kMovePieces], fy[kMovePieces], fz[kMovePieces];
-    auto indices = [&](int d0, int (&f)[kMovePieces]) {
+    const int batch = rows * PIECES;
+    uint4 x[PIECES], y[PIECES];
+    int fx[PIECES], fy[PIECES], fz[PIECES];
+    auto indices = [&](int d0, int (&f)[PIECES]) {
 #pragma unroll
-        for (int j = 0; j < kMovePieces; ++j) {
+        for (int j = 0; j < PIECES; ++j) {
             const int d = d0 + r + j * rows;
             f[j] = d < end ? kept[d] : d;
         }
     };
-    auto load = [&](int d0, const int (&f)[kMovePieces], uint4 (&v)[kMovePieces]) {
+    auto load = [&](int d0, const int (&f)[PIECES], uint4 (&v)[PIECES]) {
 #pragma unroll
-        for (int j = 0; j < kMovePieces; ++j)
+        for (int j = 0; j < PIECES; ++j)
             if (f[j] != d0 + r + j * rows) v[j] = base[(long)f[j] * p.chunks];
     };
     indices(0, fx);
@@ -293,7 +347,7 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
         load(d0 + batch, fy, y);
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < kMovePieces; ++j) {
+        for (int j = 0; j < PIECES; ++j) {
             const int d = d0 + r + j * rows;
             if (fx[j] != d) base[(long)d * p.chunks] = x[j];
             x[j] = y[j];
@@ -334,14 +388,37 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     for (int i = 0; i < layers; ++i) { p.k[i] = k[i]; p.v[i] = v[i]; p.w[i] = w[i]; }
     p.lengths = lengths; p.kept = kept; p.now = now; p.left = left;
     p.B = B; p.nkv = nkv; p.keep = keep; p.recent = recent; p.chunks = D / 8; p.T = T;
-    const int cap = (int)(T < kSelKeys ? T : kSelKeys);
-    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+    // One block per row; a cluster of up to 8 where the rows do not fill the GPU and are long (16 rows of 24,000: 29 -> 18 us).  Short rows
+    // take blocks of 256 threads, of which more fit an SM.
+    const long rows = (long)B * nkv * layers;
+    int blocks = 1;
+    while (blocks < kMaxCluster && rows * blocks * 2 <= kNumSMs && T >= 4096L * blocks) blocks *= 2;
+    const bool few = T <= 2048;
+    const long each = (T + blocks - 1) / blocks + 2048;                  // a block's stretch, rounded up to whole spans
+    const int cap = (int)(each < kSelKeys ? each : kSelKeys);
+    auto select = few ? evict_select_kernel<256> : evict_select_kernel<512>;
+    const cudaError_t e = cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
     if (e != cudaSuccess) return cuda_status(e, "cache_evict shared memory");
-    int rc = cuda_status(launch_pdl(evict_select_kernel, dim3((unsigned)(B * nkv), (unsigned)layers), kSelThreads, (size_t)cap * 4, stream, p, cap), "cache_evict select");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(B * nkv * blocks), (unsigned)layers); cfg.blockDim = dim3(few ? 256 : 512);
+    cfg.dynamicSmemBytes = (size_t)cap * 4; cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = blocks > 1 ? 2 : 1;
+    int rc = cuda_status(cudaLaunchKernelEx(&cfg, select, p, cap), "cache_evict select");
     if (rc) return rc;
-    // a block per half of a row's pieces (64 bytes or more), so that one layer of one sequence already spreads over the GPU
-    const int slab = p.chunks % 2 == 0 && p.chunks >= 8 ? p.chunks / 2 : p.chunks;
-    return cuda_status(launch_pdl(evict_move_kernel, dim3((unsigned)(B * nkv * 2 * (p.chunks / slab)), (unsigned)layers), kMoveThreads, 0, stream, p, slab), "cache_evict move");
+    // A block per half of a row's pieces (128 bytes of a head of 128), so that one layer of one sequence already spreads over the GPU:
+    // 256 threads with 8 pieces each (512 MB: 95 us; with 4 pieces 126).  Where that is a block for half of the SMs or less and each has
+    // much to move, quarters and 512 threads (16 heads, 24,000 -> 15,600 entries: 105 -> 71 us in all); where it is little, 128 threads with 4
+    // pieces, of which more fit an SM (1,536 heads, 700 -> 197 entries: 130 -> 99 us).
+    const bool much = rows * 4 <= kNumSMs / 2 && keep > 2048 && p.chunks % 4 == 0 && p.chunks >= 8, little = keep <= 512;
+    const int slabs = much ? 4 : p.chunks % 2 == 0 && p.chunks >= 8 ? 2 : 1, slab = p.chunks / slabs;
+    const dim3 grid((unsigned)(B * nkv * 2 * slabs), (unsigned)layers);
+    if (much) return cuda_status(launch_pdl(evict_move_kernel<512, 8>, grid, 512, 0, stream, p, slab), "cache_evict move");
+    if (little) return cuda_status(launch_pdl(evict_move_kernel<128, 4>, grid, 128, 0, stream, p, slab), "cache_evict move");
+    return cuda_status(launch_pdl(evict_move_kernel<256, 8>, grid, 256, 0, stream, p, slab), "cache_evict move");
 }
 
 }  // namespace flh
