@@ -8,7 +8,7 @@
 //           a batch of uneven lengths is as balanced as one long sequence.  For more jobs than CTAs, or many sequences.
 //   kParts  every job is cut into parts of nearly the same size, as many as its length is worth, a CTA for each: no CTA has
 //           parts of two jobs, whose second one costs it what several tiles do (q, the ramp of the rings, the result).
-//   kJobs   a CTA for each job; nothing is cut.
+//   kJobs   each CTA has as many whole jobs as the next; nothing is cut.
 // A job that lies within one CTA is finished there; of a job that was cut each CTA writes a partial result (sum of exponentials,
 // maximum, weighted sum of V) to a slot of its own and the join kernel adds them in order.
 #pragma once
@@ -33,7 +33,7 @@ struct TreeAttnParams {
     int T;
     float scale_log2;                      // scale * log2(e): scores live in powers of two
     int shares, min_share;                 // CTAs, tiles that a share has at least
-    int split;                             // kEven, kParts, kJobs
+    int split, jobs_each;                  // kEven, kParts, kJobs; jobs of a CTA (kJobs)
     float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
@@ -163,9 +163,12 @@ struct Parts {
 template <int TILE>
 __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, JobWalk<TILE> &job, int &u0, int &u1) {
     if (p.split == kJobs) {
-        job.at(p, blockIdx.x, lane);
+        const int all = p.B * p.nkv * p.nrb, first = blockIdx.x * p.jobs_each;
+        JobWalk<TILE> last;
+        last.at(p, min(first + p.jobs_each, all) - 1, lane);
+        job.at(p, first, lane);
         u0 = job.begin;
-        u1 = u0 + job.nt;
+        u1 = last.begin + last.nt;
     } else if (p.split == kParts) {
         Parts<TILE> c;
         c.find(p, lane);
@@ -209,7 +212,11 @@ template <bool BF16> __device__ __forceinline__ void store16(void *p, long i, fl
     if (BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
     else static_cast<__half *>(p)[i] = __float2half_rn(x);
 }
-template <bool BF16> __device__ __forceinline__ bool nonfinite16(uint16_t u) { return BF16 ? (u & 0x7f80u) == 0x7f80u : (u & 0x7c00u) == 0x7c00u; }
+// 16-bit values of a word that are not finite, as zero
+template <bool BF16> __device__ __forceinline__ uint32_t finite2(uint32_t w) {
+    const uint32_t e = BF16 ? 0x7f807f80u : 0x7c007c00u;
+    return w & ~__vcmpeq2(w & e, e);
+}
 
 // 1 / l of a row whose exponentials sum to l, as the factor of its weighted sum.  A row that sees nothing is zero; one whose scores
 // are all -inf is NaN, as a softmax has it.

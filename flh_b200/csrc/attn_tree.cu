@@ -106,10 +106,11 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
     int used = 0;                          // items taken from the ring
     bool alive = true;
 
-    // rows of q of a job: 16-byte piece q_c of every kQStep-th row, fetched while the job before is finished
+    // rows of q of a job and what they see of its drafted entries: 16-byte piece q_c of every kQStep-th row, fetched while the job before is finished
     constexpr int kQStep = kThreadsAttn / (D / 8), kQLoads = kRows / kQStep;
     const int q_c = tid % (D / 8), q_r = tid / (D / 8);
     uint4 qv[kQLoads];
+    uint64_t bits = 0;
     auto fetch_q = [&](const JobWalk<kTile> &j) {
         const int kvh = j.job / p.nrb, row0 = (j.job - kvh * p.nrb) * kRows;
 #pragma unroll
@@ -117,6 +118,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const int row = row0 + q_r + i * kQStep;
             qv[i] = row < p.R ? ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, j.b, kvh, row) + q_c * 8) : make_uint4(0, 0, 0, 0);
         }
+        if (tid < kRows) bits = row0 + tid < p.R ? drafted_bits(p, j.b, token_of(p, row0 + tid), j.len) : 0;
     };
     fetch_q(cur);
     for (int piece = u0; piece < u1;) {
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
         __syncthreads();                   // the piece before is written out
 #pragma unroll
         for (int i = 0; i < kQLoads; ++i) *reinterpret_cast<uint4 *>(sm_q + (q_r + i * kQStep) * q_pitch<D>() + q_c * 16) = qv[i];
-        if (tid < kRows) seen[tid] = row0 + tid < p.R ? drafted_bits(p, b, token_of(p, row0 + tid), len) : 0;
+        if (tid < kRows) seen[tid] = bits;
         if (tid == 0) bad = 0;
         __syncthreads();
         float o[kDT][4], m[2], l[2];
@@ -222,18 +224,17 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const uint32_t vs = ring_u + slot * kSlot;
             if (tail) {
                 // rows of V behind the sequence's end become zero, and so do values of drafted entries that are not finite
-                for (int i = lane; i < kTile * (D / 8); i += 32) {
-                    const int row = i / (D / 8), chunk = i - row * (D / 8), t = key0 + row;
-                    if (t < len) continue;
-                    uint8_t *at = ring + slot * kSlot + swizzled<kTile>(row, chunk);
-                    uint4 x = *reinterpret_cast<const uint4 *>(at);
-                    uint16_t *h = reinterpret_cast<uint16_t *>(&x);
-                    bool changed = false;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (t >= n || nonfinite16<BF16>(h[e])) { h[e] = 0; changed = true; }
-                    if (changed) *reinterpret_cast<uint4 *>(at) = x;
-                    if (changed && t < n) atomicOr(&bad, 1ull << (t - len));
+                const int row = max(len - key0, 0) + lane / (D / 8), chunk = lane % (D / 8);      // the rows behind the committed ones
+#pragma unroll 4
+                for (int r = row; r < kTile; r += 32 / (D / 8)) {
+                    const int t = key0 + r;
+                    uint4 *at = reinterpret_cast<uint4 *>(ring + slot * kSlot + swizzled<kTile>(r, chunk));
+                    const uint4 was = *at;
+                    const uint4 is = t >= n ? make_uint4(0, 0, 0, 0) : make_uint4(finite2<BF16>(was.x), finite2<BF16>(was.y), finite2<BF16>(was.z), finite2<BF16>(was.w));
+                    if (is.x != was.x || is.y != was.y || is.z != was.z || is.w != was.w) {
+                        *at = is;
+                        if (t < n) atomicOr(&bad, 1ull << (t - len));
+                    }
                 }
                 __syncwarp();
             }
@@ -562,7 +563,7 @@ __global__ void __launch_bounds__(kWeightMmaThreads) attn_weights_mma_kernel(con
 // ---- host side ------------------------------------------------------------------------------
 struct Plan {
     int rows, nrb, shares, min_share;
-    int split;
+    int split, jobs_each;
     bool scores;
     long score_ld;
     size_t part_o, part_ml, lse, sc, total;        // offsets in the workspace
@@ -574,11 +575,13 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     pl.nrb = (R + pl.rows - 1) / pl.rows;
     pl.shares = pl.rows >= 128 ? kNumSMs : 2 * kNumSMs;
     pl.min_share = pl.rows >= 128 ? 2 : kWarps;
-    // A CTA per job where the longest job (of a full cache) would not take much longer than an even share: what is saved is the join
-    // and the second piece of most CTAs.  In tiles of that share: 24 of 32 entries (one sequence of 500 entries, 32 heads: 13.7 -> 10.1 us),
+    // Whole jobs where what that makes the fullest CTA work more than an even share is little: what is saved is the join and, for most
+    // CTAs, a second piece.  In tiles: 24 of 32 entries (one sequence of 500 entries, 32 heads: 13.7 -> 10.1 us; 24 sequences of 40: X),
     // 12 of 64 entries on the tensor cores.  Else parts of the jobs, where that is worked out quickly.
-    const long jobs = (long)B * nkv * pl.nrb, tile = pl.rows >= 128 ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile;
-    pl.split = jobs > pl.shares ? kEven : nt - nt * jobs / pl.shares <= (pl.rows >= 128 ? 12 : 24) ? kJobs : B <= 32 ? kParts : kEven;
+    const long jobs = (long)B * nkv * pl.nrb, tile = pl.rows >= 128 ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile, each = (jobs + pl.shares - 1) / pl.shares;
+    pl.split = each * nt - jobs * nt / pl.shares <= (pl.rows >= 128 ? 12 : 24) ? kJobs : jobs <= pl.shares && B <= 32 ? kParts : kEven;
+    pl.jobs_each = (int)each;
+    if (pl.split == kJobs) pl.shares = (int)((jobs + each - 1) / each);
     pl.scores = weights && R <= 16;
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
@@ -608,7 +611,7 @@ int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap
     constexpr int smem = attn_smem<D>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.split == kJobs ? p.B * p.nkv * p.nrb : p.shares)), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 template <int D, bool BF16>
@@ -651,6 +654,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.shares = pl.shares;
     p.min_share = pl.min_share;
     p.split = pl.split;
+    p.jobs_each = pl.jobs_each;
     p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + pl.part_ml);
     p.lse = p.weights ? reinterpret_cast<float *>(ws + pl.lse) : nullptr;

@@ -63,12 +63,6 @@ __device__ __forceinline__ void tc_ld2(uint32_t taddr, uint32_t &a, uint32_t &b)
 }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 16-bit values of a word that are not finite, as zero
-template <bool BF16> __device__ __forceinline__ uint32_t finite2(uint32_t w) {
-    const uint32_t e = BF16 ? 0x7f807f80u : 0x7c007c00u;
-    return w & ~__vcmpeq2(w & e, e);
-}
-
 // TWO: the streams are two blocks of rows; otherwise they share one.
 template <int D, bool TWO, bool BF16>
 __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap,
@@ -463,7 +457,7 @@ int launch_tc(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap 
     constexpr int smem = smem_tc<D, TWO>();
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    return cuda_status(launch_pdl(kern, dim3((unsigned)(p.split == kJobs ? p.B * p.nkv * p.nrb : p.shares)), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
+    return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
 }
 
 }  // namespace
