@@ -16,6 +16,7 @@
 namespace flh {
 
 int launch_attn_tc(const TreeAttnParams &, int, bool, const CUtensorMap &, const CUtensorMap &, cudaStream_t);
+int launch_attn_weights_tc(const TreeAttnParams &, bool, const CUtensorMap &, cudaStream_t);
 int attn_tc_status(int *);
 int attn_tc_status_clear();
 
@@ -455,138 +456,6 @@ __global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __gr
     }
 }
 
-// The same for many rows, from K and q again: a block goes through some of a head's tiles of 128 entries, which come by asynchronous
-// copies while the one before is worked on; a warp has 16 entries of a tile in registers, and the rows pass through shared memory 64 at a
-// time (up to 64 rows stay there).
-constexpr int kWeightKeys = 128, kWeightMmaThreads = 256;
-template <int D> constexpr int weights_smem() { return (2 * kWeightKeys + 64) * (D * 2 + 16); }
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kWeightMmaThreads, 2) attn_weights_mma_kernel(const __grid_constant__ TreeAttnParams p) {
-    constexpr int kPitch = D * 2 + 16, kKS = D / 16, kChunk = 64;
-    extern __shared__ __align__(16) uint8_t sm_k[];                              // two tiles, then the rows
-    uint8_t *sm_q = sm_k + 2 * kWeightKeys * kPitch;
-    __shared__ float lse[kChunk];
-    __shared__ uint64_t seen[kChunk];
-    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = lane >> 2, quad = lane & 3;
-    pdl_wait();
-    pdl_trigger();
-    const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
-    const int tiles = (n + kWeightKeys - 1) / kWeightKeys, each = (tiles + gridDim.y - 1) / gridDim.y, first = blockIdx.y * each, last = min(first + each, tiles);
-    if (first >= last) return;
-    // pieces of 16 bytes: a thread has the same piece of every kStep-th row
-    constexpr int kStep = kWeightMmaThreads / (D / 8), kKLoads = kWeightKeys / kStep, kQLoads = kChunk / kStep;
-    const int c = tid % (D / 8), r_of = tid / (D / 8);
-    const uint16_t *k = static_cast<const uint16_t *>(p.k) + (long)bh * p.T * D + c * 8;
-    auto load = [&](int tile) {
-        const uint32_t dst = smem_u32(sm_k) + ((tile - first) & 1) * kWeightKeys * kPitch + c * 16;
-#pragma unroll
-        for (int i = 0; i < kKLoads; ++i) {
-            const int r = r_of + i * kStep, t = tile * kWeightKeys + r;
-            // entries behind the last one are not looked at: the last one's row stands in for them
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + r * kPitch), "l"(k + (long)min(t, n - 1) * D) : "memory");
-        }
-    };
-    uint4 q[kQLoads];
-    float at = 0.0f;
-    uint64_t bits = 0;
-    auto fetch = [&](int r0) {
-#pragma unroll
-        for (int i = 0; i < kQLoads; ++i)
-            q[i] = ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, min(r0 + r_of + i * kStep, p.R - 1)) + c * 8);
-        if (tid < kChunk) {
-            const int row = r0 + tid;
-            bits = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
-            // rows that do not exist or see nothing have no weight anywhere
-            at = row >= p.R || (len == 0 && !bits) ? INFINITY : p.lse[(long)bh * p.R + row];
-        }
-    };
-    auto place = [&]() {
-#pragma unroll
-        for (int i = 0; i < kQLoads; ++i) *reinterpret_cast<uint4 *>(sm_q + (r_of + i * kStep) * kPitch + c * 16) = q[i];
-        if (tid < kChunk) { seen[tid] = bits; lse[tid] = at; }
-    };
-    load(first);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    fetch(0);
-    place();
-    const bool many = p.R > kChunk;
-    for (int tile = first; tile < last; ++tile) {
-        const int t0 = tile * kWeightKeys;
-        // the entries that this lane adds to, at the end
-        const int mine = t0 + warp * 16 + (grp & 1) * 8 + quad * 2;
-        float was[2] = {};
-        if (grp < 2) {
-            if (mine < n) was[0] = p.weights[(long)bh * p.T + mine];
-            if (mine + 1 < n) was[1] = p.weights[(long)bh * p.T + mine + 1];
-        }
-        __syncthreads();                                                         // the buffer that is loaded next has been read
-        if (tile + 1 < last) load(tile + 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncthreads();
-        const uint32_t ks_at = smem_u32(sm_k) + ((tile - first) & 1) * kWeightKeys * kPitch;
-        uint32_t kf[2][kKS][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int k2 = 0; k2 < kKS / 2; ++k2)
-                ldsm4(ks_at + (warp * 16 + i * 8 + (lane & 7)) * kPitch + (k2 * 4 + (lane >> 3)) * 16, kf[i][2 * k2][0], kf[i][2 * k2][1], kf[i][2 * k2 + 1][0], kf[i][2 * k2 + 1][1]);
-        float sum[2][2] = {};
-        for (int r0 = 0; r0 < p.R; r0 += kChunk) {
-            if (many) {
-                if (r0 || tile > first) {                                        // (the first rows of the first tile are there)
-                    __syncthreads();
-                    place();
-                    __syncthreads();
-                }
-                if (r0 + kChunk < p.R || tile + 1 < last) fetch(r0 + kChunk < p.R ? r0 + kChunk : 0);
-            }
-            for (int t = 0; t < kChunk / 16 && r0 + t * 16 < p.R; ++t) {
-                float sc[2][4] = {};
-#pragma unroll
-                for (int ks = 0; ks < kKS; ++ks) {
-                    uint32_t a0, a1, a2, a3;
-                    ldsm4(smem_u32(sm_q) + (t * 16 + (lane & 15)) * kPitch + (ks * 2 + (lane >> 4)) * 16, a0, a1, a2, a3);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) mma16816<BF16>(sc[i], a0, a1, a2, a3, kf[i][ks][0], kf[i][ks][1]);
-                }
-                if (t0 + kWeightKeys <= len) {
-                    // committed entries; a row without weight has an infinite logarithm, and q of the last row
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float l = lse[t * 16 + grp + (e >> 1) * 8];
-                            sum[i][e & 1] += l == INFINITY ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -l));
-                        }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int r = t * 16 + grp + (e >> 1) * 8, j = t0 + warp * 16 + i * 8 + quad * 2 + (e & 1) - len;
-                            const bool none = lse[r] == INFINITY || (j >= 0 && (j >= 64 || !((seen[r] >> j) & 1)));
-                            sum[i][e & 1] += none ? 0.0f : exp2_approx(fmaf(sc[i][e], p.scale_log2, -lse[r]));
-                        }
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 4);
-                sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 8);
-                sum[i][e] += __shfl_xor_sync(0xffffffffu, sum[i][e], 16);
-            }
-        if (grp < 2) {
-            if (mine < n) p.weights[(long)bh * p.T + mine] = was[0] + (grp ? sum[1][0] : sum[0][0]);
-            if (mine + 1 < n) p.weights[(long)bh * p.T + mine + 1] = was[1] + (grp ? sum[1][1] : sum[0][1]);
-        }
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
 // ---- host side ------------------------------------------------------------------------------
 struct Plan {
     int rows, nrb, shares, min_share;
@@ -661,12 +530,7 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
         const int each = kWeightThreads * kWeightEach;
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + each - 1) / each)), kWeightThreads, 0, stream, p), "tree_attention weights");
     }
-    const cudaError_t e = cudaFuncSetAttribute(attn_weights_mma_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem<D>());
-    if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    // two blocks for every SM, but no more than there are tiles
-    const long tiles = (p.T + kWeightKeys - 1) / kWeightKeys, want = (2L * kNumSMs + heads - 1) / heads;
-    return cuda_status(launch_pdl(attn_weights_mma_kernel<D, BF16>, dim3(heads, (unsigned)(want < tiles ? want : tiles)), kWeightMmaThreads, weights_smem<D>(), stream, p),
-                       "tree_attention weights");
+    return launch_attn_weights_tc(p, BF16, km, stream);
 }
 
 }  // namespace

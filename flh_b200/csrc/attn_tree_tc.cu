@@ -451,6 +451,176 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
     }
 }
 
+// weights += sum over the rows of 2^(score - lse) for more rows than leave their scores (attn_tree.cu), from K and q again: S^T = K Q^T, an
+// entry per lane of tensor memory and a row per column, so that a thread adds up its entry's weights with nothing to exchange.  A
+// CTA (two an SM) has some of a head's tiles of 128 entries, 128 rows at a time; K is loaded, multiplied and added up in a pipeline of
+// two tiles.  What bounds it is one exponential for each score, 16 a clock and SM, or K; as mma.sync, where every warp reads all
+// rows for its 16 entries, 64 rows x 254,000 entries took 28 us (17 so, of which K's 65 MB are 10).
+constexpr int kWeightTile = 128, kThreadsWeights = 256, kWeightGroup = 8;
+template <int D> constexpr int smem_weights() { return 1024 + (2 * kWeightTile + kRowsTc) * D * 2; }
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap) {
+    constexpr int kTileBytes = kWeightTile * D * 2, kHalf = kWeightTile * 128, kBox = kTreeTcTile * 128;         // a box of the map is 64 entries high
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023), *sm_q = smem + 2 * kTileBytes;
+    __shared__ uint64_t full[2], empty[2], s_full[2], s_free[2];
+    __shared__ uint32_t seen[64][kRowsTc / 32];                                  // of drafted entry j: the rows that see it, a bit each
+    __shared__ __align__(16) float lse[kRowsTc];
+    __shared__ float so_far[kWeightGroup][kWeightTile];                          // an entry's sum over the rows before, its thread's own
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&s_free[i]), 4); }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(256) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait();
+    pdl_trigger();
+    const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
+    const int tiles = (n + kWeightTile - 1) / kWeightTile, each = (tiles + gridDim.y - 1) / gridDim.y, first = min((int)blockIdx.y * each, tiles), last = min(first + each, tiles);
+    bool ok = true;
+    auto wait = [&](uint64_t *bar, uint32_t phase, int code) {
+        if (ok) ok = mbar_wait_warp(g_status_attn_tc, smem_u32(bar), phase & 1, &abort_flag, code);
+    };
+    uint32_t it = 0;                                                             // tiles so far, of all rows
+    // with more rows than 128 a few tiles at a time, so that an entry's sum over all of them is added to its weight once
+    const int group = p.R > kRowsTc ? kWeightGroup : tiles;
+    for (int g0 = first; g0 < last; g0 += group)
+    for (int row0 = 0; row0 < p.R; row0 += kRowsTc) {
+        const int g1 = min(g0 + group, last);
+        __syncthreads();                                                         // the rows before have been multiplied and looked at
+        constexpr int kStep = kThreadsWeights / (D / 8), kLoads = kRowsTc / kStep;
+        const int c = tid % (D / 8), r_of = tid / (D / 8);
+        uint4 q[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            q[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, min(row0 + r_of + i * kStep, p.R - 1)) + c * 8);
+        if (tid < kRowsTc) {
+            const int row = row0 + tid;
+            const uint64_t bits = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
+            if (last * kWeightTile > len) {                                      // some of the drafted entries are this CTA's
+#pragma unroll 8
+                for (int j = 0; j < 64; ++j) {
+                    const uint32_t rows = __ballot_sync(0xffffffffu, (bits >> j) & 1);
+                    if (lane == 0) seen[j][warp] = rows;
+                }
+            }
+            // rows that do not exist or see nothing have no weight anywhere
+            lse[tid] = row >= p.R || (len == 0 && !bits) ? INFINITY : p.lse[(long)bh * p.R + row];
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = r_of + i * kStep;
+            *reinterpret_cast<uint4 *>(sm_q + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = q[i];
+        }
+        fence_proxy_async();
+        __syncthreads();
+        const int cols = (min(p.R - row0, kRowsTc) + 15) / 16 * 16;
+        if (warp == 0) {
+            for (int tile = g0; tile < g1; ++tile, ++it) {
+                const int slot = it & 1;
+                wait(&empty[slot], (it >> 1) ^ 1, 61);
+                if (ok && elect_one()) {
+                    const uint32_t bar = smem_u32(&full[slot]), dst = smem_u32(smem + slot * kTileBytes);
+                    mbar_expect_tx(bar, kTileBytes);
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                                     ::"r"(dst + (i >> 1) * kHalf + (i & 1) * kBox), "l"(&kmap), "r"((i >> 1) * 64), "r"(tile * kWeightTile + (i & 1) * kTreeTcTile), "r"(bh), "r"(bar) : "memory");
+                }
+                __syncwarp();
+            }
+        } else if (warp == 1) {
+            const uint32_t fmt = BF16 ? 1u : 0u, idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(kWeightTile >> 4) << 24);
+            for (int tile = g0; tile < g1; ++tile, ++it) {
+                const int slot = it & 1;
+                wait(&full[slot], it >> 1, 62);
+                wait(&s_free[slot], (it >> 1) ^ 1, 63);
+                tc_fence_after();
+                const uint64_t a = make_smem_desc(smem_u32(smem + slot * kTileBytes)), bq = make_smem_desc(smem_u32(sm_q));
+                if (ok && elect_one()) {
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s) {
+                        const uint64_t off = ((s >> 2) * kHalf + (s & 3) * 32) >> 4;
+                        mma_f16<false>(tmem + slot * kRowsTc, a + off, bq + off, idesc, s > 0);
+                    }
+                    tc_commit(smem_u32(&s_full[slot]));
+                    tc_commit(smem_u32(&empty[slot]));
+                }
+                __syncwarp();
+            }
+        } else if (warp >= 4) {
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            float *w = p.weights + (long)bh * p.T;
+            for (int tile = g0; tile < g1; ++tile, ++it) {
+                const int slot = it & 1, t = tile * kWeightTile + (warp & 3) * 32 + lane, j = t - len;
+                const bool done = row0 + kRowsTc >= p.R;
+                const float was = done && t < n ? w[t] : 0.0f;
+                wait(&s_full[slot], it >> 1, 64);
+                tc_fence_after();
+                float sum[4] = {};
+                if (ok) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < cols; c0 += 32) {
+                        uint32_t s[32];
+                        tc_ld32(tmem + slot * kRowsTc + lanes + c0, s);          // (columns behind the rows' are not looked at)
+                        tc_wait_ld();
+                        const uint32_t hidden = j < 0 ? 0u : j >= 64 ? ~0u : ~seen[j][c0 >> 5];
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 l4 = *reinterpret_cast<const float4 *>(&lse[c0 + e]);
+                            const float l[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float x = exp2_approx(fmaf(__uint_as_float(s[e + i]), p.scale_log2, -l[i]));
+                                sum[i] += l[i] == INFINITY || (hidden & (1u << (e + i))) ? 0.0f : x;
+                            }
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_free[slot]));
+                float &before = so_far[row0 || !done ? tile - g0 : 0][(warp & 3) * 32 + lane];
+                const float now = (row0 ? before : 0.0f) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                if (!done) before = now;
+                else if (t < n && ok) w[t] = was + now;
+            }
+        }
+    }
+    __syncwarp();
+    if (warp == 0)                                                               // as in attn_tc_kernel: nothing is on its way when the CTA leaves
+        for (uint32_t i = it > 2 ? it - 2 : 0; i < it && abort_flag; ++i)
+            for (int tries = 0; tries < 10000 && !__all_sync(0xffffffffu, mbar_try_hint(smem_u32(&full[i & 1]), (i >> 1) & 1, 20000u)); ++tries);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+    }
+}
+
+template <int D, bool BF16>
+int launch_weights(const TreeAttnParams &p, const CUtensorMap &km, cudaStream_t stream) {
+    auto kern = attn_weights_tc_kernel<D, BF16>;
+    constexpr int smem = smem_weights<D>();
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
+    // two CTAs for every SM, but none without a tile
+    const long heads = (long)p.B * p.nkv, tiles = (p.T + kWeightTile - 1) / kWeightTile, want = heads >= 2L * kNumSMs ? 1 : 2L * kNumSMs / heads;
+    return cuda_status(launch_pdl(kern, dim3((unsigned)heads, (unsigned)(want < tiles ? want : tiles)), kThreadsWeights, smem, stream, p, km), "tree_attention weights");
+}
+
 template <int D, bool TWO, bool BF16>
 int launch_tc(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     auto kern = attn_tc_kernel<D, TWO, BF16>;
@@ -470,6 +640,11 @@ int launch_attn_tc(const TreeAttnParams &p, int rows, bool bf16, const CUtensorM
     }
     if (rows == 128) return bf16 ? launch_tc<64, false, true>(p, km, vm, stream) : launch_tc<64, false, false>(p, km, vm, stream);
     return bf16 ? launch_tc<64, true, true>(p, km, vm, stream) : launch_tc<64, true, false>(p, km, vm, stream);
+}
+
+int launch_attn_weights_tc(const TreeAttnParams &p, bool bf16, const CUtensorMap &km, cudaStream_t stream) {
+    if (p.D == 128) return bf16 ? launch_weights<128, true>(p, km, stream) : launch_weights<128, false>(p, km, stream);
+    return bf16 ? launch_weights<64, true>(p, km, stream) : launch_weights<64, false>(p, km, stream);
 }
 
 int attn_tc_status(int *out) { return cuda_status(cudaMemcpyFromSymbol(out, g_status_attn_tc, sizeof(int) * 4), "attn_tc_status"); }
