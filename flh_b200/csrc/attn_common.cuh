@@ -36,6 +36,7 @@ struct TreeAttnParams {
     int split, jobs_each;                  // kEven, kParts, kJobs; jobs of a CTA (kJobs)
     float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
+    int2 *parts_of;                        // [jobs] (kParts): first CTA and number of parts, for the join
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
     float *scores;                         // [B, nkv, R, score_ld] (with weights and few rows), or null
     long score_ld;
@@ -146,8 +147,15 @@ struct Parts {
         // the smallest size for which there are CTAs enough, of 32 between an even share and the longest job (which always is)
         const int even = max((total * per + p.shares - 1) / p.shares, p.min_share);
         const int tried = lane == 31 ? max(longest, 1) : even + even * lane / 16;
+        // ceil(nt / tried) as a truncated product: a little less than the quotient, by more than its rounding (2^-22) and less than the
+        // distance to the next whole number (1 / tried, nt < 2^17), and one more
+        const float inverse = (1.0f - 0x1p-19f) / (float)tried;
         int count = 0;
-        for (int i = 0; i < p.B; ++i) count += (__shfl_sync(0xffffffffu, nt, i) + tried - 1) / tried;
+#pragma unroll 8
+        for (int i = 0; i < p.B; ++i) {
+            const int other = __shfl_sync(0xffffffffu, nt, i);
+            count += (int)((float)other * inverse) + (other > 0);
+        }
         const unsigned fits = __ballot_sync(0xffffffffu, (long)count * per <= p.shares);
         size = __shfl_sync(0xffffffffu, tried, __ffs(fits) - 1);
         parts = (nt + size - 1) / size;
@@ -185,6 +193,7 @@ __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, Jo
         job.begin = 0;                     // its own count of tiles
         u0 = (cta - first - job.job * parts) * size;
         u1 = min(u0 + size, job.nt);
+        if (u0 == 0 && threadIdx.x == 0) p.parts_of[b * per + job.job] = make_int2(cta, parts);
     } else {
         const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
         const long first = (long)blockIdx.x * share;

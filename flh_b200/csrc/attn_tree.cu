@@ -325,48 +325,112 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
     }
 }
 
-// Jobs that several shares hold: their partial results in order.  A block for each job, or for each cut between two shares where that is
-// fewer (it takes the job that is cut there, if that is the job's first cut), for 8 of its rows and 4 GROUPS columns; a thread for four
-// columns of a row, the 8 rows next to one another in a warp so that it reads whole lines, and WAYS sets of threads that share
-// out the parts.  The parts' factors come first, each from one thread.  Few jobs in many parts take 32 columns a block and 16 ways (one
-// sequence of 60,000 entries, 8 rows: 59 -> 19 us with its attention), others all columns and 256 threads (16 jobs of 256 rows: 94 -> 84 us).
+// Jobs that several CTAs hold: their partial results in order.  A block for each job, or (kEven) for each cut between two shares where that
+// is fewer: it takes the job that is cut there, if that is the job's first cut.  A thread has four columns of a row, the 8 rows next
+// to one another in a warp so that it reads whole lines.
+//
+// CTAs c0 .. c0 + parts - 1 have the job; the first of them may have begun with another one (behind).
+template <int TILE>
+__device__ __forceinline__ bool find_parts(const TreeAttnParams &p, int lane, int by_job, int &b, int &job_of, int &c0, int &parts, bool &behind) {
+    behind = false;
+    if (p.split == kParts) {
+        const int per = p.nkv * p.nrb;
+        const int2 t = p.parts_of[blockIdx.x];
+        b = blockIdx.x / per;
+        job_of = blockIdx.x - b * per;
+        c0 = t.x;
+        parts = t.y;
+        return parts > 1;
+    }
+    const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
+    JobWalk<TILE> job;
+    if (by_job) {
+        job.at(p, blockIdx.x, lane);
+    } else {
+        const long cut = (blockIdx.x + 1L) * share;
+        if (cut >= total) return false;
+        job.seek(p, (int)cut, lane);
+        if (job.begin == cut || job.begin / share != (int)blockIdx.x) return false;
+    }
+    b = job.b;
+    job_of = job.job;
+    c0 = job.begin / share;
+    parts = (job.begin + job.nt - 1) / share - c0 + 1;
+    behind = (long)c0 * share != job.begin;
+    return parts > 1;
+}
+template <int D, bool BF16>
+__device__ __forceinline__ void store_joined(const TreeAttnParams &p, int b, int kvh, int row, int group, float base, float sum, float4 acc) {
+    const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
+    float factor = 1.0f / sum;
+    if (sum == 0.0f) {
+        const int len = committed(p, b);
+        factor = row_factor(sum, len == 0 && !drafted_bits(p, b, s, len));
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + s) * p.nh + h) * D + group * 4) =
+        make_uint2(narrow<BF16>(acc.x * factor, acc.y * factor), narrow<BF16>(acc.z * factor, acc.w * factor));
+    if (group == 0 && p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum);
+}
+
+// A block has 1,024 / D rows and all columns.  Eight parts and their maxima and sums are fetched together, so that up to eight cost one
+// wait for memory; where there are more the sum goes on relative to the larger maximum.
+template <int D, int TILE, bool BF16>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+    constexpr int kRowsOf = 1024 / D, kAhead = 8;
+    const int tid = threadIdx.x, r = blockIdx.y * kRowsOf + tid % kRowsOf, group = tid / kRowsOf;
+    pdl_wait();
+    pdl_trigger();
+    int b, job, c0, parts;
+    bool behind;
+    if (!find_parts<TILE>(p, tid & 31, by_job, b, job, c0, parts, behind)) return;
+    const int kvh = job / p.nrb, row = (job - kvh * p.nrb) * p.rows + r;
+    if (r >= p.rows || row >= p.R) return;
+    float top = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0, 0, 0, 0);
+    for (int i0 = 0; i0 < parts; i0 += kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int i = min(i0 + k, parts - 1);
+            const long slot = 2L * (c0 + i) + (i == 0 && behind);
+            ml[k] = p.part_ml[slot * p.rows + r];
+            v[k] = *reinterpret_cast<const float4 *>(p.part_o + slot * p.rows * D + ((long)group * p.rows + r) * 4);
+        }
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) now = fmaxf(now, ml[k].x);
+        const float base = now == -INFINITY ? 0.0f : now, keep = exp2_approx(top - base);
+        sum *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (i0 + k >= parts) continue;
+            const float f = exp2_approx(ml[k].x - base);
+            sum += ml[k].y * f;
+            acc.x += v[k].x * f; acc.y += v[k].y * f; acc.z += v[k].z * f; acc.w += v[k].w * f;
+        }
+        top = now;
+    }
+    store_joined<D, BF16>(p, b, kvh, row, group, top == -INFINITY ? 0.0f : top, sum, acc);
+}
+
+// Few jobs in many parts: a block for 8 rows and 32 columns, with 16 sets of threads that share out the parts; the parts' factors come
+// first, each from one thread (one sequence of 60,000 entries, 8 rows, in 268 parts: 59 -> 19 us with its attention).
 constexpr int kJoinRows = 8, kMaxParts = 2 * kNumSMs;
-template <int D, int TILE, bool BF16, int GROUPS, int WAYS>
-__global__ void __launch_bounds__(8 * GROUPS * WAYS) attn_join_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+template <int D, int TILE, bool BF16>
+__global__ void __launch_bounds__(1024) attn_join_wide_kernel(const __grid_constant__ TreeAttnParams p, int by_job) {
+    constexpr int GROUPS = 8, WAYS = 16;
     __shared__ float factor_of[kMaxParts][kJoinRows], reduced[GROUPS * WAYS / 4][kJoinRows];
     __shared__ float4 sm_acc[WAYS][8 * GROUPS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, way = tid / (8 * GROUPS);
     const int r_in = tid & 7, r = blockIdx.y * kJoinRows + r_in, group = blockIdx.z * GROUPS + (tid >> 3) % GROUPS;
     pdl_wait();
     pdl_trigger();
-    JobWalk<TILE> job;
-    int c0, parts;                         // CTAs c0 .. c0 + parts - 1 have the job
-    bool behind = false;                   // the first of them has begun with another job: the only one that can have
-    if (p.split == kParts) {
-        Parts<TILE> c;
-        c.find(p, lane);
-        const int per = p.nkv * p.nrb;
-        job.b = blockIdx.x / per;
-        job.job = blockIdx.x - job.b * per;
-        job.len = committed(p, job.b);
-        parts = __shfl_sync(0xffffffffu, c.parts, job.b);
-        c0 = __shfl_sync(0xffffffffu, c.first, job.b) + job.job * parts;
-    } else {
-        const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
-        if (by_job) {
-            job.at(p, blockIdx.x, lane);
-        } else {
-            const long cut = (blockIdx.x + 1L) * share;
-            if (cut >= total) return;
-            job.seek(p, (int)cut, lane);
-            if (job.begin == cut || job.begin / share != (int)blockIdx.x) return;
-        }
-        c0 = job.begin / share;
-        parts = (job.begin + job.nt - 1) / share - c0 + 1;
-        behind = (long)c0 * share != job.begin;
-    }
-    if (parts == 1) return;
-    const int kvh = job.job / p.nrb, row0 = (job.job - kvh * p.nrb) * p.rows, row = row0 + r, b = job.b;
+    int b, job, c0, parts;
+    bool behind;
+    if (!find_parts<TILE>(p, lane, by_job, b, job, c0, parts, behind)) return;
+    const int kvh = job / p.nrb, row = (job - kvh * p.nrb) * p.rows + r;
     const bool live = r < p.rows && row < p.R;
     auto slot = [&](int i) { return 2L * (c0 + i) + (i == 0 && behind); };
     // a row's values in lanes 8 apart, then over the warps
@@ -409,18 +473,12 @@ __global__ void __launch_bounds__(8 * GROUPS * WAYS) attn_join_kernel(const __gr
             acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
     }
-    if (WAYS > 1) {
-        sm_acc[way][tid % (8 * GROUPS)] = acc;
-        __syncthreads();
-    }
+    sm_acc[way][tid % (8 * GROUPS)] = acc;
+    __syncthreads();
     if (way || !live) return;
 #pragma unroll
     for (int w = 1; w < WAYS; ++w) { const float4 v = sm_acc[w][tid]; acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w; }
-    const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
-    const float factor = row_factor(sum, sum == 0.0f && job.len == 0 && !drafted_bits(p, b, s, job.len));
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + s) * p.nh + h) * D + group * 4) =
-        make_uint2(narrow<BF16>(acc.x * factor, acc.y * factor), narrow<BF16>(acc.z * factor, acc.w * factor));
-    if (group == 0 && p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum);
+    store_joined<D, BF16>(p, b, kvh, row, group, base, sum, acc);
 }
 
 // weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
@@ -462,7 +520,7 @@ struct Plan {
     int split, jobs_each;
     bool scores;
     long score_ld;
-    size_t part_o, part_ml, lse, sc, total;        // offsets in the workspace
+    size_t part_o, part_ml, parts_of, lse, sc, total;        // offsets in the workspace
 };
 Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     Plan pl = {};
@@ -484,6 +542,7 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     pl.part_o = take((size_t)2 * pl.shares * pl.rows * D * 4);
     pl.part_ml = take((size_t)2 * pl.shares * pl.rows * 8);
+    pl.parts_of = take((size_t)pl.shares * 8);
     pl.lse = take(weights ? (size_t)B * nkv * R * 4 : 0);
     pl.sc = take(pl.scores ? (size_t)B * nkv * R * pl.score_ld * 4 : 0);
     pl.total = at;
@@ -519,10 +578,10 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
     const long jobs = (long)heads * p.nrb;
     if (p.split != kJobs) {
         const bool each = p.split == kParts || jobs < p.shares, wide = jobs * 16 <= p.shares;           // a block per job; 16 parts a job and more
-        const int rows = p.R < p.rows ? p.R : p.rows;
-        const dim3 grid(each ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + kJoinRows - 1) / kJoinRows), wide ? D / 32 : 1);
-        auto join = tc ? (wide ? attn_join_kernel<D, kTreeTcTile, BF16, 8, 16> : attn_join_kernel<D, kTreeTcTile, BF16, D / 4, 128 / D>)
-                       : (wide ? attn_join_kernel<D, kTile, BF16, 8, 16> : attn_join_kernel<D, kTile, BF16, D / 4, 128 / D>);
+        const int rows = p.R < p.rows ? p.R : p.rows, of = wide ? kJoinRows : 1024 / D;
+        const dim3 grid(each ? (unsigned)jobs : (unsigned)p.shares - 1, (unsigned)((rows + of - 1) / of), wide ? D / 32 : 1);
+        auto join = tc ? (wide ? attn_join_wide_kernel<D, kTreeTcTile, BF16> : attn_join_kernel<D, kTreeTcTile, BF16>)
+                       : (wide ? attn_join_wide_kernel<D, kTile, BF16> : attn_join_kernel<D, kTile, BF16>);
         rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)each), "tree_attention join");
     }
     if (rc || !p.weights) return rc;
@@ -550,6 +609,7 @@ int launch_tree_attention(TreeAttnParams p, bool bf16, uint8_t *ws, cudaStream_t
     p.jobs_each = pl.jobs_each;
     p.part_o = reinterpret_cast<float *>(ws + pl.part_o);
     p.part_ml = reinterpret_cast<float2 *>(ws + pl.part_ml);
+    p.parts_of = reinterpret_cast<int2 *>(ws + pl.parts_of);
     p.lse = p.weights ? reinterpret_cast<float *>(ws + pl.lse) : nullptr;
     p.scores = pl.scores ? reinterpret_cast<float *>(ws + pl.sc) : nullptr;
     p.score_ld = pl.score_ld;
