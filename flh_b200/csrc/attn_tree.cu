@@ -492,26 +492,36 @@ __global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __gr
     if (t0 >= n) return;
     const float *sc = p.scores + (long)bh * p.R * p.score_ld, *lse = p.lse + (long)bh * p.R;
     float *w = p.weights + (long)bh * p.T, was[kWeightEach], sum[kWeightEach] = {};
+    int at[kWeightEach];                   // entries; behind the last one it stands in
 #pragma unroll
     for (int k = 0; k < kWeightEach; ++k) {
-        const int t = t0 + k * kWeightThreads;
-        was[k] = t < n ? w[t] : 0.0f;
+        at[k] = min(t0 + k * kWeightThreads, n - 1);
+        was[k] = w[at[k]];
     }
-#pragma unroll 4
-    for (int r = 0; r < p.R; ++r) {
-        const float at = lse[r];
+    const bool drafted = at[kWeightEach - 1] >= len;                             // some may not be seen by every row
+    for (int r0 = 0; r0 < p.R; r0 += 4) {
+        float x[4][kWeightEach], l[4];     // fetched together
 #pragma unroll
-        for (int k = 0; k < kWeightEach; ++k) {
-            const int t = t0 + k * kWeightThreads;
-            if (t >= n || (t >= len && !((drafted_bits(p, b, token_of(p, r), len) >> (t - len)) & 1))) continue;      // an entry that the row does not see
-            sum[k] += exp2_approx(fmaf(sc[r * p.score_ld + t], p.scale_log2, -at));
+        for (int i = 0; i < 4; ++i) {
+            const int r = min(r0 + i, p.R - 1);
+            l[i] = lse[r];
+#pragma unroll
+            for (int k = 0; k < kWeightEach; ++k) x[i][k] = sc[r * p.score_ld + at[k]];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (r0 + i >= p.R) break;
+            const uint64_t bits = drafted ? drafted_bits(p, b, token_of(p, r0 + i), len) : 0;
+#pragma unroll
+            for (int k = 0; k < kWeightEach; ++k) {
+                const bool seen = at[k] < len || ((bits >> (at[k] - len)) & 1);
+                sum[k] += seen ? exp2_approx(fmaf(x[i][k], p.scale_log2, -l[i])) : 0.0f;
+            }
         }
     }
 #pragma unroll
-    for (int k = 0; k < kWeightEach; ++k) {
-        const int t = t0 + k * kWeightThreads;
-        if (t < n) w[t] = was[k] + sum[k];
-    }
+    for (int k = 0; k < kWeightEach; ++k)
+        if (t0 + k * kWeightThreads < n) w[at[k]] = was[k] + sum[k];
 }
 
 // ---- host side ------------------------------------------------------------------------------
