@@ -62,11 +62,12 @@ __device__ __forceinline__ long q_offset(const TreeAttnParams &p, int b, int kvh
 __device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
 // The drafted entries that a token sees, as bits; those behind the end of the cache do not exist.
-__device__ __forceinline__ uint64_t drafted_bits(const TreeAttnParams &p, int b, int s, int len) {
+__device__ __forceinline__ uint64_t tree_bits(const TreeAttnParams &p, int b, int s) { return p.tree ? (uint64_t)p.tree[b * p.tree_sb + s] : ~0ull >> (63 - s); }
+__device__ __forceinline__ uint64_t existing_bits(const TreeAttnParams &p, int len) {
     const int n = entries(p, len) - len;
-    const uint64_t exist = n >= 64 ? ~0ull : (1ull << n) - 1;
-    return exist & (p.tree ? (uint64_t)p.tree[b * p.tree_sb + s] : ~0ull >> (63 - s));
+    return n >= 64 ? ~0ull : (1ull << n) - 1;
 }
+__device__ __forceinline__ uint64_t drafted_bits(const TreeAttnParams &p, int b, int s, int len) { return existing_bits(p, len) & tree_bits(p, b, s); }
 
 // Tiles of all jobs up to sequence b (exclusive); warp-uniform.  upto = B: all of them.
 template <int TILE>
@@ -171,11 +172,15 @@ struct Parts {
 template <int TILE>
 __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, JobWalk<TILE> &job, int &u0, int &u1) {
     if (p.split == kJobs) {
-        const int all = p.B * p.nkv * p.nrb, first = blockIdx.x * p.jobs_each;
-        JobWalk<TILE> last;
-        last.at(p, min(first + p.jobs_each, all) - 1, lane);
-        job.at(p, first, lane);
-        u0 = job.begin;
+        const int per = p.nkv * p.nrb, first = blockIdx.x * p.jobs_each, count = min(p.jobs_each, p.B * per - first);
+        job.b = first / per;
+        job.job = first - job.b * per;
+        job.len = uniform(committed(p, job.b));
+        job.nt = (entries(p, job.len) + TILE - 1) / TILE;
+        job.begin = 0;                     // its own count of tiles
+        JobWalk<TILE> last = job;
+        for (int i = 1; i < count; ++i) last.next(p);
+        u0 = 0;
         u1 = last.begin + last.nt;
     } else if (p.split == kParts) {
         Parts<TILE> c;
@@ -220,6 +225,11 @@ template <bool BF16> __device__ __forceinline__ float load16(const void *p, long
 template <bool BF16> __device__ __forceinline__ void store16(void *p, long i, float x) {
     if (BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
     else static_cast<__half *>(p)[i] = __float2half_rn(x);
+}
+// whether one of eight 16-bit values is not finite: then its exponent, all ones, carries into the sign's place
+template <bool BF16> __device__ __forceinline__ bool any_nonfinite(const uint4 x) {
+    const uint32_t e = BF16 ? 0x7f807f80u : 0x7c007c00u, one = BF16 ? 0x00800080u : 0x04000400u;
+    return (((x.x & e) + one) | ((x.y & e) + one) | ((x.z & e) + one) | ((x.w & e) + one)) & 0x80008000u;
 }
 // 16-bit values of a word that are not finite, as zero
 template <bool BF16> __device__ __forceinline__ uint32_t finite2(uint32_t w) {

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const CUtensorMap *map = item & 1 ? &vmap : &kmap;
             mbar_expect_tx(bar, kSlot);
             for (int h = 0; h < D / 64; ++h)
-                tma_load_tile(dst + h * (kTile * 128), map, h * 64, (u_ahead - ahead.begin) * kTile, ahead.b * p.nkv + ahead.job / p.nrb, bar);
+                tma_load_tile(dst + h * (kTile * 128), map, h * 64, (u_ahead - ahead.begin) * kTile, ahead.b * p.nkv + ahead.job, bar);
         }
         if (item & 1) u_ahead += kWarps;
         ++item;
@@ -113,22 +113,21 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
     uint4 qv[kQLoads];
     uint64_t bits = 0;
     auto fetch_q = [&](const JobWalk<kTile> &j) {
-        const int kvh = j.job / p.nrb, row0 = (j.job - kvh * p.nrb) * kRows;
 #pragma unroll
         for (int i = 0; i < kQLoads; ++i) {
-            const int row = row0 + q_r + i * kQStep;
-            qv[i] = row < p.R ? ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, j.b, kvh, row) + q_c * 8) : make_uint4(0, 0, 0, 0);
+            const int row = q_r + i * kQStep;
+            qv[i] = row < p.R ? ldg_v4(static_cast<const uint16_t *>(p.q) + q_offset(p, j.b, j.job, row) + q_c * 8) : make_uint4(0, 0, 0, 0);
         }
-        if (tid < kRows) bits = row0 + tid < p.R ? drafted_bits(p, j.b, token_of(p, row0 + tid), j.len) : 0;
+        if (tid < p.R) bits = tree_bits(p, j.b, token_of(p, tid));
     };
     fetch_q(cur);
     for (int piece = u0; piece < u1;) {
         const int piece_end = min(u1, cur.begin + cur.nt);
-        const int b = cur.b, kvh = cur.job / p.nrb, row0 = (cur.job - kvh * p.nrb) * kRows, len = cur.len, n = entries(p, len);
+        const int b = cur.b, kvh = cur.job, len = cur.len, n = entries(p, len);                // one block of rows a job
         __syncthreads();                   // the piece before is written out
 #pragma unroll
         for (int i = 0; i < kQLoads; ++i) *reinterpret_cast<uint4 *>(sm_q + (q_r + i * kQStep) * q_pitch<D>() + q_c * 16) = qv[i];
-        if (tid < kRows) seen[tid] = bits;
+        if (tid < kRows) seen[tid] = tid < p.R ? bits & existing_bits(p, len) : 0;
         if (tid == 0) bad = 0;
         __syncthreads();
         float o[kDT][4], m[2], l[2];
@@ -183,7 +182,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             if (p.scores) {
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    const int row = row0 + grp + hh * 8;
+                    const int row = grp + hh * 8;
                     if (row < p.R) {
                         float *dst = p.scores + (((long)b * p.nkv + kvh) * p.R + row) * p.score_ld + key0 + quad * 2;
 #pragma unroll
@@ -224,17 +223,15 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             if (!alive) break;
             const uint32_t vs = ring_u + slot * kSlot;
             if (tail) {
-                // rows of V behind the sequence's end become zero, and so do values of drafted entries that are not finite
+                // values that are not finite become zero, of drafted entries and of what lies behind the sequence's end
                 const int row = max(len - key0, 0) + lane / (D / 8), chunk = lane % (D / 8);      // the rows behind the committed ones
 #pragma unroll 4
                 for (int r = row; r < kTile; r += 32 / (D / 8)) {
-                    const int t = key0 + r;
                     uint4 *at = reinterpret_cast<uint4 *>(ring + slot * kSlot + swizzled<kTile>(r, chunk));
-                    const uint4 was = *at;
-                    const uint4 is = t >= n ? make_uint4(0, 0, 0, 0) : make_uint4(finite2<BF16>(was.x), finite2<BF16>(was.y), finite2<BF16>(was.z), finite2<BF16>(was.w));
-                    if (is.x != was.x || is.y != was.y || is.z != was.z || is.w != was.w) {
-                        *at = is;
-                        if (t < n) atomicOr(&bad, 1ull << (t - len));
+                    const uint4 x = *at;
+                    if (any_nonfinite<BF16>(x)) {
+                        if (key0 + r < n) atomicOr(&bad, 1ull << (key0 + r - len));
+                        *at = make_uint4(finite2<BF16>(x.x), finite2<BF16>(x.y), finite2<BF16>(x.z), finite2<BF16>(x.w));
                     }
                 }
                 __syncwarp();
@@ -263,26 +260,39 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             if (quad == 0) { sm_m[warp][grp + hh * 8] = m[hh]; sm_l[warp][grp + hh * 8] = sum; }
         }
         __syncthreads();
-        float mine[2];
+        // a row's factors: of every warp, and of the sum
+        if (tid < kRows) {
+            float top = sm_m[0][tid], sum = 0.0f;
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-            const int r = grp + hh * 8;
-            float top = sm_m[0][r];
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][tid]);
+            const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-            mine[hh] = exp2_approx(m[hh] - (top == -INFINITY ? 0.0f : top));
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = exp2_approx(sm_m[w][tid] - base);
+                sum += sm_l[w][tid] * f;
+                sm_m[w][tid] = f;
+            }
+            const bool whole_job = piece == cur.begin && piece_end == cur.begin + cur.nt;
+            sm_l[0][tid] = whole_job ? row_factor(sum, len == 0 && !seen[tid]) : 1.0f;
+            sm_l[1][tid] = base;
+            if (tid < p.R) {
+                if (!whole_job) p.part_ml[(2L * blockIdx.x + (piece != u0)) * kRows + tid] = make_float2(top, sum);
+                else if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + tid] = base + log2f(sum);
+            }
         }
-        const bool whole = piece == cur.begin && piece_end == cur.begin + cur.nt;
-        const long part = 2L * blockIdx.x + (piece != u0);
         JobWalk<kTile> next = cur;
         if (piece_end < u1) {
             next.next(p);
             fetch_q(next);
         }
+        __syncthreads();
+        const float mine[2] = {sm_m[warp][grp], sm_m[warp][grp + 8]};
+        const bool whole = piece == cur.begin && piece_end == cur.begin + cur.nt;
+        const long part = 2L * blockIdx.x + (piece != u0);
         constexpr int kChunk = 4 * 128 / D;                                      // rows whose sums of all warps fit the buffer (8 KB)
 #pragma unroll
         for (int r0 = 0; r0 < kRows; r0 += kChunk) {
-            if (row0 + r0 >= p.R) break;
+            if (r0 >= p.R) break;
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 const int r = hh * 8 + grp;
@@ -293,29 +303,29 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
                 }
             }
             __syncthreads();
+            // a thread has four columns of a row
+            const int r = r0 + tid / (D / 4), d = tid % (D / 4) * 4;
+            if (r < p.R) {
+                float4 acc = *reinterpret_cast<const float4 *>(sm_o + (r - r0) * D + d);
 #pragma unroll
-            for (int i = tid; i < kChunk * D; i += kThreadsAttn) {
-                const int r = r0 + i / D, d = i % D, row = row0 + r;
-                if (row >= p.R) continue;
-                float top = sm_m[0][r], sum = 0.0f, acc = 0.0f;
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_m[w][r]);
-                const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    sum += sm_l[w][r] * exp2_approx(sm_m[w][r] - base);
-                    acc += sm_o[(w * kChunk + r - r0) * D + d];
+                for (int w = 1; w < kWarps; ++w) {
+                    const float4 v = *reinterpret_cast<const float4 *>(sm_o + (w * kChunk + r - r0) * D + d);
+                    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
                 }
-                if (bad) acc += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, row, d, len, base);
+                if (bad) {
+                    const float base = sm_l[1][r];
+                    acc.x += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, r, d, len, base);
+                    acc.y += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, r, d + 1, len, base);
+                    acc.z += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, r, d + 2, len, base);
+                    acc.w += nonfinite_part<BF16>(p, bad, seen[r], b, kvh, r, d + 3, len, base);
+                }
                 if (whole) {
-                    const int s = token_of(p, row), h = kvh * p.g + row - s * p.g;
-                    store16<BF16>(p.out, (((long)b * p.S + s) * p.nh + h) * D + d, acc * row_factor(sum, len == 0 && !seen[r]));
+                    const float f = sm_l[0][r];
+                    const int s = token_of(p, r), h = kvh * p.g + r - s * p.g;
+                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + (((long)b * p.S + s) * p.nh + h) * D + d) =
+                        make_uint2(narrow<BF16>(acc.x * f, acc.y * f), narrow<BF16>(acc.z * f, acc.w * f));
                 } else {
-                    p.part_o[part * kRows * D + (d >> 2) * (kRows * 4) + r * 4 + (d & 3)] = acc;
-                }
-                if (d == 0) {
-                    if (whole) { if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + row] = base + log2f(sum); }
-                    else p.part_ml[part * kRows + r] = make_float2(top, sum);
+                    *reinterpret_cast<float4 *>(p.part_o + part * kRows * D + d * kRows + r * 4) = acc;
                 }
             }
             if (r0 + kChunk < kRows) __syncthreads();

@@ -322,27 +322,25 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     tc_wait_st();
                 }
                 if (tail) {
-                    // rows of V behind the sequence's end become zero, and so do values of drafted entries that are not finite: half
-                    // a row a thread.  (Both streams do it where they share a tile; an entry is marked before it is changed.)
+                    // values of V that are not finite become zero, of drafted entries and of what lies behind the sequence's end: half a row
+                    // a thread.  (Both streams do it where they share a tile; an entry is marked before it is changed.)
                     const int item = 2 * (piece - u0 + t) + 1, slot = item % kItems, vr = wg >> 1, at = key0 + vr;
                     if (wait(fulls + 8 * slot, item / kItems, 47) && at >= len) {
                         uint8_t *v = smem + slot * kItem + vr * 128;
-                        uint4 was[D / 16], is[D / 16];
-                        bool changed = false;
+                        uint32_t odd = 0;                                        // pieces with such a value, a bit each
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) {
                             const int ch = (wg & 1) * (D / 16) + j;
-                            was[j] = *reinterpret_cast<const uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4));
-                            is[j] = at >= n ? make_uint4(0, 0, 0, 0) : make_uint4(finite2<BF16>(was[j].x), finite2<BF16>(was[j].y), finite2<BF16>(was[j].z), finite2<BF16>(was[j].w));
-                            changed |= is[j].x != was[j].x || is[j].y != was[j].y || is[j].z != was[j].z || is[j].w != was[j].w;
+                            odd |= (uint32_t)any_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4))) << j;
                         }
-                        if (changed) {
+                        if (odd) {
                             if (at < n) atomicOr(&bad[which], 1ull << (at - len));
                             __threadfence_block();
-#pragma unroll
                             for (int j = 0; j < D / 16; ++j) {
                                 const int ch = (wg & 1) * (D / 16) + j;
-                                *reinterpret_cast<uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4)) = is[j];
+                                uint4 *q = reinterpret_cast<uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4));
+                                const uint4 w = *q;
+                                *q = make_uint4(finite2<BF16>(w.x), finite2<BF16>(w.y), finite2<BF16>(w.z), finite2<BF16>(w.w));
                             }
                             fence_proxy_async();
                         }
