@@ -208,11 +208,7 @@ __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, Jo
     }
 }
 
-// Two 16-bit values of the tensors' type as binary32, and back.
-template <bool BF16> __device__ __forceinline__ float2 widen(uint32_t w) {
-    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
+// Two values rounded to the tensors' type; one value of it.
 template <bool BF16> __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
     if (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -221,10 +217,6 @@ template <bool BF16> __device__ __forceinline__ uint32_t narrow(float lo, float 
 template <bool BF16> __device__ __forceinline__ float load16(const void *p, long i) {
     if (BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
     return __half2float(static_cast<const __half *>(p)[i]);
-}
-template <bool BF16> __device__ __forceinline__ void store16(void *p, long i, float x) {
-    if (BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
-    else static_cast<__half *>(p)[i] = __float2half_rn(x);
 }
 // whether one of eight 16-bit values is not finite: then its exponent, all ones, carries into the sign's place
 template <bool BF16> __device__ __forceinline__ bool any_nonfinite(const uint4 x) {

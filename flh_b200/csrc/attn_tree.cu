@@ -333,6 +333,9 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
         piece = piece_end;
         cur = next;
     }
+    if (!alive)                            // a wait ran out: what is still on its way lands before the CTA leaves
+        for (int i = used; i < item; ++i)
+            for (int tries = 0; tries < 10000 && !__all_sync(0xffffffffu, mbar_try_hint(full_u + 8 * (i % kSlots), (i / kSlots) & 1, 20000u)); ++tries);
 }
 
 // Jobs that several CTAs hold: their partial results in order.  A block for each job, or (kEven) for each cut between two shares where that
@@ -560,8 +563,9 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     pl.score_ld = (T + kTile - 1) / kTile * kTile;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-    pl.part_o = take((size_t)2 * pl.shares * pl.rows * D * 4);
-    pl.part_ml = take((size_t)2 * pl.shares * pl.rows * 8);
+    const size_t slots = pl.split == kJobs ? 0 : (size_t)2 * pl.shares * pl.rows;
+    pl.part_o = take(slots * D * 4);
+    pl.part_ml = take(slots * 8);
     pl.parts_of = take((size_t)pl.shares * 8);
     pl.lse = take(weights ? (size_t)B * nkv * R * 4 : 0);
     pl.sc = take(pl.scores ? (size_t)B * nkv * R * pl.score_ld * 4 : 0);
@@ -584,7 +588,8 @@ template <int D, bool BF16>
 int launch_mma(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     auto kern = attn_mma_kernel<D, BF16>;
     constexpr int smem = attn_smem<D>();
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
     return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsAttn, smem, stream, p, km, vm), "tree_attention launch");
 }

@@ -612,7 +612,8 @@ template <int D, bool BF16>
 int launch_weights(const TreeAttnParams &p, const CUtensorMap &km, cudaStream_t stream) {
     auto kern = attn_weights_tc_kernel<D, BF16>;
     constexpr int smem = smem_weights<D>();
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
     // two CTAs for every SM, but none without a tile
     const long heads = (long)p.B * p.nkv, tiles = (p.T + kWeightTile - 1) / kWeightTile, want = heads >= 2L * kNumSMs ? 1 : 2L * kNumSMs / heads;
@@ -623,7 +624,8 @@ template <int D, bool TWO, bool BF16>
 int launch_tc(const TreeAttnParams &p, const CUtensorMap &km, const CUtensorMap &vm, cudaStream_t stream) {
     auto kern = attn_tc_kernel<D, TWO, BF16>;
     constexpr int smem = smem_tc<D, TWO>();
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
     return cuda_status(launch_pdl(kern, dim3((unsigned)p.shares), kThreadsTcA, smem, stream, p, km, vm), "tree_attention launch");
 }

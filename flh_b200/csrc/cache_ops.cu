@@ -397,7 +397,8 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     const long each = (T + blocks - 1) / blocks + 2048;                  // a block's stretch, rounded up to whole spans
     const int cap = (int)(each < kSelKeys ? each : kSelKeys);
     auto select = few ? evict_select_kernel<256> : evict_select_kernel<512>;
-    const cudaError_t e = cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+    static std::atomic<uint64_t> done[2];
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(select), kSelKeys * 4, done[few]);
     if (e != cudaSuccess) return cuda_status(e, "cache_evict shared memory");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
