@@ -57,6 +57,44 @@ template <int ROWS> __device__ __forceinline__ uint32_t swizzled(int row, int ch
     return (chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
+// weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
+// 2 D for reading K again).  A thread has EACH entries, t0 and every stride-th, and fetches ROWS rows' scores of them together.
+template <int ROWS, int EACH>
+__device__ __forceinline__ void add_weights(const TreeAttnParams &p, int b, int bh, int len, int n, int t0, int stride, const float *lse) {
+    const float *sc = p.scores + (long)bh * p.R * p.score_ld;
+    float *w = p.weights + (long)bh * p.T, was[EACH], sum[EACH] = {};
+    int at[EACH];                   // entries; behind the last one it stands in
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        at[k] = min(t0 + k * stride, n - 1);
+        was[k] = w[at[k]];
+    }
+    const bool drafted = at[EACH - 1] >= len;                             // some may not be seen by every row
+    for (int r0 = 0; r0 < p.R; r0 += ROWS) {
+        float x[ROWS][EACH], l[ROWS];     // fetched together
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int r = min(r0 + i, p.R - 1);
+            l[i] = lse[r];
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) x[i][k] = sc[r * p.score_ld + at[k]];
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            if (r0 + i >= p.R) break;
+            const uint64_t bits = drafted ? drafted_bits(p, b, token_of(p, r0 + i), len) : 0;
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) {
+                const bool seen = at[k] < len || ((bits >> (at[k] - len)) & 1);
+                sum[k] += seen ? exp2_approx(fmaf(x[i][k], p.scale_log2, -l[i])) : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+        if (t0 + k * stride < n) w[at[k]] = was[k] + sum[k];
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap) {
@@ -275,9 +313,10 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             const bool whole_job = piece == cur.begin && piece_end == cur.begin + cur.nt;
             sm_l[0][tid] = whole_job ? row_factor(sum, len == 0 && !seen[tid]) : 1.0f;
             sm_l[1][tid] = base;
+            sm_l[2][tid] = base + log2f(sum);
             if (tid < p.R) {
                 if (!whole_job) p.part_ml[(2L * blockIdx.x + (piece != u0)) * kRows + tid] = make_float2(top, sum);
-                else if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + tid] = base + log2f(sum);
+                else if (p.lse) p.lse[((long)b * p.nkv + kvh) * p.R + tid] = sm_l[2][tid];
             }
         }
         JobWalk<kTile> next = cur;
@@ -330,6 +369,12 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
             }
             if (r0 + kChunk < kRows) __syncthreads();
         }
+        // no job is cut: what its rows gave its entries is added here (16 sequences of 766 .. 1,531: 51 us without weights, 55 with, 59 as a launch of its own)
+        if (p.scores && p.split == kJobs)
+            for (int t0 = tid; t0 < n; t0 += (p.R == 1 ? 12 : 4) * kThreadsAttn) {
+                if (p.R == 1) add_weights<1, 12>(p, b, b * p.nkv + kvh, len, n, t0, kThreadsAttn, sm_l[2]);
+                else add_weights<4, 4>(p, b, b * p.nkv + kvh, len, n, t0, kThreadsAttn, sm_l[2]);
+            }
         piece = piece_end;
         cur = next;
     }
@@ -494,47 +539,14 @@ __global__ void __launch_bounds__(1024) attn_join_wide_kernel(const __grid_const
     store_joined<D, BF16>(p, b, kvh, row, group, base, sum, acc);
 }
 
-// weights += sum over the rows of 2^(score - lse), from the scores that the attention left (few rows: 8 R bytes an entry against
-// 2 D for reading K again).  A thread has four entries, 256 apart, so that it waits for memory once for all of them.
+// The same where jobs were cut: a launch behind the join.
 constexpr int kWeightThreads = 256, kWeightEach = 4;
 __global__ void __launch_bounds__(kWeightThreads) attn_weights_kernel(const __grid_constant__ TreeAttnParams p) {
     const int bh = blockIdx.x, t0 = blockIdx.y * kWeightThreads * kWeightEach + threadIdx.x;
     pdl_wait();
     pdl_trigger();
     const int b = bh / p.nkv, len = committed(p, b), n = entries(p, len);
-    if (t0 >= n) return;
-    const float *sc = p.scores + (long)bh * p.R * p.score_ld, *lse = p.lse + (long)bh * p.R;
-    float *w = p.weights + (long)bh * p.T, was[kWeightEach], sum[kWeightEach] = {};
-    int at[kWeightEach];                   // entries; behind the last one it stands in
-#pragma unroll
-    for (int k = 0; k < kWeightEach; ++k) {
-        at[k] = min(t0 + k * kWeightThreads, n - 1);
-        was[k] = w[at[k]];
-    }
-    const bool drafted = at[kWeightEach - 1] >= len;                             // some may not be seen by every row
-    for (int r0 = 0; r0 < p.R; r0 += 4) {
-        float x[4][kWeightEach], l[4];     // fetched together
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = min(r0 + i, p.R - 1);
-            l[i] = lse[r];
-#pragma unroll
-            for (int k = 0; k < kWeightEach; ++k) x[i][k] = sc[r * p.score_ld + at[k]];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (r0 + i >= p.R) break;
-            const uint64_t bits = drafted ? drafted_bits(p, b, token_of(p, r0 + i), len) : 0;
-#pragma unroll
-            for (int k = 0; k < kWeightEach; ++k) {
-                const bool seen = at[k] < len || ((bits >> (at[k] - len)) & 1);
-                sum[k] += seen ? exp2_approx(fmaf(x[i][k], p.scale_log2, -l[i])) : 0.0f;
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < kWeightEach; ++k)
-        if (t0 + k * kWeightThreads < n) w[at[k]] = was[k] + sum[k];
+    if (t0 < n) add_weights<4, kWeightEach>(p, b, bh, len, n, t0, kWeightThreads, p.lse + (long)bh * p.R);
 }
 
 // ---- host side ------------------------------------------------------------------------------
@@ -609,7 +621,7 @@ int launch_attention(const TreeAttnParams &p, const CUtensorMap &km, const CUten
                        : (wide ? attn_join_wide_kernel<D, kTile, BF16> : attn_join_kernel<D, kTile, BF16>);
         rc = cuda_status(launch_pdl(join, grid, wide ? 1024 : 256, 0, stream, p, (int)each), "tree_attention join");
     }
-    if (rc || !p.weights) return rc;
+    if (rc || !p.weights || (p.scores && p.split == kJobs)) return rc;
     if (p.scores) {
         const int each = kWeightThreads * kWeightEach;
         return cuda_status(launch_pdl(attn_weights_kernel, dim3(heads, (unsigned)((p.T + each - 1) / each)), kWeightThreads, 0, stream, p), "tree_attention weights");
