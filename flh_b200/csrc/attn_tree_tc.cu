@@ -191,9 +191,11 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 wait(fulls + 8 * ks, kph, 42);
                 qk();
             }
+            // whether a load is there is asked before the products that come first are issued, and the answer looked at behind them
+            bool v_there = mine > 0 && mbar_test(fulls + 8 * vs, vph), k_there = true;
             for (int i = 0; i < mine; ++i) {
-                wait(fulls + 8 * vs, vph, 45);
-                if (i + 2 < mine) wait(fulls + 8 * ks, kph, 42);
+                if (!__all_sync(0xffffffffu, v_there)) wait(fulls + 8 * vs, vph, 45);
+                if (i + 2 < mine) k_there = mbar_test(fulls + 8 * ks, kph);
                 bar_sync_named(3 + 2 * x + (nv & 1), 160);                       // the weights are written
                 tc_fence_after();
                 const uint64_t b = umma_desc_tc(ring + vs * kItem, kHalf, 1024);
@@ -207,7 +209,11 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 __syncwarp();
                 ++nv;
                 advance(vs, vph, kAdvance);
-                if (i + 2 < mine) qk();
+                if (i + 1 < mine) v_there = mbar_test(fulls + 8 * vs, vph);
+                if (i + 2 < mine) {
+                    if (!__all_sync(0xffffffffu, k_there)) wait(fulls + 8 * ks, kph, 42);
+                    qk();
+                }
             }
             bar_arrive_named(2, 320);                                            // this warp has seen the piece's q: the next may come (also after a wait that ran out)
             piece = end;
