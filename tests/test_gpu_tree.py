@@ -447,3 +447,84 @@ def test_a_run_of_steps(cuda):
                 got = w[b, h, :n].double()
                 assert torch.allclose(got, torch.stack([e[2] for e in held[b][h]]), rtol=1e-4, atol=1e-6)
                 assert not w[b, h, n:].any()
+
+
+def test_recorded_append_accept_and_evict(cuda):
+    """The other calls in one graph, replayed with other lengths and paths, against the same calls made eagerly."""
+    from flh_b200.model import rope_tables
+    L, B, nkv, T, D, S, nh = 2, 3, 2, 120, 64, 6, 4
+    cos, sin = rope_tables(torch.arange(300, device="cuda"), D, 10000.0)
+    k, v, w = _layers(31, L, B, nkv, T, D, torch.float16)
+    qkv, lengths, path, accepted = _normal(32, B * S, (nh + 2 * nkv) * D), _ints([5, 6, 7]), _ints([[0, 2, 4]] * B), _ints([1, 2, 3])
+    positions = (lengths[:, None] + torch.arange(S, dtype=torch.int32, device="cuda")).contiguous()
+
+    def calls(k, v, w):
+        q = [cuda.rope_kv_at(qkv, cos, sin, positions, lengths, k[y], v[y], nh) for y in range(L)]
+        now = cuda.cache_accept(list(k), list(v), lengths, path, accepted, S, weights=list(w))
+        kept, left, after = cuda.cache_evict(list(k), list(v), list(w), now, 20, 4)
+        return [*q, now, kept, left, after]
+
+    calls(*(x.clone() for x in (k, v, w)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        outs = calls(k, v, w)
+    for n, paths, counts in (([100, 0, 50], [[1, 2, 5], [0, 1, 2], [3, 4, 5]], [3, 1, 0]), ([114, 20, 30], [[0, 1, 2]] * 3, [3, 3, 3])):
+        lengths.copy_(_ints(n)), path.copy_(_ints(paths)), accepted.copy_(_ints(counts))
+        positions.copy_(lengths[:, None] + torch.arange(S, dtype=torch.int32, device="cuda"))
+        copies = [x.clone() for x in (k, v, w)]
+        g.replay()
+        want = calls(*copies)
+        for a, b in zip([*outs, k, v, w], [*want, *copies]):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_a_stream_of_their_own_and_without_the_native_ones(cuda, monkeypatch):
+    k, v, w = _layers(41, 2, 2, 2, 90, 128, torch.bfloat16)
+    q, lengths = _normal(42, 2, 3, 4, 128, dtype=torch.bfloat16), _ints([60, 33])
+    path, accepted = _ints([[0, 2], [1, 2]]), _ints([2, 2])
+
+    def calls(k, v, w):
+        out = cuda.tree_attention(q, k[0], v[0], lengths, weights=w[0])
+        now = cuda.cache_accept(list(k), list(v), lengths, path, accepted, 3, weights=list(w))
+        return [out, now, *cuda.cache_evict(list(k), list(v), list(w), now, 30, 5), k, v, w]
+
+    want = calls(*(x.clone() for x in (k, v, w)))
+    copies = [x.clone() for x in (k, v, w)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = calls(*copies)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    monkeypatch.setattr(cuda, "_host", None)
+    got = calls(*(x.clone() for x in (k, v, w)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_empty_batches(cuda):
+    k, n = torch.zeros(0, 2, 10, 64, dtype=torch.float16, device="cuda"), _ints([])
+    assert cuda.tree_attention(torch.zeros(0, 3, 4, 64, dtype=torch.float16, device="cuda"), k, k.clone(), n).shape == (0, 3, 4, 64)
+    assert cuda.cache_accept([k], [k.clone()], n, torch.zeros(0, 2, dtype=torch.int32, device="cuda"), n.clone(), 3).shape == (0,)
+    kept, left, now = cuda.cache_evict([k], [k.clone()], [torch.zeros(0, 2, 10, device="cuda")], n, 4, 1)
+    assert kept.shape == (1, 0, 2, 4) and left.shape == (1, 0, 2, 10) and now.shape == (0,)
+    one = _layers(1, 1, 2, 2, 10, 64, torch.float16)
+    assert cuda.cache_accept([one[0][0]], [one[1][0]], _ints([3, 4]), torch.zeros(2, 0, dtype=torch.int32, device="cuda"), _ints([5, 5]), 3).tolist() == [3, 4]
+
+
+@pytest.mark.parametrize("B,S,nh,nkv", [(40, 2, 8, 2), (40, 20, 8, 2), (3, 40, 64, 8), (300, 1, 2, 2), (33, 64, 16, 2)])
+def test_every_division_of_the_work(cuda, B, S, nh, nkv):
+    """More jobs than CTAs, more sequences than a warp has lanes, jobs that are cut and jobs that are not, in a cache with room to spare."""
+    r = rs(B)
+    for T, top in ((4000, 700), (150, 80)):
+        lengths = [int(x) for x in r.randint(0, top, size=B)]
+        q, k, v = _normal(1, B, S, nh, 64), _normal(2, B, nkv, T, 64), _normal(3, B, nkv, T, 64)
+        w = torch.zeros(B, nkv, T, device="cuda")
+        out = cuda.tree_attention(q, k, v, _ints(lengths), weights=w)
+        some = sorted(set([0, 1, B // 2, B - 1, *r.randint(0, B, size=4).tolist()]))
+        want, tol, ww, wtol = R.attention(q[some], k[some, :, :top + S], v[some, :, :top + S], [lengths[b] for b in some])
+        R.assert_close(out[some], want, tol)
+        R.assert_close(w[some][:, :, :top + S], ww, wtol + 2.0 ** -24 * ww)
+        assert torch.allclose(w.sum(-1), torch.full((B, nkv), float(S * nh // nkv), device="cuda"), rtol=1e-4)
+    assert cuda.tree_attention_status()[0] == 0
