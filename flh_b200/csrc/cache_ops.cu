@@ -171,14 +171,14 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t ran
 // A block per row, or a cluster of blocks that have a stretch of it each.  The smallest key that is kept is found digit by digit, eight
 // bits at a time, by counting the keys that agree with the digits found so far; then the row is walked in order, every warp over a
 // part of its own, and what lies above that key is kept, of the equal ones the first few.  The keys stay in shared memory (cap: how
-// many fit; the rest is read again).  Every lane counts in a histogram of its own: weights are much alike in their leading bits.  (With 8
+// many fit; the rest is read again).  Every lane (in small blocks every fourth) counts in a histogram of its own: weights are much alike in their leading bits.  (With 8
 // copies of the counters 256 rows of 8,192 took 31 us, finding the key two bits at a time by comparisons in registers 33, counting
 // equal digits of a warp once 28; this 25.)
-template <int THREADS>
+template <int THREADS, int COPIES>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
     constexpr int kWarps = THREADS / 32;
     extern __shared__ uint32_t keys[];
-    __shared__ __align__(16) uint32_t hist[256 * 32];     // [digit][lane]
+    __shared__ __align__(16) uint32_t hist[256 * COPIES]; // [digit][lane % COPIES]
     __shared__ uint32_t digits[2][256];    // of one digit and the next, in turn: the cluster may still read the last ones
     __shared__ uint32_t total[256];
     __shared__ uint32_t found[2];          // prefix, how many of the keys that match it are to be kept
@@ -212,24 +212,26 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     if (need) {
         for (int shift = 24, turn = 0; shift >= 0; shift -= 8, turn ^= 1) {
 #pragma unroll
-            for (int i = 0; i < 256 * 8 / THREADS; ++i) reinterpret_cast<uint4 *>(hist)[tid + i * THREADS] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 64 * COPIES / THREADS; ++i) reinterpret_cast<uint4 *>(hist)[tid + i * THREADS] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
 #pragma unroll 4
             for (int i = tid; i < own; i += THREADS) {
                 const uint32_t u = key(i);
-                if ((u & mask) == prefix) atomicAdd(&hist[((u >> shift) & 255u) * 32 + lane], 1u);
+                if ((u & mask) == prefix) atomicAdd(&hist[((u >> shift) & 255u) * COPIES + lane % COPIES], 1u);
             }
             __syncthreads();
-            // four lanes have eight of a digit's counts each
+            // a lane has eight of a digit's counts
+            constexpr int kLanes = COPIES / 8;
 #pragma unroll
-            for (int i = 0; i < 256 / kWarps; i += 8) {
-                const int d = warp * (256 / kWarps) + i + (lane >> 2);
-                const uint4 u = *reinterpret_cast<const uint4 *>(&hist[d * 32 + (lane & 3) * 4]), v = *reinterpret_cast<const uint4 *>(&hist[d * 32 + 16 + (lane & 3) * 4]);
+            for (int i = 0; i < 256 / kWarps; i += 32 / kLanes) {
+                const int d = warp * (256 / kWarps) + i + lane / kLanes;
+                const uint32_t *h = &hist[d * COPIES + lane % kLanes * 4];
+                const uint4 u = *reinterpret_cast<const uint4 *>(h), v = *reinterpret_cast<const uint4 *>(h + COPIES / 2);
                 uint32_t c = u.x + u.y + u.z + u.w + v.x + v.y + v.z + v.w;
-                c += __shfl_xor_sync(0xffffffffu, c, 1);
-                c += __shfl_xor_sync(0xffffffffu, c, 2);
-                if ((lane & 3) == 0) digits[turn][d] = c;
+#pragma unroll
+                for (int o = 1; o < kLanes; o <<= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+                if (lane % kLanes == 0) digits[turn][d] = c;
             }
             if (blocks > 1) {
                 cluster_sync_of();
@@ -396,7 +398,7 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     const bool few = T <= 2048;
     const long each = (T + blocks - 1) / blocks + 2048;                  // a block's stretch, rounded up to whole spans
     const int cap = (int)(each < kSelKeys ? each : kSelKeys);
-    auto select = few ? evict_select_kernel<256> : evict_select_kernel<512>;
+    auto select = few ? evict_select_kernel<256, 8> : evict_select_kernel<512, 32>;
     static std::atomic<uint64_t> done[2];
     const cudaError_t e = allow_smem(reinterpret_cast<const void *>(select), kSelKeys * 4, done[few]);
     if (e != cudaSuccess) return cuda_status(e, "cache_evict shared memory");
@@ -413,7 +415,7 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     // A block per half of a row's pieces (128 bytes of a head of 128), so that one layer of one sequence already spreads over the GPU:
     // 256 threads with 8 pieces each (512 MB: 95 us; with 4 pieces 126).  Where that is a block for half of the SMs or less and each has
     // much to move, quarters and 512 threads (16 heads, 24,000 -> 15,600 entries: 105 -> 71 us in all); where it is little, 128 threads with 4
-    // pieces, of which more fit an SM (1,536 heads, 700 -> 197 entries: 130 -> 99 us).
+    // pieces, of which more fit an SM (1,536 heads, 700 -> 197 entries: 130 -> 82 us with the smaller blocks of the selection).
     const bool much = rows * 4 <= kNumSMs / 2 && keep > 2048 && p.chunks % 4 == 0 && p.chunks >= 8, little = keep <= 512;
     const int slabs = much ? 4 : p.chunks % 2 == 0 && p.chunks >= 8 ? 2 : 1, slab = p.chunks / slabs;
     const dim3 grid((unsigned)(B * nkv * 2 * slabs), (unsigned)layers);
