@@ -315,6 +315,17 @@ class Decoder(torch.nn.Module):
                 + ([torch.zeros(batch, nkv, max_len, dtype=torch.float32, device=self.device)] if observe else [])
                 for _ in range(c.n_layers)]
 
+    def _draft_tables(self):
+        """The rotary tables over all positions, kept from the first call on for every stream: so they are waited for once.  Those that
+        are made while a graph is recorded belong to the graph, and hold nothing before it is replayed."""
+        if self._tables is not None:
+            return self._tables
+        tables = rope_tables(torch.arange(self.cfg.max_positions, device=self.device), self.cfg.head_dim, self.cfg.rope_theta)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(self.device).synchronize()
+            self._tables = tables
+        return tables
+
     @torch.no_grad()
     def draft(self, ids, cache, lengths, tree=None, positions=None):
         """One pass over drafted tokens ids [B, S] (S = 1 .. 64): token s of sequence b goes to entry lengths[b] + s of the cache and sees
@@ -324,14 +335,13 @@ class Decoder(torch.nn.Module):
         a head).  lengths and positions are read on the device: a recorded step follows them.  What is kept of the tokens is
         what accept() is told."""
         B, S = ids.shape
-        if self._tables is None:
-            self._tables = rope_tables(torch.arange(self.cfg.max_positions, device=self.device), self.cfg.head_dim, self.cfg.rope_theta)
+        tables = self._draft_tables()
         at = lengths if positions is None else positions
         at = at[:, None] + (torch.arange(S, dtype=torch.int32, device=self.device) if tree is None else tree.depth)
         bits = None if tree is None else tree.bits
         x, pre = self.embed(ids), None
         for i, layer in enumerate(self.layers):
-            out = layer(x, None, cache[i], self._tables, pre=pre, next_layer=self.layers[i + 1] if i + 1 < len(self.layers) else None,
+            out = layer(x, None, cache[i], tables, pre=pre, next_layer=self.layers[i + 1] if i + 1 < len(self.layers) else None,
                         draft=(lengths, at, bits))
             x, pre = out if isinstance(out, tuple) else (out, None)
         x = self.norm(x)

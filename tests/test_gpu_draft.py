@@ -85,6 +85,26 @@ def test_a_recorded_draft_follows_the_lengths(cuda):
             c[0].copy_(k), c[1].copy_(v)
 
 
+def test_the_first_draft_may_be_a_recorded_one(cuda):
+    """What a decoder keeps from its first drafted pass on holds its values when that pass was only recorded."""
+    m, other = _model(), _model()
+    prompt, tree = _ids(7, 2, 24), DraftTree([-1, 0, 0], "cuda")
+    ids, lengths = _ids(8, 2, 3), torch.tensor([24, 20], dtype=torch.int32, device="cuda")
+    want = None
+    for d in (other, m):
+        cache = d.new_cache(2, 64)
+        d(prompt, cache=cache, start=0)
+        if d is other:
+            want = d.draft(ids, cache, lengths, tree)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = m.draft(ids, cache, lengths, tree)
+    assert torch.equal(m.draft(ids, cache, lengths, tree), want)
+    g.replay()
+    assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("S", [1, 30, 100])
 def test_observed_weights(cuda, S):
     """They sum to the tokens and heads that were counted, and the logits are those of a cache without them."""
