@@ -346,7 +346,7 @@ def rope_kv(qkv, cos, sin, q_out, k_cache, v_cache, B, S, nh, nkv, cur, q_by_tok
 
 # ---- a KV cache that is drafted into and evicted from (include/flh_b200.h): sequences with lengths of their own, a tree of drafted
 # tokens behind each of them.  lengths, positions, tree, path and accepted are tensors on the device: what they hold is read when the
-# work runs, also when a recorded graph is replayed.
+# work runs, also when a recorded graph is replayed.  The caches of a call, K and V of every layer, are tensors that do not overlap.
 _TREE_MAX, _CACHE_MAX_LAYERS = 64, 128
 
 

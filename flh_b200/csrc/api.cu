@@ -298,7 +298,7 @@ int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int 
     // every count of tiles, rows and blocks stays within 31 bits
     FLH_REQUIRE(nh / nkv <= 4096 && (long)B * nkv < 1L << 26 && (long)B * nkv * (((long)S * (nh / nkv) + 15) / 16) * ((T + 31) / 32) < 1L << 31 &&
                 (long)B * nh * S < 1L << 31, FLH_B200_EINVAL, "too many sequences, heads or entries: B=%d S=%d nh=%d T=%ld", B, S, nh, T);
-    FLH_REQUIRE(scale > 0.0f && scale <= 3.0e38f, FLH_B200_EINVAL, "scale must be positive and finite");
+    FLH_REQUIRE(scale > 0.0f && scale <= 2.0e38f, FLH_B200_EINVAL, "scale must be positive, and finite in powers of two too");
     FLH_REQUIRE(q_sb % 8 == 0 && q_ss % 8 == 0 && q_sh % 8 == 0, FLH_B200_EALIGN, "strides of q must be multiples of 8 elements");
     FLH_REQUIRE(tree_stride == 0 || tree_stride == S, FLH_B200_EINVAL, "tree must be [S] or [B, S]");
     if (B == 0) return 0;

@@ -5,6 +5,7 @@
 //   * evict_move_kernel     their rows moved together in place.
 // All of them move bytes; what a pass cannot do without is each moved row read once and written once.
 #include "act_common.cuh"
+#include <algorithm>
 
 namespace flh {
 namespace {
@@ -367,7 +368,7 @@ int launch_rope_kv_at(const void *qkv, int dtype, const float *cos, const float 
     p.qkv = qkv; p.cos = cos; p.sin = sin; p.positions = positions; p.lengths = lengths;
     p.q_out = q_out; p.k_cache = k_cache; p.v_cache = v_cache;
     p.S = S; p.nh = nh; p.nkv = nkv; p.D = D; p.P = P; p.T = T;
-    const long tokens = (long)B * S, items = (long)(nh + 2 * nkv) * (D / 16), parts = (items + 255) / 256;
+    const long tokens = (long)B * S, items = (long)(nh + 2 * nkv) * (D / 16), parts = std::min((items + 255) / 256, 65535L);
     const dim3 grid((unsigned)tokens, (unsigned)(tokens >= 4L * kNumSMs ? 1 : parts));
     return cuda_status(launch_pdl(dtype == FLH_B200_BF16 ? rope_kv_at_kernel<true> : rope_kv_at_kernel<false>, grid, 256, 0, stream, p), "rope_kv_at launch");
 }

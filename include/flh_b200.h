@@ -179,8 +179,9 @@ int flh_b200_rope_kv_by_token_f16(const void *qkv, const float *cos, const float
 
 /* ---- a KV cache that is drafted into and evicted from ---------------------------------------
  *
- * Caches are [B, nkv, T, D], f16 or bf16 (dtype), contiguous; sequence b has lengths[b] committed entries (int32, 0 .. T; values
- * outside are taken as the nearer end), the same for all its heads.  S drafted tokens of a tree (1 .. FLH_B200_TREE_MAX_TOKENS) lie
+ * Caches are [B, nkv, T, D], f16 or bf16 (dtype), contiguous, each in memory of its own; sequence b has lengths[b] committed entries
+ * (int32, 0 .. T), the same for all its heads.  Of a length outside, the attention and the eviction take the nearer end; the append
+ * writes what of lengths[b] + s lies in the cache, and the acceptance moves nothing.  S drafted tokens of a tree (1 .. FLH_B200_TREE_MAX_TOKENS) lie
  * behind them, token s in entry lengths[b] + s; entries T and up do not exist.  Entries behind the last drafted one are neither
  * used nor changed, whatever they hold.  lengths, tree, positions, path and accepted are read on the device, when the work runs. */
 #define FLH_B200_TREE_MAX_TOKENS 64
@@ -220,7 +221,8 @@ int flh_b200_cache_accept(void *const *k, void *const *v, float *const *w, int l
 /* Down to `keep` entries a head: of every (layer, sequence, kv head) with more than that the last `recent` (<= keep) stay and, of the
  * others, the keep - recent with the largest weights (NaN counts as the largest; ties: the lower index).  Rows of k[l] and v[l]
  * move together in order, in place; kept (int32 [layers, B, nkv, keep]) has the entries that stay, -1 behind the last; left (f32
- * [layers, B, nkv, T]) their weights, 0 behind the last; now (int32 [B]) the new lengths.  w[l] is only read. */
+ * [layers, B, nkv, T]) their weights, 0 behind the last; now (int32 [B]) the new lengths.  w[l] is only read, and may not overlap
+ * with left. */
 int flh_b200_cache_evict(void *const *k, void *const *v, const float *const *w, int layers, int dtype, const int32_t *lengths, int keep, int recent,
                          int32_t *kept, float *left, int32_t *now, int B, int nkv, int D, long T, void *stream);
 
