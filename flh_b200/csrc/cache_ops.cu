@@ -177,7 +177,9 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t ran
 // equal digits of a warp once 28; this 25.)
 template <int THREADS, int COPIES>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
-    constexpr int kWarps = THREADS / 32;
+    constexpr int kWarps = THREADS / 32, kLanes = COPIES / 8, kDigits = 256 / kWarps;            // lanes for a digit's counts, digits of a warp
+    static_assert(64 * COPIES % THREADS == 0, "whole steps to clear the histogram");
+    static_assert(COPIES % 8 == 0 && 32 % kLanes == 0 && kDigits % (32 / kLanes) == 0, "whole steps over a warp's digits");
     extern __shared__ uint32_t keys[];
     __shared__ __align__(16) uint32_t hist[256 * COPIES]; // [digit][lane % COPIES]
     __shared__ uint32_t digits[2][256];    // of one digit and the next, in turn: the cluster may still read the last ones
@@ -223,10 +225,9 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
             }
             __syncthreads();
             // a lane has eight of a digit's counts
-            constexpr int kLanes = COPIES / 8;
 #pragma unroll
-            for (int i = 0; i < 256 / kWarps; i += 32 / kLanes) {
-                const int d = warp * (256 / kWarps) + i + lane / kLanes;
+            for (int i = 0; i < kDigits; i += 32 / kLanes) {
+                const int d = warp * kDigits + i + lane / kLanes;
                 const uint32_t *h = &hist[d * COPIES + lane % kLanes * 4];
                 const uint4 u = *reinterpret_cast<const uint4 *>(h), v = *reinterpret_cast<const uint4 *>(h + COPIES / 2);
                 uint32_t c = u.x + u.y + u.z + u.w + v.x + v.y + v.z + v.w;
