@@ -172,7 +172,8 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t ran
 // A block per row, or a cluster of blocks that have a stretch of it each.  The smallest key that is kept is found digit by digit, eight
 // bits at a time, by counting the keys that agree with the digits found so far; then the row is walked in order, every warp over a
 // part of its own, and what lies above that key is kept, of the equal ones the first few.  The keys stay in shared memory (cap: how
-// many fit; the rest is read again).  Every lane (in small blocks every fourth) counts in a histogram of its own: weights are much alike in their leading bits.  (With 8
+// many fit; the rest is read again).  Every lane counts in a histogram of its own, in rows of few keys every second or fourth one, since the histograms have to be cleared
+// and added up for each digit: weights are much alike in their leading bits.  (With 8
 // copies of the counters 256 rows of 8,192 took 31 us, finding the key two bits at a time by comparisons in registers 33, counting
 // equal digits of a warp once 28; this 25.)
 template <int THREADS, int COPIES>
@@ -393,16 +394,16 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     p.lengths = lengths; p.kept = kept; p.now = now; p.left = left;
     p.B = B; p.nkv = nkv; p.keep = keep; p.recent = recent; p.chunks = D / 8; p.T = T;
     // One block per row; a cluster of up to 8 where the rows do not fill the GPU and are long (16 rows of 24,000: 29 -> 18 us).  Short rows
-    // take blocks of 256 threads, of which more fit an SM.
+    // take blocks of 256 threads, of which more fit an SM, and rows up to 4,096 half the histograms (32 rows of 2,047: 16.6 -> 15.8 us).
     const long rows = (long)B * nkv * layers;
     int blocks = 1;
     while (blocks < kMaxCluster && rows * blocks * 2 <= kNumSMs && T >= 4096L * blocks) blocks *= 2;
-    const bool few = T <= 2048;
+    const bool few = T <= 2048, medium = T <= 4096;
     const long each = (T + blocks - 1) / blocks + 2048;                  // a block's stretch, rounded up to whole spans
     const int cap = (int)(each < kSelKeys ? each : kSelKeys);
-    auto select = few ? evict_select_kernel<256, 8> : evict_select_kernel<512, 32>;
-    static std::atomic<uint64_t> done[2];
-    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(select), kSelKeys * 4, done[few]);
+    auto select = few ? evict_select_kernel<256, 8> : medium ? evict_select_kernel<512, 16> : evict_select_kernel<512, 32>;
+    static std::atomic<uint64_t> done[3];
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(select), kSelKeys * 4, done[few ? 0 : medium ? 1 : 2]);
     if (e != cudaSuccess) return cuda_status(e, "cache_evict shared memory");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];

@@ -377,6 +377,14 @@ def test_cache_evict_ties_and_odd_weights(cuda, kind, keep, recent):
     _check_evict(cuda, k, v, w, [1200, 1001], keep, recent)
 
 
+@pytest.mark.parametrize("B,T", [(1, 3000), (80, 4500), (2, 40000)])
+def test_cache_evict_ties_in_longer_rows(cuda, B, T):
+    """Three values in all weights, in every form of the selection: rows of a few thousand entries, longer ones, those of several blocks."""
+    k, v, w = _layers(6, 1, B, 1, T, 8, torch.float16)
+    w.copy_((w * 3).floor() / 4)
+    _check_evict(cuda, k, v, w, [T - b % 7 for b in range(B)], T // 3, 50)
+
+
 def test_cache_evict_of_sequences_that_fit(cuda):
     k, v, w = _layers(6, 2, 4, 1, 50, 128, torch.bfloat16)
     _check_evict(cuda, k, v, w, [0, 1, 50, -3], 50, 10)
