@@ -15,8 +15,9 @@
 // the reads of K and V); with up to 128 they are the same rows over every other tile, and their results become one at the end of a
 // piece, straight from tensor memory.
 //
-// The running maximum that the exponentials are relative to follows the true one only when that is 2^8 ahead: O is then read, scaled
-// and written back.  P reaches 2^8 at most, far from the end of float16.
+// The reference m that the exponentials are relative to follows the true maximum only when that is 2^8 ahead: O is then read, scaled and
+// written back.  In float16, which ends at 2^-24 and at 2^16, m is 2^7 below the maximum that it was taken from: P reaches 2^15 at most, and
+// what is 2^-26 of the heaviest keeps five bits and more of itself (relative to the maximum it vanished from O, not from the sum).
 #include "attn_common.cuh"
 #include "tc_pair.cuh"
 #include "tc_quant_common.cuh"
@@ -31,7 +32,8 @@ constexpr int kThreadsTcA = 384;           // warp 0 TMA, warps 1 and 2 MMA, war
 // registers: 384 threads are launched with 168; 128 * 112 + 256 * 192 are less than those 64,512
 constexpr int kRegsIssue = 112, kRegsSoftmax = 192;
 static_assert(128 * kRegsIssue + 256 * kRegsSoftmax <= kThreadsTcA * 168, "more registers than the CTA was launched with");
-constexpr float kLag = 8.0f;               // powers of two that the true maximum may be ahead
+constexpr float kLag = 8.0f;               // powers of two that the true maximum may be ahead of the one that m was taken from
+template <bool BF16> constexpr float kRaise = BF16 ? 0.0f : 7.0f;                      // and that m lies below that one
 
 template <int D> constexpr int item_bytes() { return kTileTc * D * 2; }                         // K or V of a tile
 template <int D> constexpr int q_bytes() { return kRowsTc * D * 2; }                            // a block of rows of Q
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2 - kRaise<BF16>;
                     if (i == 0) m = mx;
                     else if (__any_sync(0xffffffffu, (mx > m + kLag || m == -INFINITY) && mx != m)) {
                         // the product before this one has to be done (the one before that is: these scores were made behind it)

@@ -94,6 +94,28 @@ def test_scores_that_single_entries_out(cuda, S, dtype):
     _check_attention(cuda, q, k, v, _ints([800, 333]), None, scale=0.5)
 
 
+@pytest.mark.parametrize("S,g,nkv", [(2, 4, 296), (8, 4, 148), (64, 3, 148)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_light_entries_beside_heavy_ones(cuda, S, g, nkv, dtype):
+    """Four entries with value 0 whose weights are e^18 = 2^26 times those of all the others, which have value 1: together these give the
+    result, and each by itself is below float16's smallest number where the heaviest weight is 1."""
+    n, D = 16384, 64
+    k, v = torch.zeros(1, nkv, n + S, D, device="cuda", dtype=dtype), torch.ones(1, nkv, n + S, D, device="cuda", dtype=dtype)
+    k[:, :, 0:128:32, 0], v[:, :, 0:128:32] = 18.0, 0.0                       # in a tile of every warp, and of both streams of many rows
+    q = torch.zeros(1, S, nkv * g, D, device="cuda", dtype=dtype)
+    q[..., 0] = 1.0
+    out = cuda.tree_attention(q, k, v, _ints([n]), scale=1.0).double()
+    light = (n - 4 + torch.arange(1, S + 1, device="cuda")).double() * np.exp(-18.0)
+    want = (light / (4 + light))[None, :, None, None].expand(out.shape)
+    # a weight and the result are off by half a step each, the exponentials by less than 2^-18 (a score of 18 of exact products, its scaling
+    # and the power of two: 26 * 2^-23 + 2^-21); a weight under 2^-14 absolutely by half of float16's smallest number: 2^-25 relative to a
+    # heaviest weight that is raised to 2^7 at least, 2^-32; a result under 2^-14 by 2^-25.  Sums of up to 16,384 weights in binary32: 2^-10
+    # at most if one after the other, and equal ones are summed in tiles
+    u = R.HALF_STEP[dtype]
+    tol = want * (2.02 * u + 2.0 ** -17 + 2.0 ** -10) + (light[None, :, None, None].expand(out.shape) * np.exp(18.0) * 2.0 ** -32 / 4 + 2.0 ** -25 if dtype == torch.float16 else 0.0)
+    R.assert_close(out, want, tol)
+
+
 @pytest.mark.parametrize("S,nh,nkv,D", [(4, 2, 1, 64), (9, 8, 4, 128), (64, 4, 1, 128), (64, 8, 1, 64)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_tokens_that_see_nothing(cuda, S, nh, nkv, D, dtype):
