@@ -7,7 +7,10 @@
 //   kEven   all tiles of all jobs in a row (sequence, then head, then block of rows) are cut into equal shares, wherever the cuts fall:
 //           a batch of uneven lengths is as balanced as one long sequence.  For more jobs than CTAs, or many sequences.
 //   kParts  every job is cut into parts of nearly the same size, as many as its length is worth, a CTA for each: no CTA has
-//           parts of two jobs, whose second one costs it what several tiles do (q, the ramp of the rings, the result).
+//           parts of two jobs, whose second one costs it what several tiles do (q, the ramp of the rings, the result).  Where that
+//           makes the fullest CTA work longer than equal shares and a second part would (one long sequence among many short ones,
+//           each of which takes a CTA a head), the CTAs take equal shares instead: 60,000 entries beside 31 sequences of 500, 8 rows,
+//           8 heads: 429 us in parts, 44 in equal shares.
 //   kJobs   each CTA has as many whole jobs as the next; nothing is cut.
 // A job that lies within one CTA is finished there; of a job that was cut each CTA writes a partial result (sum of exponentials,
 // maximum, weighted sum of V) to a slot of its own and the join kernel adds them in order.
@@ -18,6 +21,9 @@ namespace flh {
 
 enum { kEven, kParts, kJobs };
 constexpr int kTreeTcTile = 64;            // entries of a key tile of attn_tc_kernel
+constexpr int kBehind = 1 << 30;           // the first CTA of a job began with another one
+// What a second job costs a CTA, in tiles of 32 (attn_mma_kernel), 64 (attn_tc_kernel) and 128 entries (attn_weights_tc_kernel).
+template <int TILE> constexpr int kSecondJob = TILE == 32 ? 24 : TILE == 64 ? 12 : 2;
 
 struct TreeAttnParams {
     const void *q;
@@ -36,7 +42,7 @@ struct TreeAttnParams {
     int split, jobs_each;                  // kEven, kParts, kJobs; jobs of a CTA (kJobs)
     float *part_o;                         // [2 shares][D / 4][rows of a block][4]: 32 rows of a thread each write whole lines
     float2 *part_ml;                       // [2 shares][rows of a block]: maximum, sum
-    int2 *parts_of;                        // [jobs] (kParts): first CTA and number of parts, for the join
+    int2 *parts_of;                        // [jobs] (kParts), or null: first CTA (and kBehind), number of parts, for the join
     float *lse;                            // [B, nkv, R]: log2 of the sum of powers (with weights), or null
     float *scores;                         // [B, nkv, R, score_ld] (with weights and few rows), or null
     long score_ld;
@@ -137,17 +143,17 @@ struct JobWalk {
 template <int TILE>
 struct Parts {
     int nt, parts, size, first;            // tiles of a job, its parts, tiles of a part (the last may have fewer), first CTA of the sequence
-    __device__ __forceinline__ void find(const TreeAttnParams &p, int lane) {
+    int total;                             // tiles of all jobs
+    // false: no size that is at most kSecondJob tiles over an even share has CTAs enough
+    __device__ __forceinline__ bool find(const TreeAttnParams &p, int lane) {
+        static_assert(kSecondJob<TILE> < 32, "a lane for every size");
         const int per = p.nkv * p.nrb;
         nt = lane < p.B ? (entries(p, committed(p, lane)) + TILE - 1) / TILE : 0;
-        int total = nt, longest = nt;
-        for (int o = 16; o; o >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, o);
-            longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
-        }
-        // the smallest size for which there are CTAs enough, of 32 between an even share and the longest job (which always is)
-        const int even = max((total * per + p.shares - 1) / p.shares, p.min_share);
-        const int tried = lane == 31 ? max(longest, 1) : even + even * lane / 16;
+        total = nt;
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        total *= per;
+        // a lane tries a size: the smallest for which there are CTAs enough
+        const int tried = share_tiles(p, total) + lane;
         // ceil(nt / tried) as a truncated product: a little less than the quotient, by more than its rounding (2^-22) and less than the
         // distance to the next whole number (1 / tried, nt < 2^17), and one more
         const float inverse = (1.0f - 0x1p-19f) / (float)tried;
@@ -157,7 +163,8 @@ struct Parts {
             const int other = __shfl_sync(0xffffffffu, nt, i);
             count += (int)((float)other * inverse) + (other > 0);
         }
-        const unsigned fits = __ballot_sync(0xffffffffu, (long)count * per <= p.shares);
+        const unsigned fits = __ballot_sync(0xffffffffu, lane <= kSecondJob<TILE> && (long)count * per <= p.shares);
+        if (!fits) return false;
         size = __shfl_sync(0xffffffffu, tried, __ffs(fits) - 1);
         parts = (nt + size - 1) / size;
         size = nt ? (nt + parts - 1) / parts : 1;
@@ -165,6 +172,7 @@ struct Parts {
         int incl = parts * per;
         for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += t; }
         first = incl - parts * per;
+        return true;
     }
 };
 
@@ -182,29 +190,44 @@ __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, Jo
         for (int i = 1; i < count; ++i) last.next(p);
         u0 = 0;
         u1 = last.begin + last.nt;
-    } else if (p.split == kParts) {
+        return;
+    }
+    int total;
+    if (p.split == kParts) {
         Parts<TILE> c;
-        c.find(p, lane);
-        const int per = p.nkv * p.nrb, cta = blockIdx.x;
-        const unsigned at = __ballot_sync(0xffffffffu, lane < p.B && cta < c.first + c.parts * per);
-        u0 = u1 = 0;
-        if (!at) return;
-        const int b = __ffs(at) - 1;
-        const int first = uniform(__shfl_sync(0xffffffffu, c.first, b)), parts = uniform(__shfl_sync(0xffffffffu, c.parts, b)), size = uniform(__shfl_sync(0xffffffffu, c.size, b));
-        job.b = b;
-        job.job = (cta - first) / parts;
-        job.len = uniform(committed(p, b));
-        job.nt = (entries(p, job.len) + TILE - 1) / TILE;
-        job.begin = 0;                     // its own count of tiles
-        u0 = (cta - first - job.job * parts) * size;
-        u1 = min(u0 + size, job.nt);
-        if (u0 == 0 && threadIdx.x == 0) p.parts_of[b * per + job.job] = make_int2(cta, parts);
+        if (c.find(p, lane)) {
+            const int per = p.nkv * p.nrb, cta = blockIdx.x;
+            const unsigned at = __ballot_sync(0xffffffffu, lane < p.B && cta < c.first + c.parts * per);
+            u0 = u1 = 0;
+            if (!at) return;
+            const int b = __ffs(at) - 1;
+            const int first = uniform(__shfl_sync(0xffffffffu, c.first, b)), parts = uniform(__shfl_sync(0xffffffffu, c.parts, b)), size = uniform(__shfl_sync(0xffffffffu, c.size, b));
+            job.b = b;
+            job.job = (cta - first) / parts;
+            job.len = uniform(committed(p, b));
+            job.nt = (entries(p, job.len) + TILE - 1) / TILE;
+            job.begin = 0;                 // its own count of tiles
+            u0 = (cta - first - job.job * parts) * size;
+            u1 = min(u0 + size, job.nt);
+            if (u0 == 0 && threadIdx.x == 0 && p.parts_of) p.parts_of[b * per + job.job] = make_int2(cta, parts);
+            return;
+        }
+        total = uniform(c.total);
     } else {
-        const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);
-        const long first = (long)blockIdx.x * share;
-        u0 = (int)min(first, (long)total);
-        u1 = (int)min((long)total, first + share);
-        if (u0 < u1) job.seek(p, u0, lane);
+        total = tiles_before<TILE>(p, p.B, lane);
+    }
+    const int share = share_tiles(p, total);
+    const long first = (long)blockIdx.x * share;
+    u0 = (int)min(first, (long)total);
+    u1 = (int)min((long)total, first + share);
+    if (u0 >= u1) return;
+    job.seek(p, u0, lane);
+    if (p.split == kParts && p.parts_of && threadIdx.x < 32) {                   // the jobs that begin here
+        JobWalk<TILE> at = job;
+        if (at.begin < u0) at.next(p);
+        for (; at.begin < u1 && at.b < p.B; at.next(p))
+            if (threadIdx.x == 0)
+                p.parts_of[at.b * p.nkv * p.nrb + at.job] = make_int2(blockIdx.x | (at.begin != u0 ? kBehind : 0), (at.begin + at.nt - 1) / share - (int)blockIdx.x + 1);
     }
 }
 

@@ -401,8 +401,9 @@ __device__ __forceinline__ bool find_parts(const TreeAttnParams &p, int lane, in
         const int2 t = p.parts_of[blockIdx.x];
         b = blockIdx.x / per;
         job_of = blockIdx.x - b * per;
-        c0 = t.x;
+        c0 = t.x & ~kBehind;
         parts = t.y;
+        behind = (t.x & kBehind) != 0;
         return parts > 1;
     }
     const int total = tiles_before<TILE>(p, p.B, lane), share = share_tiles(p, total);

@@ -558,3 +558,50 @@ def test_every_division_of_the_work(cuda, B, S, nh, nkv):
         R.assert_close(w[some][:, :, :top + S], ww, wtol + 2.0 ** -24 * ww)
         assert torch.allclose(w.sum(-1), torch.full((B, nkv), float(S * nh // nkv), device="cuda"), rtol=1e-4)
     assert cuda.tree_attention_status()[0] == 0
+
+
+def _graph_time(f):
+    """Device time of a call, replayed in a graph: the best of several."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        f()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        f()
+    best = float("inf")
+    for _ in range(12):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        g.replay()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("S,nh,nkv,long,short,others,observe", [
+    (5, 64, 8, 60000, 1000, 15, False), (1, 64, 8, 60000, 500, 31, False), (1, 64, 8, 60000, 500, 31, True), (1, 64, 8, 40000, 2000, 20, False), (64, 32, 8, 30000, 300, 4, False),
+])
+def test_one_long_sequence_among_short_ones(cuda, S, nh, nkv, long, short, others, observe):
+    """The work goes by what the sequences hold: one long one costs about what the same entries cost in sequences that are alike."""
+    B, T, D = 1 + others, long + S, 64
+    lengths, total = [short] * others, long + others * short
+    lengths.insert(others // 3, long)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = _normal(4, B, S, nh, D)
+    k, v = (torch.randn(B, nkv, T, D, dtype=torch.float16, device="cuda", generator=g) for _ in range(2))
+    w = torch.zeros(B, nkv, T, device="cuda") if observe else None
+    n, even = _ints(lengths), _ints([total // B] * B)
+    out = cuda.tree_attention(q, k, v, n, weights=w)
+    for b in (0, others // 3, B - 1):
+        want, tol, ww, wtol = R.attention(q[b:b + 1], k[b:b + 1, :, :lengths[b] + S], v[b:b + 1, :, :lengths[b] + S], lengths[b:b + 1])
+        R.assert_close(out[b:b + 1], want, tol)
+        if observe:
+            R.assert_close(w[b:b + 1, :, :lengths[b] + S], ww, wtol + 2.0 ** -24 * ww)
+            assert not w[b, :, lengths[b] + S:].any()
+    uneven, even = (_graph_time(lambda: cuda.tree_attention(q, k, v, x, weights=w)) for x in (n, even))
+    print(f"\nuneven {uneven:.1f} us, even {even:.1f} us")
+    assert uneven < 2.5 * even, (uneven, even)
+    assert cuda.tree_attention_status()[0] == 0
