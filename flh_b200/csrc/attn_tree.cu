@@ -570,11 +570,16 @@ Plan plan_of(int B, int S, int nh, int nkv, int D, long T, bool weights) {
     pl.nrb = (R + pl.rows - 1) / pl.rows;
     pl.shares = pl.rows >= 128 ? kNumSMs : 2 * kNumSMs;
     pl.min_share = pl.rows >= 128 ? 2 : kWarps;
-    // Whole jobs where what that makes the fullest CTA work more than an even share is little: what is saved is the join and, for most
-    // CTAs, a second piece.  In tiles: 24 of 32 entries (one sequence of 500 entries, 32 heads: 13.7 -> 10.1 us; 24 sequences of 40: 31 -> 20 us),
-    // 12 of 64 entries on the tensor cores.  Else parts of the jobs, where that is worked out quickly.
-    const long jobs = (long)B * nkv * pl.nrb, tile = pl.rows >= 128 ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile, each = (jobs + pl.shares - 1) / pl.shares;
-    pl.split = each * nt - jobs * nt / pl.shares <= (pl.rows >= 128 ? 12 : 24) ? kJobs : jobs <= pl.shares && B <= 32 ? kParts : kEven;
+    // Whole jobs where what that makes the fullest CTA work more than an even share is little, if the sequences are about as long as one another:
+    // what is saved is the join and, for most CTAs, a second piece (kSecondJob tiles; one sequence of 500 entries, 32 heads: 13.7 -> 10.1
+    // us; 24 sequences of 40: 31 -> 20; 4 of 2,478 .. 4,000, 32 heads of 64 rows: 57 -> 50).  The lengths are not known here: a CTA has at most
+    // `most` tiles whatever they are, so that one long sequence among short ones costs little even then (8 rows, 16 sequences: 1,531 entries
+    // and 15 of 20 33 us, 30 if cut; 40 rows, 18 sequences: 2,000 and 17 of 100 27 us, 18 if cut).  Else parts of the jobs, where that is
+    // worked out quickly.
+    const bool tc = pl.rows >= 128;
+    const long jobs = (long)B * nkv * pl.nrb, tile = tc ? kTreeTcTile : kTile, nt = (T + tile - 1) / tile, each = (jobs + pl.shares - 1) / pl.shares;
+    const long over = each * nt - jobs * nt / pl.shares, most = tc ? 72 : 128;
+    pl.split = over <= (tc ? kSecondJob<kTreeTcTile> : kSecondJob<kTile>) && each * nt <= most ? kJobs : jobs <= pl.shares && B <= 32 ? kParts : kEven;
     pl.jobs_each = (int)each;
     if (pl.split == kJobs) pl.shares = (int)((jobs + each - 1) / each);
     pl.scores = weights && R <= 16;
