@@ -459,8 +459,8 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
 
 // weights += sum over the rows of 2^(score - lse) for more rows than leave their scores (attn_tree.cu), from K and q again: S^T = K Q^T, an
 // entry per lane of tensor memory and a row per column, so that a thread adds up its entry's weights with nothing to exchange.  A
-// CTA (two an SM) has some of a head's tiles of 128 entries, 128 rows at a time; K is loaded, multiplied and added up in a pipeline of
-// two tiles.  What bounds it is one exponential for each score, 16 a clock and SM, or K; as mma.sync, where every warp reads all
+// CTA (two an SM) has some of the heads' tiles of 128 entries, divided by the lengths as those of the attention are, 128 rows at a time; K is
+// loaded, multiplied and added up in a pipeline of two tiles.  What bounds it is one exponential for each score, 16 a clock and SM, or K; as mma.sync, where every warp reads all
 // rows for its 16 entries, 64 rows x 254,000 entries took 28 us (17 so, of which K's 65 MB are 10).
 constexpr int kWeightTile = 128, kThreadsWeights = 256, kWeightGroup = 8;
 template <int D> constexpr int smem_weights() { return 1024 + (2 * kWeightTile + kRowsTc) * D * 2; }
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
     __shared__ float so_far[kWeightGroup][kWeightTile];                          // an entry's sum over the rows before, its thread's own
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
-    const int bh = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); mbar_init(smem_u32(&s_full[i]), 1); mbar_init(smem_u32(&s_free[i]), 4); }
         abort_flag = 0;
@@ -490,17 +490,24 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
+    // the lengths may be read here: the kernel before this one is the attention or the join of the same call, which lets this one start when
+    // it has itself waited for all that came before the call
+    JobWalk<kWeightTile> job;
+    int u0, u1;
+    take_share(p, lane, job, u0, u1);
     pdl_wait();
     pdl_trigger();
-    const int b = bh / p.nkv, kvh = bh - b * p.nkv, len = committed(p, b), n = entries(p, len);
-    const int tiles = (n + kWeightTile - 1) / kWeightTile, each = (tiles + gridDim.y - 1) / gridDim.y, first = min((int)blockIdx.y * each, tiles), last = min(first + each, tiles);
     bool ok = true;
     auto wait = [&](uint64_t *bar, uint32_t phase, int code) {
         if (ok) ok = mbar_wait_warp(g_status_attn_tc, smem_u32(bar), phase & 1, &abort_flag, code);
     };
     uint32_t it = 0;                                                             // tiles so far, of all rows
     // with more rows than 128 a few tiles at a time, so that an entry's sum over all of them is added to its weight once
-    const int group = p.R > kRowsTc ? kWeightGroup : tiles;
+    const int group = p.R > kRowsTc ? kWeightGroup : 1 << 20;
+    for (int piece = u0, piece_end; piece < u1; piece = piece_end) {
+    while (piece >= job.begin + job.nt) job.next(p);
+    piece_end = min(u1, job.begin + job.nt);
+    const int b = job.b, kvh = job.job, bh = b * p.nkv + kvh, len = job.len, n = entries(p, len), first = piece - job.begin, last = piece_end - job.begin;
     for (int g0 = first; g0 < last; g0 += group)
     for (int row0 = 0; row0 < p.R; row0 += kRowsTc) {
         const int g1 = min(g0 + group, last);
@@ -604,6 +611,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
             }
         }
     }
+    }
     __syncwarp();
     if (warp == 0)                                                               // as in attn_tc_kernel: nothing is on its way when the CTA leaves
         for (uint32_t i = it > 2 ? it - 2 : 0; i < it && abort_flag; ++i)
@@ -623,9 +631,19 @@ int launch_weights(const TreeAttnParams &p, const CUtensorMap &km, cudaStream_t 
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, done);
     if (e != cudaSuccess) return cuda_status(e, "tree_attention shared memory");
-    // two CTAs for every SM, but none without a tile
-    const long heads = (long)p.B * p.nkv, tiles = (p.T + kWeightTile - 1) / kWeightTile, want = heads >= 2L * kNumSMs ? 1 : 2L * kNumSMs / heads;
-    return cuda_status(launch_pdl(kern, dim3((unsigned)heads, (unsigned)(want < tiles ? want : tiles)), kThreadsWeights, smem, stream, p, km), "tree_attention weights");
+    // Two CTAs for every SM, but none without a tile; a job is a head here.  Whole heads, as plan_of has whole jobs, where a CTA has few
+    // tiles whatever the lengths are (37 sequences of 511 .. 1,000, 8 heads of 40 rows: 51 us with the attention, 57 in equal shares).
+    const long heads = (long)p.B * p.nkv, nt = (p.T + kWeightTile - 1) / kWeightTile;
+    TreeAttnParams q = p;
+    q.nrb = 1;
+    q.shares = heads * nt < 2L * kNumSMs ? (int)(heads * nt) : 2 * kNumSMs;
+    q.min_share = 1;
+    const long each = (heads + q.shares - 1) / q.shares;
+    q.split = each * nt - heads * nt / q.shares <= kSecondJob<kWeightTile> && each * nt <= 20 ? kJobs : heads <= q.shares && p.B <= 32 ? kParts : kEven;
+    q.jobs_each = (int)each;
+    if (q.split == kJobs) q.shares = (int)((heads + each - 1) / each);
+    q.parts_of = nullptr;
+    return cuda_status(launch_pdl(kern, dim3((unsigned)q.shares), kThreadsWeights, smem, stream, q, km), "tree_attention weights");
 }
 
 template <int D, bool TWO, bool BF16>

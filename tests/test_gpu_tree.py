@@ -583,6 +583,7 @@ def _graph_time(f):
 
 @pytest.mark.parametrize("S,nh,nkv,long,short,others,observe", [
     (5, 64, 8, 60000, 1000, 15, False), (1, 64, 8, 60000, 500, 31, False), (1, 64, 8, 60000, 500, 31, True), (1, 64, 8, 40000, 2000, 20, False), (64, 32, 8, 30000, 300, 4, False),
+    (5, 64, 8, 60000, 1000, 15, True), (5, 64, 8, 16000, 500, 73, True), (64, 32, 8, 30000, 300, 4, True),
     (1, 64, 8, 60000, 500, 36, False), (1, 32, 32, 28000, 500, 8, False), (5, 64, 8, 16000, 500, 17, False), (5, 64, 8, 16000, 500, 73, False), (1, 64, 8, 60000, 500, 36, True),
 ])
 def test_one_long_sequence_among_short_ones(cuda, S, nh, nkv, long, short, others, observe):
