@@ -331,21 +331,23 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 }
                 if (tail) {
                     // values of V that are not finite become zero, of drafted entries and of what lies behind the sequence's end: half a row
-                    // a thread.  (Both streams do it where they share a tile; an entry is marked before it is changed.)
-                    const int item = 2 * (piece - u0 + t) + 1, slot = item % kItems, vr = wg >> 1, at = key0 + vr;
+                    // a thread, or a quarter where both streams are at this tile.  Then they share the work and wait for one another: each
+                    // thread makes its own writes known to the async proxy, and no product begins before all have.
+                    const bool both = TWO && row0 + kRowsTc < p.R;
+                    const int item = 2 * (piece - u0 + t) + 1, slot = item % kItems, of = both ? 4 : 2, mate = both ? wg + x * 128 : wg, vr = mate / of, at = key0 + vr;
+                    const int first_ch = (mate % of) * (D / 8 / of), chunks = D / 8 / of;
                     if (wait(fulls + 8 * slot, item / kItems, 47) && at >= len) {
                         uint8_t *v = smem + slot * kItem + vr * 128;
                         uint32_t odd = 0;                                        // pieces with such a value, a bit each
 #pragma unroll
                         for (int j = 0; j < D / 16; ++j) {
-                            const int ch = (wg & 1) * (D / 16) + j;
-                            odd |= (uint32_t)any_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4))) << j;
+                            const int ch = first_ch + j;
+                            if (j < chunks) odd |= (uint32_t)any_nonfinite<BF16>(*reinterpret_cast<const uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4))) << j;
                         }
                         if (odd) {
                             if (at < n) atomicOr(&bad[which], 1ull << (at - len));
-                            __threadfence_block();
-                            for (int j = 0; j < D / 16; ++j) {
-                                const int ch = (wg & 1) * (D / 16) + j;
+                            for (int j = 0; j < chunks; ++j) {
+                                const int ch = first_ch + j;
                                 uint4 *q = reinterpret_cast<uint4 *>(v + (ch >> 3) * kHalf + (((ch & 7) ^ (vr & 7)) << 4));
                                 const uint4 w = *q;
                                 *q = make_uint4(finite2<BF16>(w.x), finite2<BF16>(w.y), finite2<BF16>(w.z), finite2<BF16>(w.w));
@@ -353,6 +355,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                             fence_proxy_async();
                         }
                     }
+                    if (both) bar_sync_named(1, 256);                            // (reached by both for every such tile, also after a wait that ran out)
                 }
                 tc_fence_before();
                 bar_arrive_named(3 + 2 * x + (count & 1), 160);

@@ -607,3 +607,29 @@ def test_one_long_sequence_among_short_ones(cuda, S, nh, nkv, long, short, other
     print(f"\nuneven {uneven:.1f} us, even {even:.1f} us")
     assert uneven < 2.5 * even, (uneven, even)
     assert cuda.tree_attention_status()[0] == 0
+
+
+@pytest.mark.parametrize("g,D", [(8, 128), (4, 128), (3, 64), (8, 64)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_odd_values_where_two_blocks_of_rows_share_a_tile(cuda, g, D, dtype):
+    """Stale and drafted values that are not finite, in tiles that two streams of rows read: as without them for the rows that do not see them,
+    the same every time."""
+    S, B, T = 64, 40, 400
+    r = rs(g + D)
+    lengths = [int(x) for x in r.randint(0, T - S, size=B)]
+    q, k, v = _normal(1, B, S, 2 * g, D, dtype=dtype), _normal(2, B, 2, T, D, dtype=dtype), _normal(3, B, 2, T, D, dtype=dtype)
+    tree = torch.stack([R.random_tree(r, S)[0] for _ in lengths]).cuda()
+    tree[:, S - 1] = 1 | -(1 << 63)                                            # only the last token sees the last one
+    clean = v.clone()
+    for b, n in enumerate(lengths):
+        clean[b, :, n + S:] = 0
+        v[b, :, n + S:] = float("nan")
+        v[b, :, n + S - 1, b % 8::8] = float("inf")
+    want = cuda.tree_attention(q, k, clean, _ints(lengths), tree=tree)
+    for _ in range(20):
+        got = cuda.tree_attention(q, k, v, _ints(lengths), tree=tree)
+        assert torch.equal(got[:, :S - 1], want[:, :S - 1])
+        for b in (0, 1, 17, B - 1):
+            odd = torch.arange(D, device="cuda") % 8 == b % 8
+            assert torch.equal(got[b, S - 1][:, ~odd], want[b, S - 1][:, ~odd]) and bool((got[b, S - 1][:, odd] == float("inf")).all())
+    assert cuda.tree_attention_status()[0] == 0
