@@ -37,8 +37,6 @@ class DecoderConfig:
     n_layers: int = 32
     vocab: int = 32000
     rope_theta: float = 10000.0
-    max_positions: int = 32768           # rows of the rotary tables that Decoder.draft reads (built at its first call): tokens behind
-                                         # them come out as NaN
     eps: float = 1e-5
     act_mode: str = "group_sym"          # or "token_asym"
     tp: int = 1
@@ -51,6 +49,8 @@ class DecoderConfig:
     seq_parallel: bool = True            # tensor-parallel prefill with the residual stream sharded by tokens: row-parallel
                                          # outputs are reduce-scattered, norm + quantiser run on T / tp rows, and the all-gather
                                          # carries int4 codes (a quarter of the f16 bytes)
+    max_positions: int = 32768           # rows of the rotary tables that Decoder.draft reads (built at its first call): tokens behind
+                                         # them come out as NaN
 
     @property
     def head_dim(self):

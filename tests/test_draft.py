@@ -37,3 +37,9 @@ def test_accept_greedy():
     one = DraftTree([-1])
     path, accepted, chosen = one.accept_greedy(torch.zeros(2, 1, dtype=torch.int64), logits[:2, :1])
     assert path.tolist() == [[0], [0]] and accepted.tolist() == [1, 1] and chosen.tolist() == [3, 5]
+
+
+def test_the_configuration_takes_its_fields_in_the_order_they_had():
+    from flh_b200.model import DecoderConfig
+    c = DecoderConfig(4096, 32, 8, 14336, 4, 32000, 500000.0, 1e-6, "token_asym", 2)
+    assert (c.rope_theta, c.eps, c.act_mode, c.tp) == (500000.0, 1e-6, "token_asym", 2) and c.max_positions == 32768
