@@ -24,6 +24,7 @@ import torch.distributed as dist
 import torch.nn.functional as F
 
 from . import _CUDA, timing
+from .draft import MAX_TOKENS
 from .nn import ActQuantizer, LinearFLH
 from .tp import ColumnParallelLinearFLH, RowParallelLinearFLH, gather_quantised, gather_rows, local_rows
 
@@ -309,11 +310,18 @@ class Decoder(torch.nn.Module):
         """A list of [k, v, cursor] per layer.  observe: [k, v, cursor, weights], where every call adds to weights (f32 [B, kv heads,
         max_len]) the attention that its last 64 tokens gave each entry, which evict() goes by."""
         c = self.cfg
+        if observe:
+            self._check_attention(max_len)
         nkv = max(c.n_kv_heads // c.tp, 1)
         return [[torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device),
                  torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device), 0]
                 + ([torch.zeros(batch, nkv, max_len, dtype=torch.float32, device=self.device)] if observe else [])
                 for _ in range(c.n_layers)]
+
+    def _check_attention(self, max_len):
+        """What _CUDA.tree_attention takes of a decoder and its cache."""
+        if self.cfg.head_dim not in (64, 128) or max_len > 1 << 21:
+            raise RuntimeError("drafted tokens and observed caches need heads of 64 or 128 values and caches of at most 2^21 entries")
 
     def _draft_tables(self):
         """The rotary tables over all positions, kept from the first call on for every stream: so they are waited for once.  Those that
@@ -335,6 +343,10 @@ class Decoder(torch.nn.Module):
         a head).  lengths and positions are read on the device: a recorded step follows them.  What is kept of the tokens is
         what accept() is told."""
         B, S = ids.shape
+        # before anything is written: the attention, which comes after the first layer's append, would refuse these
+        if not 1 <= S <= MAX_TOKENS or (tree is not None and tree.depth.shape[-1] != S):
+            raise RuntimeError(f"draft takes 1 .. {MAX_TOKENS} tokens of a sequence, as many as its tree has")
+        self._check_attention(cache[0][0].shape[2])
         tables = self._draft_tables()
         at = lengths if positions is None else positions
         at = at[:, None] + (torch.arange(S, dtype=torch.int32, device=self.device) if tree is None else tree.depth)

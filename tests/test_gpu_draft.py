@@ -176,3 +176,18 @@ def test_speculative_run_equals_one_token_at_a_time(cuda):
         lengths = m.accept(cache, lengths, path, accepted, tree.size)
         step += 1
         assert got == [w[0] for w in want[:len(got)]]
+
+
+def test_what_draft_refuses_leaves_the_cache_as_it_was(cuda):
+    m = _model()
+    cache, lengths = m.new_cache(2, 100), torch.tensor([3, 0], dtype=torch.int32, device="cuda")
+    for ids, tree in ((_ids(1, 2, 65), None), (_ids(1, 2, 0), None), (_ids(1, 2, 4), DraftTree([-1, 0, 0], "cuda"))):
+        with pytest.raises(RuntimeError, match="1 .. 64 tokens"):
+            m.draft(ids, cache, lengths, tree)
+    small = _model(hidden=256, n_heads=8, n_kv_heads=8)                        # heads of 32
+    other = small.new_cache(2, 100)
+    with pytest.raises(RuntimeError, match="64 or 128"):
+        small.draft(_ids(1, 2, 4), other, lengths)
+    with pytest.raises(RuntimeError, match="64 or 128"):
+        small.new_cache(2, 100, observe=True)
+    assert not any(bool(c[i].any()) for c in (*cache, *other) for i in (0, 1))
