@@ -50,8 +50,8 @@ class DecoderConfig:
     seq_parallel: bool = True            # tensor-parallel prefill with the residual stream sharded by tokens: row-parallel
                                          # outputs are reduce-scattered, norm + quantiser run on T / tp rows, and the all-gather
                                          # carries int4 codes (a quarter of the f16 bytes)
-    max_positions: int = 32768           # rows of the rotary tables that Decoder.draft reads (built at its first call): tokens behind
-                                         # them come out as NaN
+    max_positions: int = 32768           # rows of the rotary tables that Decoder.draft reads (at least those of its cache; built at its
+                                         # first call): tokens behind them, after evictions, come out as NaN
 
     @property
     def head_dim(self):
@@ -294,7 +294,7 @@ class Decoder(torch.nn.Module):
         self.embed.weight.data.copy_(torch.randn(cfg.vocab, cfg.hidden, device=device, generator=rep).half())
         self.layers = torch.nn.ModuleList(DecoderLayer(cfg, device, gen, group) for _ in range(cfg.n_layers))
         self.norm = RMSNorm(cfg.hidden, cfg.eps).to(device)
-        self._tables = None                              # rotary tables of draft()
+        self._tables = {}                                # rotary tables of draft(), by their rows
         self.head = torch.nn.Linear(cfg.hidden, cfg.vocab, bias=False, device=device, dtype=torch.float16) if with_head else None
         if self.head is not None:
             self.head.weight.data.copy_((torch.randn(cfg.vocab, cfg.hidden, device=device, generator=rep) * cfg.hidden ** -0.5).half())
@@ -323,15 +323,17 @@ class Decoder(torch.nn.Module):
         if self.cfg.head_dim not in (64, 128) or max_len > 1 << 21:
             raise RuntimeError("drafted tokens and observed caches need heads of 64 or 128 values and caches of at most 2^21 entries")
 
-    def _draft_tables(self):
-        """The rotary tables over all positions, kept from the first call on for every stream: so they are waited for once.  Those that
-        are made while a graph is recorded belong to the graph, and hold nothing before it is replayed."""
-        if self._tables is not None:
-            return self._tables
-        tables = rope_tables(torch.arange(self.cfg.max_positions, device=self.device), self.cfg.head_dim, self.cfg.rope_theta)
+    def _draft_tables(self, max_len):
+        """The rotary tables over all positions, of max_positions rows or, for a longer cache, as many as the next power of two of its
+        length.  They are kept from the first call on for every stream: so they are waited for once.  Those that are made while a graph
+        is recorded belong to the graph, and hold nothing before it is replayed."""
+        rows = max(self.cfg.max_positions, 1 << (max_len - 1).bit_length() if max_len > self.cfg.max_positions else 0)
+        if rows in self._tables:
+            return self._tables[rows]
+        tables = rope_tables(torch.arange(rows, device=self.device), self.cfg.head_dim, self.cfg.rope_theta)
         if not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream(self.device).synchronize()
-            self._tables = tables
+            self._tables[rows] = tables                  # all that were ever handed out stay: recorded steps read them
         return tables
 
     @torch.no_grad()
@@ -346,8 +348,9 @@ class Decoder(torch.nn.Module):
         # before anything is written: the attention, which comes after the first layer's append, would refuse these
         if not 1 <= S <= MAX_TOKENS or (tree is not None and tree.depth.shape[-1] != S):
             raise RuntimeError(f"draft takes 1 .. {MAX_TOKENS} tokens of a sequence, as many as its tree has")
-        self._check_attention(cache[0][0].shape[2])
-        tables = self._draft_tables()
+        T = cache[0][0].shape[2]
+        self._check_attention(T)
+        tables = self._draft_tables(T)
         at = lengths if positions is None else positions
         at = at[:, None] + (torch.arange(S, dtype=torch.int32, device=self.device) if tree is None else tree.depth)
         bits = None if tree is None else tree.bits

@@ -191,3 +191,17 @@ def test_what_draft_refuses_leaves_the_cache_as_it_was(cuda):
     with pytest.raises(RuntimeError, match="64 or 128"):
         small.new_cache(2, 100, observe=True)
     assert not any(bool(c[i].any()) for c in (*cache, *other) for i in (0, 1))
+
+
+def test_a_cache_longer_than_max_positions(cuda):
+    """What forward() takes draft() goes on with: the tables reach to the cache's end."""
+    m, other = _model(max_positions=16), _model()
+    prompt, ids, lengths = _ids(21, 2, 40), _ids(22, 2, 3), torch.tensor([40, 37], dtype=torch.int32, device="cuda")
+    got = []
+    for d in (m, other):
+        small, cache = d.new_cache(2, 10), d.new_cache(2, 70)
+        first = d.draft(ids, small, torch.tensor([0, 0], dtype=torch.int32, device="cuda"))       # (the tables of a short cache come first)
+        d(prompt, cache=cache, start=0)
+        got.append((first, d.draft(ids, cache, lengths)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and bool(a.isfinite().all())
