@@ -44,10 +44,12 @@ class DraftTree:
     @torch.no_grad()
     def accept_greedy(self, ids, logits):
         """The longest branch all of whose tokens (below the root) are what the model would have chosen after their parents; of
-        branches that are as long the first.  ids [B, S], logits [B, S, vocab] -> path int32 [B, depth of the tree + 1] (indices
+        branches that are as long the first.  Tokens below the root whose logits have a NaN (they did not fit the cache), or their
+        parent's, are not accepted; what follows a root with NaN logits is not chosen by the model.  ids [B, S], logits [B, S, vocab] -> path int32 [B, depth of the tree + 1] (indices
         behind the branch's end are not used), accepted int32 [B], chosen [B]: what the model chooses after the branch's last token."""
         choice = logits.argmax(dim=-1)                                                    # [B, S]
-        agreed = ids == choice[:, self._up]
+        lost = logits.gather(2, choice[:, :, None])[:, :, 0].isnan()                      # argmax takes a NaN for the largest
+        agreed = (ids == choice[:, self._up]) & ~lost & ~lost[:, self._up]
         agreed[:, 0] = True
         whole = (agreed[:, None, :] | ~self._above).all(dim=-1)                           # every token from the root down to i
         best = torch.where(whole, self.depth + 1, 0).argmax(dim=-1)                       # the first of the deepest

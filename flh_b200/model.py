@@ -343,7 +343,10 @@ class Decoder(torch.nn.Module):
         before).  lengths int32 [B]: entries that the sequences have, each its own.  positions int32 [B]: how many tokens they are
         long, where entries were evicted (default: lengths).  -> logits [B, S, vocab] of all tokens (the normed hidden states without
         a head).  lengths and positions are read on the device: a recorded step follows them.  What is kept of the tokens is
-        what accept() is told."""
+        what accept() is told.
+        A token whose entry would lie behind the cache's end is not stored and sees less than it should: its logits are NaN.  So are
+        those of a token whose position is behind the rotary tables (max_positions or the cache's length); its k is NaN in the cache
+        too, and once accepted makes NaN of all that follows it in its sequence."""
         B, S = ids.shape
         # before anything is written: the attention, which comes after the first layer's append, would refuse these
         if not 1 <= S <= MAX_TOKENS or (tree is not None and tree.depth.shape[-1] != S):
@@ -352,20 +355,23 @@ class Decoder(torch.nn.Module):
         self._check_attention(T)
         tables = self._draft_tables(T)
         at = lengths if positions is None else positions
-        at = at[:, None] + (torch.arange(S, dtype=torch.int32, device=self.device) if tree is None else tree.depth)
+        order = torch.arange(S, dtype=torch.int32, device=self.device)
+        at = at[:, None] + (order if tree is None else tree.depth)
         bits = None if tree is None else tree.bits
         x, pre = self.embed(ids), None
         for i, layer in enumerate(self.layers):
             out = layer(x, None, cache[i], tables, pre=pre, next_layer=self.layers[i + 1] if i + 1 < len(self.layers) else None,
                         draft=(lengths, at, bits))
             x, pre = out if isinstance(out, tuple) else (out, None)
-        x = self.norm(x)
+        entry = lengths[:, None] + order
+        x = self.norm(x).masked_fill(((entry < 0) | (entry >= T))[..., None], float("nan"))
         return x if self.head is None else self.head(x)
 
     @torch.no_grad()
     def accept(self, cache, lengths, path, accepted, drafted):
         """Keeps entries path[b, :accepted[b]] (int32 [B, A], from the root down) of the `drafted` ones behind lengths[b], in all
-        layers.  -> the new lengths."""
+        layers.  -> the new lengths, at most the cache's: a sequence that has filled it has to be evicted from (or ended) before the
+        next draft()."""
         return _CUDA.cache_accept([c[0] for c in cache], [c[1] for c in cache], lengths, path, accepted, drafted,
                                   weights=[c[3] for c in cache] if len(cache[0]) > 3 else None)
 

@@ -43,3 +43,13 @@ def test_the_configuration_takes_its_fields_in_the_order_they_had():
     from flh_b200.model import DecoderConfig
     c = DecoderConfig(4096, 32, 8, 14336, 4, 32000, 500000.0, 1e-6, "token_asym", 2)
     assert (c.rope_theta, c.eps, c.act_mode, c.tp) == (500000.0, 1e-6, "token_asym", 2) and c.max_positions == 32768
+
+
+def test_tokens_without_logits_are_not_accepted():
+    t = DraftTree([-1, 0, 0, 1])
+    logits = torch.nn.functional.one_hot(torch.tensor([[4, 0, 5, 2], [0, 3, 3, 3], [4, 2, 5, 2]]), 6).float()
+    logits[0, 1, 3] = float("nan")                  # token 1, which agrees
+    logits[1, 0] = float("nan")                     # the root: its children would agree with what argmax makes of it
+    logits[2, 3] = float("nan")
+    path, accepted, chosen = t.accept_greedy(torch.tensor([[1, 4, 4, 0], [1, 0, 0, 3], [1, 4, 1, 2]]), logits)
+    assert [p[:n] for p, n in zip(path.tolist(), accepted.tolist())] == [[0, 2], [0], [0, 1]] and chosen[0] == 5 and chosen[2] == 2

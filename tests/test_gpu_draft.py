@@ -205,3 +205,26 @@ def test_a_cache_longer_than_max_positions(cuda):
         got.append((first, d.draft(ids, cache, lengths)))
     for a, b in zip(*got):
         assert torch.equal(a, b) and bool(a.isfinite().all())
+
+
+@pytest.mark.parametrize("mode", ["group_sym", "token_asym"])
+def test_tokens_behind_the_end_of_the_cache(cuda, mode):
+    """They have no logits, and are not accepted; the others have those that they have in a longer cache."""
+    m = _model(mode)
+    prompt, tree = _ids(23, 4, 22), DraftTree([-1, 0, 1, 1, 2], "cuda")
+    lengths = torch.tensor([20, 22, 17, 18], dtype=torch.int32, device="cuda")
+    short, roomy = m.new_cache(4, 22), m.new_cache(4, 30)
+    for c in (short, roomy):
+        m(prompt, cache=c, start=0)
+    ids = _ids(24, 4, 5)
+    full = m.draft(ids, roomy, lengths, tree)
+    for i in range(1, 5):                                                      # every token below the root is what the model would choose
+        ids[:, i] = full[:, tree.parents[i]].argmax(-1)
+        full = m.draft(ids, roomy, lengths, tree)
+    got = m.draft(ids, short, lengths, tree)
+    fits = (lengths[:, None] + torch.arange(5, device="cuda") < 22)
+    assert fits.sum(1).tolist() == [2, 0, 5, 4]
+    assert bool(got[~fits].isnan().all()) and torch.equal(got[fits], full[fits])
+    path, accepted, chosen = tree.accept_greedy(ids, got)
+    assert accepted.tolist() == [2, 1, 4, 3] and [p[:n] for p, n in zip(path.tolist(), accepted.tolist())] == [[0, 1], [0], [0, 1, 2, 4], [0, 1, 2]]
+    assert m.accept(short, lengths, path, accepted, 5).tolist() == [22, 22, 21, 21]
