@@ -391,15 +391,16 @@ def rope_kv_at(qkv, cos, sin, positions, lengths, k_cache, v_cache, nh):
     return q
 
 
-def tree_attention(q, k_cache, v_cache, lengths, tree=None, weights=None, scale=None):
+def tree_attention(q, k_cache, v_cache, lengths, tree=None, weights=None, scale=None, counted=None):
     """Attention of S = 1 .. 64 drafted tokens of every sequence over a cache: token (b, s) sees entries 0 .. lengths[b] - 1 and, of the
     drafted entries lengths[b] + j, those whose bit j is set in tree[b, s].  q [B, S, nh, D] (any strides that are multiples of
     8 elements, the last dimension contiguous), caches [B, nkv, T, D], D 64 or 128, all float16 or all bfloat16; nh a multiple of
     nkv; lengths int32 [B]; tree int64 [S] or [B, S], or None for a chain (S = 1: ordinary decode).  scale: 1 / sqrt(D) by default.
     weights (f32 [B, nkv, T]): to every entry is added what all tokens and heads of the group gave it, what
-    cache_evict goes by.  -> [B, S, nh, D].  A token that sees no entry has zeros."""
+    cache_evict goes by; counted (int32 [B]): only by the first counted[b] tokens of sequence b.  -> [B, S, nh, D].  A token that sees
+    no entry has zeros."""
     if _host is not None:
-        r = _host.tree_attention(q, k_cache, v_cache, lengths, tree, weights, scale)
+        r = _host.tree_attention(q, k_cache, v_cache, lengths, tree, weights, scale, counted)
         if r is not None:
             return r
     _check_caches(k_cache, v_cache)
@@ -414,15 +415,18 @@ def tree_attention(q, k_cache, v_cache, lengths, tree=None, weights=None, scale=
     _check_ints(lengths, (B,), "lengths")
     _check(tree is None or (tree.dtype == torch.int64 and tree.is_contiguous() and tuple(tree.shape) in ((S,), (B, S))), "tree must be contiguous int64 [S] or [B, S]")
     _check(weights is None or (weights.dtype == torch.float32 and weights.is_contiguous() and tuple(weights.shape) == (B, nkv, T)), "weights must be contiguous float32 [B, kv heads, T]")
-    _check_device(q, k_cache, v_cache, lengths, tree, weights)
+    _check(counted is None or weights is not None, "counted goes with weights")
+    if counted is not None:
+        _check_ints(counted, (B,), "counted")
+    _check_device(q, k_cache, v_cache, lengths, tree, weights, counted)
     out = torch.empty((B, S, nh, D), dtype=q.dtype, device=q.device)
     sb, ss, sh = (st if n > 1 else 0 for st, n in zip(q.stride()[:3], q.shape))
     lib = _lib.load()
     with _guard(q.device):
         ws = _scratch(q.device, max(16, lib.flh_b200_tree_attention_workspace_bytes(B, S, nh, nkv, D, T, weights is not None)))
-        _lib.check(lib.flh_b200_tree_attention(
+        _lib.check(lib.flh_b200_tree_attention_counted(
             _ptr(q), sb, ss, sh, BF16 if q.dtype == torch.bfloat16 else F16, _ptr(k_cache), _ptr(v_cache), _ptr(lengths), _ptr(tree),
-            0 if tree is None or tree.dim() == 1 else S, 1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(out), _ptr(weights), B, S, nh, nkv, D, T,
+            0 if tree is None or tree.dim() == 1 else S, 1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(out), _ptr(weights), _ptr(counted), B, S, nh, nkv, D, T,
             _ptr(ws), ws.numel(), _stream(q)), "tree_attention")
     return out
 

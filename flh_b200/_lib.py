@@ -37,6 +37,8 @@ SIGNATURES = {
     "flh_b200_tree_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_long, c_int]),
     "flh_b200_tree_attention": (c_int, [c_void_p, c_long, c_long, c_long, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_float, c_void_p,
                                         c_void_p, c_int, c_int, c_int, c_int, c_int, c_long, c_void_p, c_size_t, c_void_p]),
+    "flh_b200_tree_attention_counted": (c_int, [c_void_p, c_long, c_long, c_long, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_long, c_float, c_void_p,
+                                                c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_long, c_void_p, c_size_t, c_void_p]),
     "flh_b200_tree_attention_status": (c_int, [c_void_p]),
     "flh_b200_cache_accept": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_long,
                                       c_int, c_int, c_void_p]),

@@ -292,6 +292,13 @@ size_t flh_b200_tree_attention_workspace_bytes(int B, int S, int nh, int nkv, in
 int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache, const int32_t *lengths,
                             const int64_t *tree, long tree_stride, float scale, void *out, float *weights, int B, int S, int nh, int nkv, int D, long T,
                             void *ws, size_t ws_bytes, void *stream) {
+    return flh_b200_tree_attention_counted(q, q_sb, q_ss, q_sh, dtype, k_cache, v_cache, lengths, tree, tree_stride, scale, out, weights, nullptr, B, S, nh, nkv, D, T, ws,
+                                           ws_bytes, stream);
+}
+
+int flh_b200_tree_attention_counted(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache, const int32_t *lengths,
+                                    const int64_t *tree, long tree_stride, float scale, void *out, float *weights, const int32_t *counted, int B, int S, int nh, int nkv,
+                                    int D, long T, void *ws, size_t ws_bytes, void *stream) {
     FLH_REQUIRE(dtype == FLH_B200_F16 || dtype == FLH_B200_BF16, FLH_B200_EINVAL, "bad dtype %d", dtype);
     FLH_REQUIRE(tree_shape(B, S, nh, nkv, D, T), FLH_B200_EINVAL, "bad shape B=%d S=%d nh=%d nkv=%d D=%d T=%ld (S 1 .. 64, D 64 or 128, nh a multiple of nkv)", B, S, nh, nkv,
                 D, T);
@@ -301,6 +308,7 @@ int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int 
     FLH_REQUIRE(scale > 0.0f && scale <= 2.0e38f, FLH_B200_EINVAL, "scale must be positive, and finite in powers of two too");
     FLH_REQUIRE(q_sb % 8 == 0 && q_ss % 8 == 0 && q_sh % 8 == 0, FLH_B200_EALIGN, "strides of q must be multiples of 8 elements");
     FLH_REQUIRE(tree_stride == 0 || tree_stride == S, FLH_B200_EINVAL, "tree must be [S] or [B, S]");
+    FLH_REQUIRE(weights || !counted, FLH_B200_EINVAL, "counted goes with weights");
     if (B == 0) return 0;
     FLH_REQUIRE(q && k_cache && v_cache && lengths && out, FLH_B200_EINVAL, "null pointer");
     FLH_REQUIRE(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out) && aligned16(ws), FLH_B200_EALIGN, "pointers must be 16-byte aligned");
@@ -308,7 +316,7 @@ int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int 
     TreeAttnParams p = {};
     p.q = q; p.q_sb = q_sb; p.q_ss = q_ss; p.q_sh = q_sh;
     p.lengths = lengths; p.tree = tree; p.tree_sb = tree_stride;
-    p.k = k_cache; p.v = v_cache; p.out = out; p.weights = weights;
+    p.k = k_cache; p.v = v_cache; p.out = out; p.weights = weights; p.counted = counted;
     p.B = B; p.S = S; p.nh = nh; p.nkv = nkv; p.D = D; p.T = (int)T;
     p.scale_log2 = scale * 1.4426950408889634f;
     return launch_tree_attention(p, dtype == FLH_B200_BF16, static_cast<uint8_t *>(ws), static_cast<cudaStream_t>(stream));

@@ -34,6 +34,7 @@ struct TreeAttnParams {
     const void *k, *v;                     // [B, nkv, T, D]
     void *out;                             // [B, S, nh, D]
     float *weights;                        // [B, nkv, T], added to; or null
+    const int32_t *counted;                // [B]: tokens of each sequence whose weights are added; null: all
     int B, S, nh, nkv, g, D, R, nrb, rows; // nrb: blocks of `rows` rows
     uint32_t g_inverse;                    // 2^32 / g, rounded up (g > 1)
     int T;
@@ -58,6 +59,8 @@ __device__ __forceinline__ int entries(const TreeAttnParams &p, int len) { retur
 
 // row / g: exact for row < 64 g with g <= 4096, where row * (g_inverse * g - 2^32) < 64 g * g < 2^32
 __device__ __forceinline__ int token_of(const TreeAttnParams &p, int row) { return p.g == 1 ? row : (int)__umulhi((uint32_t)row, p.g_inverse); }
+// rows of a sequence whose weights are added
+__device__ __forceinline__ int counted_rows(const TreeAttnParams &p, int b) { return p.counted ? min(max(p.counted[b], 0), p.S) * p.g : p.R; }
 // element offset of a row of q
 __device__ __forceinline__ long q_offset(const TreeAttnParams &p, int b, int kvh, int row) {
     const int s = token_of(p, row);

@@ -75,7 +75,8 @@ __device__ __forceinline__ void add_weights(const TreeAttnParams &p, int b, int 
         was[k] = w[at[k]];
     }
     const bool drafted = at[EACH - 1] >= len;                             // some may not be seen by every row
-    for (int r0 = 0; r0 < p.R; r0 += ROWS) {
+    const int rows = counted_rows(p, b);
+    for (int r0 = 0; r0 < rows; r0 += ROWS) {
         float x[ROWS][EACH], l[ROWS];     // fetched together
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
@@ -86,7 +87,7 @@ __device__ __forceinline__ void add_weights(const TreeAttnParams &p, int b, int 
         }
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            if (r0 + i >= p.R) break;
+            if (r0 + i >= rows) break;
             const uint64_t bits = drafted ? drafted_bits(p, b, token_of(p, r0 + i), len) : 0;
 #pragma unroll
             for (int k = 0; k < EACH; ++k) {

@@ -505,14 +505,14 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
         if (ok) ok = mbar_wait_warp(g_status_attn_tc, smem_u32(bar), phase & 1, &abort_flag, code);
     };
     uint32_t it = 0;                                                             // tiles so far, of all rows
-    // with more rows than 128 a few tiles at a time, so that an entry's sum over all of them is added to its weight once
-    const int group = p.R > kRowsTc ? kWeightGroup : 1 << 20;
     for (int piece = u0, piece_end; piece < u1; piece = piece_end) {
     while (piece >= job.begin + job.nt) job.next(p);
     piece_end = min(u1, job.begin + job.nt);
     const int b = job.b, kvh = job.job, bh = b * p.nkv + kvh, len = job.len, n = entries(p, len), first = piece - job.begin, last = piece_end - job.begin;
+    // with more rows than 128 a few tiles at a time, so that an entry's sum over all of them is added to its weight once
+    const int rows = counted_rows(p, b), group = rows > kRowsTc ? kWeightGroup : 1 << 20;
     for (int g0 = first; g0 < last; g0 += group)
-    for (int row0 = 0; row0 < p.R; row0 += kRowsTc) {
+    for (int row0 = 0; row0 < rows; row0 += kRowsTc) {
         const int g1 = min(g0 + group, last);
         __syncthreads();                                                         // the rows before have been multiplied and looked at
         constexpr int kStep = kThreadsWeights / (D / 8), kLoads = kRowsTc / kStep;
@@ -523,16 +523,16 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
             q[i] = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.q) + q_offset(p, b, kvh, min(row0 + r_of + i * kStep, p.R - 1)) + c * 8);
         if (tid < kRowsTc) {
             const int row = row0 + tid;
-            const uint64_t bits = row < p.R ? drafted_bits(p, b, token_of(p, row), len) : 0;
+            const uint64_t bits = row < rows ? drafted_bits(p, b, token_of(p, row), len) : 0;
             if (last * kWeightTile > len) {                                      // some of the drafted entries are this CTA's
 #pragma unroll 8
                 for (int j = 0; j < 64; ++j) {
-                    const uint32_t rows = __ballot_sync(0xffffffffu, (bits >> j) & 1);
-                    if (lane == 0) seen[j][warp] = rows;
+                    const uint32_t seeing = __ballot_sync(0xffffffffu, (bits >> j) & 1);
+                    if (lane == 0) seen[j][warp] = seeing;
                 }
             }
-            // rows that do not exist or see nothing have no weight anywhere
-            lse[tid] = row >= p.R || (len == 0 && !bits) ? INFINITY : p.lse[(long)bh * p.R + row];
+            // rows that do not count or see nothing have no weight anywhere
+            lse[tid] = row >= rows || (len == 0 && !bits) ? INFINITY : p.lse[(long)bh * p.R + row];
         }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
         }
         fence_proxy_async();
         __syncthreads();
-        const int cols = (min(p.R - row0, kRowsTc) + 15) / 16 * 16;
+        const int cols = (min(rows - row0, kRowsTc) + 15) / 16 * 16;
         if (warp == 0) {
             for (int tile = g0; tile < g1; ++tile, ++it) {
                 const int slot = it & 1;
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
             float *w = p.weights + (long)bh * p.T;
             for (int tile = g0; tile < g1; ++tile, ++it) {
                 const int slot = it & 1, t = tile * kWeightTile + (warp & 3) * 32 + lane, j = t - len;
-                const bool done = row0 + kRowsTc >= p.R;
+                const bool done = row0 + kRowsTc >= rows;
                 const float was = done && t < n ? w[t] : 0.0f;
                 wait(&s_full[slot], it >> 1, 64);
                 tc_fence_after();

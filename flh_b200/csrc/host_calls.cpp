@@ -214,21 +214,22 @@ bool is_cache(const at::Tensor &t) { return t.dim() == 4 && (t.scalar_type() == 
 int dtype_of(const at::Tensor &t) { return t.scalar_type() == at::kBFloat16 ? FLH_B200_BF16 : FLH_B200_F16; }
 bool ints(const at::Tensor &t, at::IntArrayRef sizes) { return t.scalar_type() == at::kInt && t.sizes() == sizes; }
 
-// tree_attention(q, k, v, lengths, tree or None, weights or None, scale or None) -> out
+// tree_attention(q, k, v, lengths, tree or None, weights or None, scale or None, counted or None) -> out
 PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 7) Py_RETURN_NONE;
-    const at::Tensor *t[6];
-    for (int i = 0; i < 6; ++i) {
-        t[i] = tensor(args[i]);
-        if (!t[i] && (args[i] != Py_None || i < 4)) Py_RETURN_NONE;
+    if (n != 8) Py_RETURN_NONE;
+    const at::Tensor *t[7];
+    for (int i = 0; i < 7; ++i) {
+        PyObject *arg = args[i < 6 ? i : 7];
+        t[i] = tensor(arg);
+        if (!t[i] && (arg != Py_None || i < 4)) Py_RETURN_NONE;
     }
     const double given = args[6] == Py_None ? 0 : PyFloat_AsDouble(args[6]);
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
     const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2];
     if (!q.is_cuda() || observed() || q.dim() != 4 || !is_cache(k) || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || q.scalar_type() != k.scalar_type()) Py_RETURN_NONE;
     const c10::DeviceIndex dev = c10::cuda::current_device();
-    for (int i = 0; i < 6; ++i)
+    for (int i = 0; i < 7; ++i)
         if (t[i] && !plain(*t[i], dev, i == 0)) Py_RETURN_NONE;
     const int64_t B = k.size(0), nkv = k.size(1), T = k.size(2), D = k.size(3), S = q.size(1), nh = q.size(2);
     if (q.size(0) != B || q.size(3) != D || B == 0 || S == 0 || S > FLH_B200_TREE_MAX_TOKENS || nkv == 0 || nh == 0 || nh % nkv || T == 0 || q.stride(3) != 1 || !ints(*t[3], {B}) ||
@@ -241,11 +242,12 @@ PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     }
     if (t[4] && (t[4]->scalar_type() != at::kLong || (t[4]->sizes() != at::IntArrayRef({S}) && t[4]->sizes() != at::IntArrayRef({B, S})))) Py_RETURN_NONE;
     if (t[5] && (t[5]->scalar_type() != at::kFloat || t[5]->sizes() != at::IntArrayRef({B, nkv, T}))) Py_RETURN_NONE;
+    if (t[6] && (!t[5] || !ints(*t[6], {B}))) Py_RETURN_NONE;
     const float scale = args[6] == Py_None ? (float)(1.0 / std::sqrt((double)D)) : (float)given;
     const long tree_stride = t[4] && t[4]->dim() == 2 ? S : 0;
-    at::Tensor held[6], out, ws;
-    void *ptr[6] = {};
-    for (int i = 0; i < 6; ++i)
+    at::Tensor held[7], out, ws;
+    void *ptr[7] = {};
+    for (int i = 0; i < 7; ++i)
         if (t[i]) { held[i] = *t[i]; ptr[i] = t[i]->data_ptr(); }
     const size_t need = flh_b200_tree_attention_workspace_bytes((int)B, (int)S, (int)nh, (int)nkv, (int)D, T, ptr[5] != nullptr);
     if (!need) Py_RETURN_NONE;
@@ -254,8 +256,8 @@ PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const Unlocked unlocked;
         out = empty({B, S, nh, D}, held[0].scalar_type(), held[0]);
         ws = empty({(int64_t)need}, at::kByte, held[0]);                // of this call alone, freed in stream order when it returns
-        rc = flh_b200_tree_attention(ptr[0], st[0], st[1], st[2], dtype_of(held[0]), ptr[1], ptr[2], static_cast<const int32_t *>(ptr[3]), static_cast<const int64_t *>(ptr[4]),
-                                     tree_stride, scale, out.data_ptr(), static_cast<float *>(ptr[5]), (int)B, (int)S, (int)nh, (int)nkv, (int)D, T, ws.data_ptr(), need,
+        rc = flh_b200_tree_attention_counted(ptr[0], st[0], st[1], st[2], dtype_of(held[0]), ptr[1], ptr[2], static_cast<const int32_t *>(ptr[3]), static_cast<const int64_t *>(ptr[4]),
+                                     tree_stride, scale, out.data_ptr(), static_cast<float *>(ptr[5]), static_cast<const int32_t *>(ptr[6]), (int)B, (int)S, (int)nh, (int)nkv, (int)D, T, ws.data_ptr(), need,
                                      c10::cuda::getCurrentCUDAStream(dev).stream());
     }
     if (rc) return failed("tree_attention", rc);

@@ -149,7 +149,11 @@ class DecoderLayer(torch.nn.Module):
         """Attention of drafted tokens behind sequences of their own lengths (Decoder.draft): [B, S, heads * D]."""
         lengths, positions, bits = draft
         q = _CUDA.rope_kv_at(qkv.view(-1, qkv.shape[-1]), tables[0], tables[1], positions, lengths, cache[0], cache[1], self.nh)
-        att = _CUDA.tree_attention(q, cache[0], cache[1], lengths, tree=bits, weights=cache[3] if len(cache) > 3 else None)
+        S, weights = q.shape[1], cache[3] if len(cache) > 3 else None
+        if weights is not None and S > 1:                # what these tokens look at counts when they are accepted (Decoder.accept)
+            cache.drafted[:, :S].copy_(q)
+            weights = None
+        att = _CUDA.tree_attention(q, cache[0], cache[1], lengths, tree=bits, weights=weights)
         return att.view(qkv.shape[0], qkv.shape[1], -1)
 
     def forward(self, x, pos, cache=None, tables=None, shape=None, pre=None, next_layer=None, draft=None):
@@ -162,7 +166,7 @@ class DecoderLayer(torch.nn.Module):
         layer's quantised input) to it.
         draft = (lengths, positions, tree bits): the tokens are drafted ones behind entries lengths[b] of the cache, tables are
         over all positions (Decoder.draft).  A cache with accumulated weights (Decoder.new_cache(observe=True)) gets those of the
-        last 64 tokens of a call."""
+        last 64 tokens of a call; of several drafted tokens it keeps q until it is known which of them stay."""
         cfg = self.cfg
         sp = x.dim() == 2                                # sequence-parallel: x holds this rank's T / tp of the B * S rows (tp.local_rows)
         if sp:
@@ -280,6 +284,10 @@ class DecoderLayer(torch.nn.Module):
             return x + y
 
 
+class ObservedLayer(list):
+    """[k, v, cursor, weights] of a layer of Decoder.new_cache(observe=True), and drafted: the rotated q of the last draft's tokens."""
+
+
 class Decoder(torch.nn.Module):
     """Embedding -> layers -> final norm -> f16 lm_head (the head stays f16 in FLH, :1032-1046)."""
 
@@ -307,16 +315,21 @@ class Decoder(torch.nn.Module):
         return self
 
     def new_cache(self, batch, max_len, observe=False):
-        """A list of [k, v, cursor] per layer.  observe: [k, v, cursor, weights], where every call adds to weights (f32 [B, kv heads,
-        max_len]) the attention that its last 64 tokens gave each entry, which evict() goes by."""
+        """A list of [k, v, cursor] per layer.  observe: [k, v, cursor, weights], where the tokens of every sequence add to weights (f32
+        [B, kv heads, max_len]) the attention that they gave each entry, which evict() goes by: the last 64 of each forward() (padding, where a
+        batch has some, among them), the one token of a draft() of one, and of a draft() of several those that accept() keeps."""
         c = self.cfg
         if observe:
             self._check_attention(max_len)
         nkv = max(c.n_kv_heads // c.tp, 1)
-        return [[torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device),
-                 torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device), 0]
-                + ([torch.zeros(batch, nkv, max_len, dtype=torch.float32, device=self.device)] if observe else [])
-                for _ in range(c.n_layers)]
+        cache = [[torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device),
+                  torch.zeros(batch, nkv, max_len, c.head_dim, dtype=torch.float16, device=self.device), 0] for _ in range(c.n_layers)]
+        if not observe:
+            return cache
+        cache = [ObservedLayer(layer + [torch.zeros(batch, nkv, max_len, dtype=torch.float32, device=self.device)]) for layer in cache]
+        for layer in cache:                              # of this size from the start: recorded steps write and read it
+            layer.drafted = torch.zeros(batch, MAX_TOKENS, c.n_heads // c.tp, c.head_dim, dtype=torch.float16, device=self.device)
+        return cache
 
     def _check_attention(self, max_len):
         """What _CUDA.tree_attention takes of a decoder and its cache."""
@@ -351,6 +364,8 @@ class Decoder(torch.nn.Module):
         # before anything is written: the attention, which comes after the first layer's append, would refuse these
         if not 1 <= S <= MAX_TOKENS or (tree is not None and tree.depth.shape[-1] != S):
             raise RuntimeError(f"draft takes 1 .. {MAX_TOKENS} tokens of a sequence, as many as its tree has")
+        if S > 1 and len(cache[0]) > 3 and not all(hasattr(c, "drafted") for c in cache):
+            raise RuntimeError("a cache with accumulated weights has to be one of new_cache(observe=True)")
         T = cache[0][0].shape[2]
         self._check_attention(T)
         tables = self._draft_tables(T)
@@ -358,6 +373,8 @@ class Decoder(torch.nn.Module):
         order = torch.arange(S, dtype=torch.int32, device=self.device)
         at = at[:, None] + (order if tree is None else tree.depth)
         bits = None if tree is None else tree.bits
+        if len(cache[0]) > 3:                            # nobody has looked at the drafted entries yet, whatever was there before
+            _CUDA.cache_accept(*self._layers(cache), lengths, lengths.new_empty((B, 0)), torch.zeros_like(lengths), S, weights=[c[3] for c in cache])
         x, pre = self.embed(ids), None
         for i, layer in enumerate(self.layers):
             out = layer(x, None, cache[i], tables, pre=pre, next_layer=self.layers[i + 1] if i + 1 < len(self.layers) else None,
@@ -371,9 +388,25 @@ class Decoder(torch.nn.Module):
     def accept(self, cache, lengths, path, accepted, drafted):
         """Keeps entries path[b, :accepted[b]] (int32 [B, A], from the root down) of the `drafted` ones behind lengths[b], in all
         layers.  -> the new lengths, at most the cache's: a sequence that has filled it has to be evicted from (or ended) before the
-        next draft()."""
-        return _CUDA.cache_accept([c[0] for c in cache], [c[1] for c in cache], lengths, path, accepted, drafted,
-                                  weights=[c[3] for c in cache] if len(cache[0]) > 3 else None)
+        next draft().  In a cache with accumulated weights, `drafted` tokens of the last draft(), more than one, add theirs now: each layer
+        attends once more, with the accepted tokens alone, so that what was guessed wrong leaves nothing behind."""
+        observe = len(cache[0]) > 3
+        now = _CUDA.cache_accept(*self._layers(cache), lengths, path, accepted, drafted, weights=[c[3] for c in cache] if observe else None)
+        B, A = path.shape
+        if observe and drafted > 1 and A:
+            # the tokens that the entries behind lengths now hold: a chain
+            own = torch.arange(A, dtype=torch.int32, device=path.device)
+            taken = (path >= 0) & (path < drafted) & (lengths[:, None] + path < cache[0][0].shape[2])
+            held = torch.where(taken, path, own).long()[:, :, None, None]
+            counted = now - lengths
+            for c in cache:
+                q = c.drafted.gather(1, held.expand(B, A, *c.drafted.shape[2:]))
+                _CUDA.tree_attention(q, c[0], c[1], lengths, weights=c[3], counted=counted)
+        return now
+
+    @staticmethod
+    def _layers(cache):
+        return [c[0] for c in cache], [c[1] for c in cache]
 
     @torch.no_grad()
     def evict(self, cache, lengths, keep, recent):
@@ -381,7 +414,7 @@ class Decoder(torch.nn.Module):
         -> the new lengths; the tokens that follow go through draft() with the positions they would have had."""
         if len(cache[0]) < 4:
             raise RuntimeError("evict needs a cache with accumulated weights (new_cache(observe=True))")
-        _, left, now = _CUDA.cache_evict([c[0] for c in cache], [c[1] for c in cache], [c[3] for c in cache], lengths, keep, recent)
+        _, left, now = _CUDA.cache_evict(*self._layers(cache), [c[3] for c in cache], lengths, keep, recent)
         for c, w in zip(cache, left.unbind(0)):
             c[3].copy_(w)                                # in place: a recorded step goes on adding to it
         return now

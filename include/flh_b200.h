@@ -207,6 +207,11 @@ size_t flh_b200_tree_attention_workspace_bytes(int B, int S, int nh, int nkv, in
 int flh_b200_tree_attention(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache,
                             const int32_t *lengths, const int64_t *tree, long tree_stride, float scale, void *out, float *weights,
                             int B, int S, int nh, int nkv, int D, long T, void *ws, size_t ws_bytes, void *stream);
+/* The same, where of sequence b only the first counted[b] tokens (int32 [B], on the device; the nearer end of 0 .. S; NULL: all) add to
+ * weights: what a branch gave once it is known how much of it is kept. */
+int flh_b200_tree_attention_counted(const void *q, long q_sb, long q_ss, long q_sh, int dtype, const void *k_cache, const void *v_cache,
+                                    const int32_t *lengths, const int64_t *tree, long tree_stride, float scale, void *out, float *weights,
+                                    const int32_t *counted, int B, int S, int nh, int nkv, int D, long T, void *ws, size_t ws_bytes, void *stream);
 /* [code, cta, 0, 0] of the attention's bounded waits, as flh_b200_gemm_status; synchronises. */
 int flh_b200_tree_attention_status(int *out);
 

@@ -228,3 +228,122 @@ def test_tokens_behind_the_end_of_the_cache(cuda, mode):
     path, accepted, chosen = tree.accept_greedy(ids, got)
     assert accepted.tolist() == [2, 1, 4, 3] and [p[:n] for p, n in zip(path.tolist(), accepted.tolist())] == [[0, 1], [0], [0, 1, 2, 4], [0, 1, 2]]
     assert m.accept(short, lengths, path, accepted, 5).tolist() == [22, 22, 21, 21]
+
+
+def _observed(m, prompt, room=40):
+    cache = m.new_cache(prompt.shape[0], prompt.shape[1] + room, observe=True)
+    m(prompt, cache=cache, start=0)
+    return cache
+
+
+@pytest.mark.parametrize("n_heads,n_kv_heads", [(4, 2), (4, 1)])
+def test_what_is_not_accepted_leaves_no_weights(cuda, n_heads, n_kv_heads):
+    """Accepted tokens add what they would have added one at a time; whatever else was drafted makes no difference."""
+    m = _model(n_heads=n_heads, n_kv_heads=n_kv_heads)
+    prompt = _ids(31, 2, 30)
+    # 8 tokens of which 0 2 3 6 and 0 1 are accepted; 40 of which the same are: more rows than one kernel takes
+    for size in (8, 40):
+        tree = DraftTree([-1, 0, 0, 2, 2, 1, 3, 4] + [7] * (size - 8), "cuda")
+        path, accepted = torch.tensor([[0, 2, 3, 6], [0, 1, 0, 0]], dtype=torch.int32, device="cuda"), torch.tensor([4, 2], dtype=torch.int32, device="cuda")
+        runs = []
+        for seed in (33, 34):                                                  # other tokens where nothing is accepted
+            ids = _ids(seed, 2, size)
+            right = _ids(32, 2, 8)
+            ids[0, [0, 2, 3, 6]], ids[1, [0, 1]] = right[0, [0, 2, 3, 6]], right[1, [0, 1]]
+            cache, lengths = _observed(m, prompt, 50), torch.tensor([30, 30], dtype=torch.int32, device="cuda")
+            before = [c[3].clone() for c in cache]
+            m.draft(ids, cache, lengths, tree)
+            assert all(torch.equal(c[3], w) for c, w in zip(cache, before))
+            now = m.accept(cache, lengths, path, accepted, size)
+            runs.append((cache, ids))
+            assert now.tolist() == [34, 32]
+            for c in cache:
+                for b, n in enumerate((4, 2)):
+                    total = (30 + n) * n_heads / n_kv_heads
+                    assert torch.allclose(c[3][b].sum(-1), torch.full((n_kv_heads,), total, device="cuda"), rtol=1e-4)
+                    assert not c[3][b, :, 30 + n:].any() and bool((c[3][b, :, 30:30 + n] > 0).all())
+        for a, b in zip(runs[0][0], runs[1][0]):
+            assert torch.equal(a[3], b[3])
+        # the same, one token at a time
+        cache, ids = runs[0]
+        for b, branch in enumerate(([0, 2, 3, 6], [0, 1])):
+            one = _observed(m, prompt[b:b + 1], 50)
+            for i, t in enumerate(branch):
+                m.draft(ids[b:b + 1, t:t + 1], one, torch.tensor([30 + i], dtype=torch.int32, device="cuda"))
+            # the first layer sees the same q and k up to a rounding of the products before them; in the second a quantised code may flip
+            assert torch.allclose(cache[0][3][b], one[0][3][0], rtol=2e-2, atol=1e-3)
+            assert (cache[1][3][b] - one[1][3][0]).abs().sum() < 0.05 * one[1][3][0].sum()
+
+
+def test_entries_that_are_drafted_over_have_no_weights_of_before(cuda):
+    """The second sequence is shorter than the prompt that was run: what lies behind its length counts for nothing."""
+    m = _model()
+    prompt = _ids(41, 2, 30)
+    lengths = torch.tensor([30, 22], dtype=torch.int32, device="cuda")
+    for S, accepted in ((1, None), (5, 3)):
+        cache = _observed(m, prompt)
+        kept = [c[3].clone() for c in cache]
+        m.draft(_ids(42, 2, S), cache, lengths)
+        if accepted:
+            m.accept(cache, lengths, torch.arange(S, dtype=torch.int32, device="cuda").repeat(2, 1), torch.full_like(lengths, accepted), S)
+        for c, w in zip(cache, kept):
+            n = accepted or 1
+            assert bool(((c[3] - w)[1, :, :22] >= 0).all()) and torch.allclose((c[3][1, :, :22 + n].sum(-1) - w[1, :, :22].sum(-1)), torch.tensor(2.0 * n, device="cuda"), rtol=1e-3)
+
+
+def test_recorded_drafts_of_an_observed_cache(cuda):
+    """Two recorded steps, of one tree and of another, replayed in turn: accept counts those of the last replay."""
+    m = _model()
+    prompt, trees = _ids(51, 2, 24), [DraftTree([-1, 0, 0, 1], "cuda"), DraftTree([-1, 0, 1, 0, 3, 4], "cuda")]
+    lengths, ids = torch.tensor([24, 20], dtype=torch.int32, device="cuda"), [_ids(52, 2, 4), _ids(53, 2, 6)]
+    paths = [torch.tensor([[0, 1, 3], [0, 2, 0]], dtype=torch.int32, device="cuda"), torch.tensor([[0, 3, 4, 5], [0, 1, 2, 0]], dtype=torch.int32, device="cuda")]
+    counts = [torch.tensor([3, 2], dtype=torch.int32, device="cuda"), torch.tensor([4, 0], dtype=torch.int32, device="cuda")]
+    cache, eager = _observed(m, prompt, 60), _observed(m, prompt, 60)
+    other, at = _observed(m, prompt, 60), lengths.clone()
+    for t, i in zip(trees, ids):
+        m.draft(i, other, at, t)                                               # (what is made at the first call)
+    torch.cuda.synchronize()
+    drafts, accepts = [], []
+    for k in range(2):
+        g, h = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            m.draft(ids[k], cache, at, trees[k])
+        with torch.cuda.graph(h):
+            now = m.accept(cache, at, paths[k], counts[k], trees[k].size)
+        drafts.append(g), accepts.append((h, now))
+    n = lengths.clone()
+    for k, recorded in ((0, True), (1, False), (0, False), (1, True)):
+        drafts[k].replay()
+        if recorded:
+            accepts[k][0].replay()
+            at.copy_(accepts[k][1])
+        else:
+            at.copy_(m.accept(cache, at, paths[k], counts[k], trees[k].size))
+        m.draft(ids[k], eager, n, trees[k])
+        n = m.accept(eager, n, paths[k], counts[k], trees[k].size)
+        assert torch.equal(at, n)
+        for a, b in zip(cache, eager):
+            assert torch.equal(a[3], b[3])
+            for s, e in enumerate(n.tolist()):
+                assert torch.equal(a[0][s, :, :e], b[0][s, :, :e]) and torch.equal(a[1][s, :, :e], b[1][s, :, :e])
+
+
+def test_evicting_by_what_was_accepted(cuda):
+    """Draft, accept and evict on an observed cache: the same entries stay whatever was guessed beside the accepted tokens."""
+    m = _model()
+    prompt, tree = _ids(61, 1, 40), DraftTree([-1, 0, 0, 1, 2, 4], "cuda")
+    path, accepted, kept = torch.tensor([[0, 2, 4]], dtype=torch.int32, device="cuda"), torch.tensor([3], dtype=torch.int32, device="cuda"), []
+    for seed in (62, 63):
+        cache, lengths, positions = _observed(m, prompt), torch.tensor([40], dtype=torch.int32, device="cuda"), torch.tensor([40], dtype=torch.int32, device="cuda")
+        for step in range(4):
+            ids, right = _ids(seed + 10 * step, 1, 6), _ids(70 + step, 1, 6)
+            ids[:, [0, 2, 4]] = right[:, [0, 2, 4]]
+            m.draft(ids, cache, lengths, tree, positions=positions)
+            lengths, positions = m.accept(cache, lengths, path, accepted, 6), positions + accepted
+            if step % 2:
+                lengths = m.evict(cache, lengths, 24, 6)
+        kept.append([(c[0][:, :, :24].clone(), c[3].clone()) for c in cache])
+    for (ka, wa), (kb, wb) in zip(*kept):
+        assert torch.equal(ka, kb) and torch.equal(wa, wb)
+    with pytest.raises(RuntimeError, match="observe=True"):
+        m.draft(_ids(1, 1, 3), [list(c) for c in cache], lengths)

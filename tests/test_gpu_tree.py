@@ -633,3 +633,40 @@ def test_odd_values_where_two_blocks_of_rows_share_a_tile(cuda, g, D, dtype):
             odd = torch.arange(D, device="cuda") % 8 == b % 8
             assert torch.equal(got[b, S - 1][:, ~odd], want[b, S - 1][:, ~odd]) and bool((got[b, S - 1][:, odd] == float("inf")).all())
     assert cuda.tree_attention_status()[0] == 0
+
+
+@pytest.mark.parametrize("B,S,nh,nkv,D,T", [(3, 4, 8, 2, 128, 200), (3, 4, 8, 2, 64, 9000), (40, 5, 6, 3, 64, 700), (3, 33, 8, 2, 128, 500), (4, 64, 12, 2, 64, 300), (2, 64, 16, 2, 128, 5000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_of_the_first_tokens_only(cuda, B, S, nh, nkv, D, T, dtype):
+    """counted tokens of each sequence add to the weights, none to all of them; the output is that of all tokens."""
+    r = rs(B + S)
+    lengths, counted = [int(x) for x in r.randint(0, T - S, size=B)], [int(x) for x in r.randint(0, S + 1, size=B)]
+    lengths[0], counted[-1], counted[0], counted[1] = T - S, 1, 0, S
+    q, k, v = _normal(1, B, S, nh, D, dtype=dtype), _normal(2, B, nkv, T, D, dtype=dtype), _normal(3, B, nkv, T, D, dtype=dtype)
+    tree = torch.stack([R.random_tree(r, S)[0] for _ in lengths]).cuda()
+    start = torch.rand(B, nkv, T, device="cuda")
+    w, every, given = start.clone(), start.clone(), list(counted)
+    given[1], given[0] = S + 100, -3                                           # the nearer end
+    out = cuda.tree_attention(q, k, v, _ints(lengths), tree=tree, weights=w, counted=_ints(given))
+    assert torch.equal(out.view(torch.int16), cuda.tree_attention(q, k, v, _ints(lengths), tree=tree).view(torch.int16))
+    for b, c in enumerate(counted):
+        if c == 0:
+            assert torch.equal(w[b], start[b])
+            continue
+        _, _, ww, wtol = R.attention(q[b:b + 1, :c], k[b:b + 1], v[b:b + 1], lengths[b:b + 1], tree[b:b + 1, :c])
+        total = start[b:b + 1].double() + ww
+        R.assert_close(w[b:b + 1], total, wtol + 2.0 ** -24 * total.abs())
+    cuda.tree_attention(q, k, v, _ints(lengths), tree=tree, weights=every, counted=_ints([S] * B))
+    again = start.clone()
+    cuda.tree_attention(q, k, v, _ints(lengths), tree=tree, weights=again)
+    assert torch.equal(every, again) and cuda.tree_attention_status()[0] == 0
+
+
+def test_counted_without_the_native_call(cuda, monkeypatch):
+    q, k, v, lengths, counted = _normal(1, 2, 3, 4, 64), _normal(2, 2, 2, 90, 64), _normal(3, 2, 2, 90, 64), _ints([60, 33]), _ints([1, 2])
+    got = []
+    for host in (cuda._host, None):
+        monkeypatch.setattr(cuda, "_host", host)
+        w = torch.zeros(2, 2, 90, device="cuda")
+        got.append((cuda.tree_attention(q, k, v, lengths, weights=w, counted=counted), w))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.allclose(w.sum((1, 2)), torch.tensor([4.0, 8.0], device="cuda"), rtol=1e-4)

@@ -143,3 +143,22 @@ def test_reference_eviction_order():
     w = np.array([1, np.nan, 2, 2, np.inf, -0.0, 0.0, 9], dtype=np.float32)
     assert R.evict(w, 8, 3, 1).tolist() == [1, 4, 7] and R.evict(w, 8, 4, 1).tolist() == [1, 2, 4, 7] and R.evict(w, 7, 6, 0).tolist() == [0, 1, 2, 3, 4, 5]
     assert R.evict(w, 3, 3, 1).tolist() == [0, 1, 2] and R.evict(w, 8, 2, 2).tolist() == [6, 7]
+
+
+@pytest.mark.parametrize("other,message", [
+    (dict(counted=_i32(2)), "counted goes with weights"),
+    (dict(counted=_i32(3), weights=torch.zeros(2, 2, 20)), "counted"),
+    (dict(counted=_i32(2).long(), weights=torch.zeros(2, 2, 20)), "counted"),
+    (dict(counted=_i32(2), weights=torch.zeros(2, 2, 20)), "must be CUDA"),
+])
+def test_counted_is_refused(other, message):
+    from flh_b200 import _CUDA
+    with pytest.raises(RuntimeError, match=message):
+        _CUDA.tree_attention(**_attention(**other))
+
+
+def test_the_c_entry_refuses_counted_without_weights():
+    from flh_b200 import _lib
+    lib, one = _lib.load(), ctypes.c_void_p(16)
+    assert lib.flh_b200_tree_attention_counted(one, 768, 256, 64, 0, one, one, one, None, 0, 1.0, one, None, one, 2, 3, 4, 2, 64, 20, one, 1 << 30, None) == 1
+    assert b"counted" in lib.flh_b200_last_error()
