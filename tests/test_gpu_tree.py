@@ -670,3 +670,13 @@ def test_counted_without_the_native_call(cuda, monkeypatch):
         w = torch.zeros(2, 2, 90, device="cuda")
         got.append((cuda.tree_attention(q, k, v, lengths, weights=w, counted=counted), w))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and torch.allclose(w.sum((1, 2)), torch.tensor([4.0, 8.0], device="cuda"), rtol=1e-4)
+
+
+@pytest.mark.parametrize("L,B,nkv,T,lengths", [(4, 4, 5, 50001, [50001, 45056, 45057, 49000]), (1, 1, 1, 400003, [400001]), (1, 1, 2, 364600, [364571])])
+def test_cache_evict_of_rows_longer_than_a_block_keeps(cuda, L, B, nkv, T, lengths):
+    """More keys in a block's stretch than its shared memory holds: those behind are read again, with ties on both sides."""
+    k, v, w = _layers(6, L, B, nkv, T, 8, torch.float16)
+    w.copy_((w * 5).floor() / 4)
+    _check_evict(cuda, k, v, w, lengths, T // 2, 1000)
+    k, v, w = _layers(7, L, B, nkv, T, 8, torch.float16)
+    _check_evict(cuda, k, v, w, lengths, T - 6000, 3)
