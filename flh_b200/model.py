@@ -148,12 +148,14 @@ class DecoderLayer(torch.nn.Module):
     def _attend_drafted(self, qkv, cache, tables, draft):
         """Attention of drafted tokens behind sequences of their own lengths (Decoder.draft): [B, S, heads * D]."""
         lengths, positions, bits = draft
-        q = _CUDA.rope_kv_at(qkv.view(-1, qkv.shape[-1]), tables[0], tables[1], positions, lengths, cache[0], cache[1], self.nh)
-        S, weights = q.shape[1], cache[3] if len(cache) > 3 else None
-        if weights is not None and S > 1:                # what these tokens look at counts when they are accepted (Decoder.accept)
-            cache.drafted[:, :S].copy_(q)
-            weights = None
-        att = _CUDA.tree_attention(q, cache[0], cache[1], lengths, tree=bits, weights=weights)
+        with timing.region("glue"):
+            q = _CUDA.rope_kv_at(qkv.view(-1, qkv.shape[-1]), tables[0], tables[1], positions, lengths, cache[0], cache[1], self.nh)
+            S, weights = q.shape[1], cache[3] if len(cache) > 3 else None
+            if weights is not None and S > 1:            # what these tokens look at counts when they are accepted (Decoder.accept)
+                cache.drafted[:, :S].copy_(q)
+                weights = None
+        with timing.region("attention"):
+            att = _CUDA.tree_attention(q, cache[0], cache[1], lengths, tree=bits, weights=weights)
         return att.view(qkv.shape[0], qkv.shape[1], -1)
 
     def forward(self, x, pos, cache=None, tables=None, shape=None, pre=None, next_layer=None, draft=None):
@@ -185,8 +187,7 @@ class DecoderLayer(torch.nn.Module):
             z = None if z is None else z.view(B, S, -1)
         qkv = self.qkv(q, s, z)
         if draft is not None:
-            with timing.region("attention"):
-                att = self._attend_drafted(qkv, cache, tables, draft)
+            att = self._attend_drafted(qkv, cache, tables, draft)
             return self._after_attention(x, att, sp, blocks if sp else None, next_layer)
         with timing.region("glue"):
             mask, causal = None, S > 1
@@ -204,9 +205,6 @@ class DecoderLayer(torch.nn.Module):
                 # q stays in token order: the attention output follows its layout and needs no transposing copy
                 qh = torch.empty((B, S, self.nh, hd), dtype=qkv.dtype, device=qkv.device)
                 _CUDA.rope_kv(qkv.view(B * S, -1), tables[0], tables[1], qh, kc, vc, B, S, self.nh, self.nkv, cur, q_by_token=True)
-                if observe:
-                    last = min(S, 64)
-                    seen = _CUDA.tree_attention(qh[:, S - last:], kc, vc, torch.full((B,), cur + S - last, dtype=torch.int32, device=x.device), weights=cache[3])
                 qh = qh.transpose(1, 2)
                 kh, vh = kc[:, :, :cur + S], vc[:, :, :cur + S]
             else:
@@ -226,7 +224,10 @@ class DecoderLayer(torch.nn.Module):
                 # triangle with the top-left corner, which is only right for cur = 0)
                 mask, causal = torch.ones(S, cur + S, dtype=torch.bool, device=x.device).tril(diagonal=cur), False
         with timing.region("attention"):
-            if observe and S <= 64:
+            if observe:
+                last = min(S, MAX_TOKENS)
+                seen = _CUDA.tree_attention(qh.transpose(1, 2)[:, S - last:], kc, vc, torch.full((B,), cur + S - last, dtype=torch.int32, device=x.device), weights=cache[3])
+            if observe and S <= MAX_TOKENS:
                 att = seen.view(B, S, self.nh * hd)      # all of the call's tokens: the same attention
             else:
                 att = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=mask, is_causal=causal, enable_gqa=self.nh != self.nkv)

@@ -347,3 +347,23 @@ def test_evicting_by_what_was_accepted(cuda):
         assert torch.equal(ka, kb) and torch.equal(wa, wb)
     with pytest.raises(RuntimeError, match="observe=True"):
         m.draft(_ids(1, 1, 3), [list(c) for c in cache], lengths)
+
+
+def test_attention_is_timed_as_attention(cuda, monkeypatch):
+    import contextlib
+    from flh_b200 import model
+    m, inside, seen = _model(), [], []
+
+    @contextlib.contextmanager
+    def region(name):
+        inside.append(name)
+        yield
+        inside.pop()
+
+    monkeypatch.setattr(model.timing, "region", region)
+    for name in ("tree_attention", "rope_kv", "rope_kv_at"):
+        monkeypatch.setattr(cuda, name, lambda *a, _f=getattr(cuda, name), _n=name, **k: (seen.append((_n, list(inside))), _f(*a, **k))[1])
+    cache = m.new_cache(2, 200, observe=True)
+    m(_ids(1, 2, 80), cache=cache, start=0), m(_ids(2, 2, 5), cache=cache, start=80)
+    m.draft(_ids(3, 2, 4), cache, torch.tensor([85, 85], dtype=torch.int32, device="cuda"))
+    assert {(n, *at) for n, at in seen} == {("tree_attention", "attention"), ("rope_kv", "glue"), ("rope_kv_at", "glue")} and len(seen) == 12
