@@ -234,6 +234,12 @@ __device__ __forceinline__ void take_share(const TreeAttnParams &p, int lane, Jo
     }
 }
 
+// A box of a cache's tensor map [heads, entries, values], from (c2, c1, c0) to shared memory
+__device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+
 // Two values rounded to the tensors' type; one value of it.
 template <bool BF16> __device__ __forceinline__ uint32_t narrow(float lo, float hi) {
     if (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }

@@ -38,10 +38,6 @@ template <int D> constexpr int slot_bytes() { return kTile * D * 2; }
 template <int D> constexpr int q_pitch() { return D * 2 + 16; }                       // bytes; the 16 keep ldmatrix free of conflicts
 template <int D> constexpr int attn_smem() { return 1024 + kWarps * kSlots * slot_bytes<D>() + kRows * q_pitch<D>() + kWarps * 4 * 128 * 4; }
 
-__device__ __forceinline__ void tma_load_tile(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t &a, uint32_t &b, uint32_t &c, uint32_t &d) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(addr) : "memory");
 }

@@ -129,9 +129,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                 if (ok && elect_one()) {
                     mbar_expect_tx(bar, kItem);
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                     ::"r"(dst + h * kHalf), "l"(map), "r"(h * 64), "r"(key0), "r"(head), "r"(bar) : "memory");
+                    for (int h = 0; h < D / 64; ++h) tma_load_tile(dst + h * kHalf, map, h * 64, key0, head, bar);
                 }
                 __syncwarp();
                 item += ok;
@@ -551,8 +549,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
                     mbar_expect_tx(bar, kTileBytes);
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i)
-                        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                                     ::"r"(dst + (i >> 1) * kHalf + (i & 1) * kBox), "l"(&kmap), "r"((i >> 1) * 64), "r"(tile * kWeightTile + (i & 1) * kTreeTcTile), "r"(bh), "r"(bar) : "memory");
+                        tma_load_tile(dst + (i >> 1) * kHalf + (i & 1) * kBox, &kmap, (i >> 1) * 64, tile * kWeightTile + (i & 1) * kTreeTcTile, bh, bar);
                 }
                 __syncwarp();
             }

@@ -5,6 +5,8 @@
 //   * evict_move_kernel     their rows moved together in place.
 // All of them move bytes; what a pass cannot do without is each moved row read once and written once.
 #include "act_common.cuh"
+#include "attn_common.cuh"
+#include "tc_pair.cuh"
 #include <algorithm>
 
 namespace flh {
@@ -26,11 +28,6 @@ struct RopeAtParams {
 template <bool BF16> __device__ __forceinline__ float2 widen2(uint32_t w) {
     if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
-template <bool BF16> __device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
-    if (BF16) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t *>(&h); }
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // One block per token (and part of its heads), a thread takes 16 bytes of the first half of a head and their rotation partners, as in
@@ -59,8 +56,8 @@ __global__ void __launch_bounds__(256) rope_kv_at_kernel(const RopeAtParams p) {
                 const float2 cc = known ? *reinterpret_cast<const float2 *>(ct + 2 * e) : make_float2(nan, nan);
                 const float2 ss = known ? *reinterpret_cast<const float2 *>(st + 2 * e) : make_float2(nan, nan);
                 const float2 x1 = widen2<BF16>(a[e]), x2 = widen2<BF16>(c[e]);
-                a[e] = narrow2<BF16>(__fsub_rn(__fmul_rn(x1.x, cc.x), __fmul_rn(x2.x, ss.x)), __fsub_rn(__fmul_rn(x1.y, cc.y), __fmul_rn(x2.y, ss.y)));
-                c[e] = narrow2<BF16>(__fadd_rn(__fmul_rn(x2.x, cc.x), __fmul_rn(x1.x, ss.x)), __fadd_rn(__fmul_rn(x2.y, cc.y), __fmul_rn(x1.y, ss.y)));
+                a[e] = narrow<BF16>(__fsub_rn(__fmul_rn(x1.x, cc.x), __fmul_rn(x2.x, ss.x)), __fsub_rn(__fmul_rn(x1.y, cc.y), __fmul_rn(x2.y, ss.y)));
+                c[e] = narrow<BF16>(__fadd_rn(__fmul_rn(x2.x, cc.x), __fmul_rn(x1.x, ss.x)), __fadd_rn(__fmul_rn(x2.y, cc.y), __fmul_rn(x1.y, ss.y)));
             }
         }
         uint16_t *dst;
@@ -155,12 +152,7 @@ constexpr int kSelKeys = 45056;            // of a block in shared memory, 176 K
 constexpr int kMaxCluster = 8;
 constexpr int kSelAhead = 4;               // times 32 entries that a warp has under way
 
-__device__ __forceinline__ uint32_t cluster_rank_of() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size_of() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync_of() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // a word of shared memory of another CTA of the cluster, at the place that `local` has in this one
 __device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t rank) {
     uint32_t at, v;
@@ -172,10 +164,10 @@ __device__ __forceinline__ uint32_t peer_u32(const uint32_t *local, uint32_t ran
 // A block per row, or a cluster of blocks that have a stretch of it each.  The smallest key that is kept is found digit by digit, eight
 // bits at a time, by counting the keys that agree with the digits found so far; then the row is walked in order, every warp over a
 // part of its own, and what lies above that key is kept, of the equal ones the first few.  The keys stay in shared memory (cap: how
-// many fit; the rest is read again).  Every lane counts in a histogram of its own, in rows of few keys every second or fourth one, since the histograms have to be cleared
-// and added up for each digit: weights are much alike in their leading bits.  (With 8
-// copies of the counters 256 rows of 8,192 took 31 us, finding the key two bits at a time by comparisons in registers 33, counting
-// equal digits of a warp once 28; this 25.)
+// many fit; the rest is read again).  Every lane counts in a histogram of its own, since weights are much alike in their leading bits;
+// in small caches two or four lanes share one, since the histograms have to be cleared and added up for each digit.  (With 8 copies of
+// the counters 256 rows of 8,192 took 31 us, finding the key two bits at a time by comparisons in registers 33, counting equal digits
+// of a warp once 28; this 25.)
 template <int THREADS, int COPIES>
 __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p, int cap) {
     constexpr int kWarps = THREADS / 32, kLanes = COPIES / 8, kDigits = 256 / kWarps;            // lanes for a digit's counts, digits of a warp
@@ -188,7 +180,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     __shared__ uint32_t found[2];          // prefix, how many of the keys that match it are to be kept
     __shared__ uint32_t above[kWarps], equal[kWarps], sides[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int blocks = cluster_size_of(), rank = cluster_rank_of();
+    const int blocks = cluster_size_of(), rank = cluster_rank();
     const int layer = blockIdx.y, head = blockIdx.x / blocks, b = head / p.nkv;
     pdl_wait();
     pdl_trigger();
@@ -237,7 +229,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
                 if (lane % kLanes == 0) digits[turn][d] = c;
             }
             if (blocks > 1) {
-                cluster_sync_of();
+                cluster_sync_all();
                 for (int i = tid; i < 256; i += THREADS) {
                     uint32_t c = 0;
                     for (int r = 0; r < blocks; ++r) c += peer_u32(&digits[turn][i], r);
@@ -289,7 +281,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
     for (int i = 0; i < warp; ++i) { a0 += above[i]; e0 += equal[i]; }
     if (blocks > 1) {
         if (warp == kWarps - 1 && lane == 0) { sides[0] = a0 + na; sides[1] = e0 + ne; }
-        cluster_sync_of();
+        cluster_sync_all();
         for (int r = 0; r < rank; ++r) { a0 += peer_u32(&sides[0], r); e0 += peer_u32(&sides[1], r); }
     }
     for (int i = from; i < to; i += 32 * kSelAhead) {
@@ -310,7 +302,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
             e0 += __popc(be);
         }
     }
-    if (blocks > 1) cluster_sync_of();     // the others have read this block's counts
+    if (blocks > 1) cluster_sync_all();     // the others have read this block's counts
 }
 
 // Rows kept[0 .. m) of K and V to rows 0 .. m - 1, in place.  kept rises, so kept[d] >= d: rows that a batch writes are read by
@@ -394,7 +386,8 @@ int launch_cache_evict(void *const *k, void *const *v, const float *const *w, in
     p.lengths = lengths; p.kept = kept; p.now = now; p.left = left;
     p.B = B; p.nkv = nkv; p.keep = keep; p.recent = recent; p.chunks = D / 8; p.T = T;
     // One block per row; a cluster of up to 8 where the rows do not fill the GPU and are long (16 rows of 24,000: 29 -> 18 us).  Short rows
-    // take blocks of 256 threads, of which more fit an SM, and rows up to 4,096 half the histograms (32 rows of 2,047: 16.6 -> 15.8 us).
+    // take blocks of 256 threads, of which more fit an SM; caches of up to 4,096 entries half the histograms (32 rows of 2,047 of 2,111
+    // entries 15.7 -> 14.8 us, 256 of 4,090 of 4,096 21.3 -> 19.9).  What counts is the cache's size: the lengths are not known here.
     const long rows = (long)B * nkv * layers;
     int blocks = 1;
     while (blocks < kMaxCluster && rows * blocks * 2 <= kNumSMs && T >= 4096L * blocks) blocks *= 2;
