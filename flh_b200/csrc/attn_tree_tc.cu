@@ -21,6 +21,7 @@
 #include "attn_common.cuh"
 #include "tc_pair.cuh"
 #include "tc_quant_common.cuh"
+#include <type_traits>
 
 namespace flh {
 namespace {
@@ -465,7 +466,8 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
 // rows for its 16 entries, 64 rows x 254,000 entries took 28 us (17 so, of which K's 65 MB are 10).
 constexpr int kWeightTile = 128, kThreadsWeights = 256, kWeightGroup = 8;
 template <int D> constexpr int smem_weights() { return 1024 + (2 * kWeightTile + kRowsTc) * D * 2; }
-template <int D, bool BF16>
+// COUNTED: of p.counted rows only (the number of rows in a register instead of a constant costs 0.5 us).
+template <int D, bool BF16, bool COUNTED>
 __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(const __grid_constant__ TreeAttnParams p, const __grid_constant__ CUtensorMap kmap) {
     constexpr int kTileBytes = kWeightTile * D * 2, kHalf = kWeightTile * 128, kBox = kTreeTcTile * 128;         // a box of the map is 64 entries high
     extern __shared__ uint8_t smem_raw[];
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
     piece_end = min(u1, job.begin + job.nt);
     const int b = job.b, kvh = job.job, bh = b * p.nkv + kvh, len = job.len, n = entries(p, len), first = piece - job.begin, last = piece_end - job.begin;
     // with more rows than 128 a few tiles at a time, so that an entry's sum over all of them is added to its weight once
-    const int rows = counted_rows(p, b), group = rows > kRowsTc ? kWeightGroup : 1 << 20;
+    const int rows = COUNTED ? counted_rows(p, b) : p.R, group = rows > kRowsTc ? kWeightGroup : 1 << 20;
     for (int g0 = first; g0 < last; g0 += group)
     for (int row0 = 0; row0 < rows; row0 += kRowsTc) {
         const int g1 = min(g0 + group, last);
@@ -624,9 +626,9 @@ __global__ void __launch_bounds__(kThreadsWeights, 2) attn_weights_tc_kernel(con
     }
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool COUNTED>
 int launch_weights(const TreeAttnParams &p, const CUtensorMap &km, cudaStream_t stream) {
-    auto kern = attn_weights_tc_kernel<D, BF16>;
+    auto kern = attn_weights_tc_kernel<D, BF16, COUNTED>;
     constexpr int smem = smem_weights<D>();
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kern), smem, done);
@@ -669,8 +671,12 @@ int launch_attn_tc(const TreeAttnParams &p, int rows, bool bf16, const CUtensorM
 }
 
 int launch_attn_weights_tc(const TreeAttnParams &p, bool bf16, const CUtensorMap &km, cudaStream_t stream) {
-    if (p.D == 128) return bf16 ? launch_weights<128, true>(p, km, stream) : launch_weights<128, false>(p, km, stream);
-    return bf16 ? launch_weights<64, true>(p, km, stream) : launch_weights<64, false>(p, km, stream);
+    auto launch = [&](auto counted) {
+        constexpr bool COUNTED = decltype(counted)::value;
+        if (p.D == 128) return bf16 ? launch_weights<128, true, COUNTED>(p, km, stream) : launch_weights<128, false, COUNTED>(p, km, stream);
+        return bf16 ? launch_weights<64, true, COUNTED>(p, km, stream) : launch_weights<64, false, COUNTED>(p, km, stream);
+    };
+    return p.counted ? launch(std::true_type()) : launch(std::false_type());
 }
 
 int attn_tc_status(int *out) { return cuda_status(cudaMemcpyFromSymbol(out, g_status_attn_tc, sizeof(int) * 4), "attn_tc_status"); }

@@ -360,7 +360,7 @@ class Decoder(torch.nn.Module):
         what accept() is told.
         A token whose entry would lie behind the cache's end is not stored and sees less than it should: its logits are NaN.  So are
         those of a token whose position is behind the rotary tables (max_positions or the cache's length); its k is NaN in the cache
-        too, and once accepted makes NaN of all that follows it in its sequence."""
+        too, and once accepted makes NaN of all that follows it in its sequence.  (A sampler that takes no NaN has to leave them out.)"""
         B, S = ids.shape
         # before anything is written: the attention, which comes after the first layer's append, would refuse these
         if not 1 <= S <= MAX_TOKENS or (tree is not None and tree.depth.shape[-1] != S):
