@@ -70,6 +70,14 @@ __device__ __forceinline__ long q_offset(const TreeAttnParams &p, int b, int kvh
 // registers, and a value out of a shuffle or a load is moved there anew for every instruction (measured: 900 clocks for eight MMAs).
 __device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
+// The reference of a row's exponentials: RAISE powers of two below its largest score x, so that the heaviest weight is 2^RAISE.  Where x is so
+// large that its last place is a power of two and more, what the reference is rounded by would push weights over the end of float16: there it
+// is x itself.
+template <int RAISE> __device__ __forceinline__ float reference_of(float x) {
+    if (RAISE == 0) return x;
+    return x - (fabsf(x) < 0x1p22f ? (float)RAISE : 0.0f);
+}
+
 // The drafted entries that a token sees, as bits; those behind the end of the cache do not exist.
 __device__ __forceinline__ uint64_t tree_bits(const TreeAttnParams &p, int b, int s) { return p.tree ? (uint64_t)p.tree[b * p.tree_sb + s] : ~0ull >> (63 - s); }
 __device__ __forceinline__ uint64_t existing_bits(const TreeAttnParams &p, int len) {

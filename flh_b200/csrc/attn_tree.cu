@@ -33,7 +33,7 @@ constexpr int kWarps = 4, kThreadsAttn = kWarps * 32;
 
 constexpr int kRows = 16;                  // of a job
 constexpr int kSlots = 3;                  // ring slots of a warp, so that two CTAs fit an SM; a slot is the K or the V part of a tile
-template <bool BF16> constexpr float kRaise = BF16 ? 0.0f : 14.0f;                     // powers of two that the heaviest weight of a product is
+template <bool BF16> constexpr int kRaise = BF16 ? 0 : 14;                             // powers of two that the heaviest weight of a product is
 template <int D> constexpr int slot_bytes() { return kTile * D * 2; }
 template <int D> constexpr int q_pitch() { return D * 2 + 16; }                       // bytes; the 16 keep ldmatrix free of conflicts
 template <int D> constexpr int attn_smem() { return 1024 + kWarps * kSlots * slot_bytes<D>() + kRows * q_pitch<D>() + kWarps * 4 * 128 * 4; }
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreadsAttn, 2) attn_mma_kernel(const __grid_
                 for (int i = 0; i < kNT; ++i) mx = fmaxf(mx, fmaxf(sc[i][2 * hh], sc[i][2 * hh + 1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                mx = mx * p.scale_log2 - kRaise<BF16>;                       // scale > 0
+                mx = reference_of<kRaise<BF16>>(mx * p.scale_log2);          // scale > 0
                 const float was = m[hh], now = fmaxf(was, mx), base = now == -INFINITY ? 0.0f : now;
                 m[hh] = now;
                 float sum = 0.0f;

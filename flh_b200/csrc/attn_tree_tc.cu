@@ -34,7 +34,7 @@ constexpr int kThreadsTcA = 384;           // warp 0 TMA, warps 1 and 2 MMA, war
 constexpr int kRegsIssue = 112, kRegsSoftmax = 192;
 static_assert(128 * kRegsIssue + 256 * kRegsSoftmax <= kThreadsTcA * 168, "more registers than the CTA was launched with");
 constexpr float kLag = 8.0f;               // powers of two that the true maximum may be ahead of the one that m was taken from
-template <bool BF16> constexpr float kRaise = BF16 ? 0.0f : 7.0f;                      // and that m lies below that one
+template <bool BF16> constexpr int kRaise = BF16 ? 0 : 7;                              // and that m lies below that one
 
 template <int D> constexpr int item_bytes() { return kTileTc * D * 2; }                         // K or V of a tile
 template <int D> constexpr int q_bytes() { return kRowsTc * D * 2; }                            // a block of rows of Q
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kThreadsTcA, 1) attn_tc_kernel(const __grid_co
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int e = 0; e < 64; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[e]));
-                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2 - kRaise<BF16>;
+                    const float mx = reference_of<kRaise<BF16>>(fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2);
                     if (i == 0) m = mx;
                     else if (__any_sync(0xffffffffu, (mx > m + kLag || m == -INFINITY) && mx != m)) {
                         // the product before this one has to be done (the one before that is: these scores were made behind it)

@@ -680,3 +680,23 @@ def test_cache_evict_of_rows_longer_than_a_block_keeps(cuda, L, B, nkv, T, lengt
     _check_evict(cuda, k, v, w, lengths, T // 2, 1000)
     k, v, w = _layers(7, L, B, nkv, T, 8, torch.float16)
     _check_evict(cuda, k, v, w, lengths, T - 6000, 3)
+
+
+@pytest.mark.parametrize("S,nh,nkv", [(2, 4, 2), (8, 8, 2), (64, 8, 1)])
+@pytest.mark.parametrize("k0", [512.0, 2048.0, 4096.0, 8192.0, 16384.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_of_millions(cuda, S, nh, nkv, k0, dtype):
+    """Scores whose last place is 2^-2 .. 8 in powers of two: the entries of the largest one share the weight evenly."""
+    n, D = 700, 64
+    k, v = torch.zeros(1, nkv, n + S, D, device="cuda", dtype=dtype), _normal(3, 1, nkv, n + S, D, dtype=dtype)
+    k[..., 0] = k0
+    k[:, :, ::3, 0] = k0 * 0.75                                                # lower by hundreds of thousands and more: no weight
+    q = torch.zeros(1, S, nh, D, device="cuda", dtype=dtype)
+    q[..., 0] = 4096.0                                                         # products of powers of two: exact
+    out = cuda.tree_attention(q, k, v, _ints([n]), scale=1.0)
+    for s in range(S):
+        at = [t for t in range(n + s + 1) if t % 3]
+        for h in range(nh):
+            x = v[0, h * nkv // nh, at].double()
+            # equal weights, whatever they are rounded to: only the result's rounding and sums of 32 bits
+            R.assert_close(out[0, s, h], x.mean(0), R.HALF_STEP[dtype] * 1.01 * x.mean(0).abs() + (2.02 * R.HALF_STEP[dtype] + 2.0 ** -14) * x.abs().mean(0))
